@@ -5,6 +5,7 @@ parallel) and the objects of a part are linked into that part's shared library n
 
     gemm     _da_gemm.so      matrix products
     token    _da_token.so     norms, embeddings, pooling, RoPE, samplers
+    cache4   _da_cache4.so    4-bit key / value cache: write, read, attention, eviction
     hybrid   _da_hybrid.so    recurrent mixers, paged attention, 32-bit residual stream, fp32 products
     kernels  _da_kernels.so   everything else (attention, vector search, collectives, runtime)
 
@@ -35,7 +36,8 @@ ARCH = os.environ.get("DA_OFFLOAD_ARCH", "gfx950")
 
 _PART_SOURCES = {
     "gemm": ("gemm.hip", "gemm256.hip", "gemm4w.hip", "gemm8p.hip", "gemm_dk.hip"),
-    "token": ("norm.hip", "rope_sample.hip"),
+    "token": ("norm.hip", "rope_sample.hip", "sample_filter.hip"),
+    "cache4": ("cache4.hip",),
     "hybrid": ("delta.hip", "gemm_any.hip", "latent_attn.hip", "paged_attn.hip", "recurrent.hip", "stream_norm.hip"),
 }
 PARTS = (*_PART_SOURCES, "kernels")

@@ -19,6 +19,8 @@ from pathlib import Path
 import numpy as np
 import torch
 
+from .cache4 import SCALE_BYTES, Cache4, new_cache4  # noqa: F401 (the cache's names beside its operators)
+
 _LOCK = threading.Lock()
 # What the rules below choose for a shape, looked up instead of worked out for each product of each layer (2 us each, which
 # an encoder's layers that are launched one by one wait for)
@@ -118,12 +120,22 @@ _SIGS = {
     "da_pool_l2norm_f16": [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "da_topk_dense_ws": [c_int] * 4,
     "da_topk_stream_ws": [c_int] * 4,
+    "da_sample_filtered": [c_void_p] + [c_int] * 4 + [ctypes.c_double] * 3 + [c_int] + [c_void_p] * 5 + [c_uint, c_uint] + [c_void_p] * 10
+                          + [c_int] * 5 + [c_void_p],
+    "da_sample_filtered_ws": [c_int] * 2,
+    "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 9 + [c_int] * 6 + [c_void_p],
+    "da_cache4_read": [c_void_p] * 4 + [c_int] * 6 + [c_void_p] * 3,
+    "da_cache4_evict": [c_void_p] * 9 + [c_int] * 8 + [c_void_p],
+    "da_decode_attn4": [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_float] + [c_void_p] * 3 + [c_int, c_void_p],
+    "da_decode_attn4_ws": [c_int] * 6,
 }
 # the library part (build.py) of each launcher that is not in "kernels"; da_gemm* are in "gemm"
 _PART_OF = {n: "token" for n in (
     "da_quant_fp8_rows", "da_rmsnorm", "da_swiglu_interleaved", "da_layernorm", "da_layernorm_q", "da_layernorm_f16",
     "da_bert_embed_ln", "da_bert_embed_ln_q", "da_bert_embed_ln_f16", "da_embed", "da_pool_l2norm", "da_pool_l2norm_f16",
-    "da_rope_cache", "da_sample", "da_sample_partial", "da_sample_chunked", "da_sample_finalize")}
+    "da_rope_cache", "da_sample", "da_sample_partial", "da_sample_chunked", "da_sample_finalize",
+    "da_sample_filtered", "da_sample_filtered_ws")}
+_PART_OF |= {n: "cache4" for n in _SIGS if n.startswith(("da_cache4", "da_decode_attn4"))}
 
 
 class KernelLibraryMissing(RuntimeError):
@@ -1537,6 +1549,61 @@ def sample(logits, temperature: float, seed: int, step: int = 0, out_tok=None, o
     return out_tok, out_lp
 
 
+SAMPLE_FILTERED_MAX_V = 1 << 18  # entries of a row that sample_filtered takes (csrc/sample_filter.hip, SF_MAX_V)
+
+
+def _row_option(v, B: int, dtype, dev, name: str):
+    """A sampling option as (number for all rows, tensor with each row's)."""
+    if not isinstance(v, torch.Tensor):
+        return v, None
+    _req(v.is_cuda and v.device == dev and v.dtype == dtype and v.is_contiguous() and v.numel() >= B, name + ": one a row, contiguous, beside the logits")
+    return 0, v
+
+
+def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, top_p=1.0, min_p=0.0, u=None, out_tok=None,
+                    out_lp=None, conf=None, active=None, ctr=None, pos=None, lens=None, hist=None, start=None, eos=()):
+    """``sample`` from the entries that top-k, top-p and min-p leave (csrc/sample_filter.hip has the definition): logits [B, V]
+    (bf16 or fp32, rows of any stride, V up to 262144), one uniform number a row. u (fp32 [B], in [0, 1)): those numbers; None: drawn from (seed,
+    ctr or step, row), as ``sample``'s are. temperature, top_p, min_p: numbers, or fp32 [B] on the GPU; top_k: a number, or int32
+    [B]. temperature <= 0: greedy; top_k <= 0, top_p >= 1 and min_p <= 0 are off. Ties go to the lower index, NaN counts as -inf, and a
+    row of nothing else gives token 0 with log-probability -inf. Returns (tokens, logprobs): the untempered, unfiltered
+    distribution's. Bookkeeping as ``sample``'s."""
+    f32 = logits.dtype == torch.float32
+    _req(logits.is_cuda and (f32 or logits.dtype == torch.bfloat16), "logits must be bf16 or fp32 on GPU")
+    B, V = logits.shape
+    dev = logits.device
+    _req(logits.stride(1) == 1 or V == 1, "logits layout")
+    _req(1 <= V <= SAMPLE_FILTERED_MAX_V and 0 <= logits.stride(0) < 1 << 31, "sample_filtered: vocabulary")
+    _same_device(logits)
+    T, Ts = _row_option(temperature, B, torch.float32, dev, "temperature")
+    p, ps = _row_option(top_p, B, torch.float32, dev, "top_p")
+    m, ms = _row_option(min_p, B, torch.float32, dev, "min_p")
+    k, ks = _row_option(top_k, B, torch.int32, dev, "top_k")
+    _row_option(u, B, torch.float32, dev, "u")
+    out_tok = torch.empty(B, dtype=torch.int32, device=dev) if out_tok is None else out_tok
+    out_lp = torch.empty(B, dtype=torch.float32, device=dev) if out_lp is None else out_lp
+    _i32(out_tok, "out_tok"); _req(out_tok.numel() >= B, "out_tok too short")
+    _req(out_lp.is_cuda and out_lp.dtype == torch.float32 and out_lp.is_contiguous() and out_lp.numel() >= B, "out_lp must be fp32 [B]")
+    if conf is not None:
+        _req(conf.is_cuda and conf.dtype == torch.float32 and conf.is_contiguous() and conf.shape == (B, 2), "conf must be fp32 [B, 2]")
+    for t in (active, ctr, pos, lens, start):
+        if t is not None:
+            _i32(t, "bookkeeping"); _req(t.numel() >= B, "bookkeeping: one a row")
+    hist_ld = 0
+    if hist is not None:
+        _i32(hist, "hist"); _req(hist.dim() == 2 and hist.shape[0] >= B, "hist [B, n]")
+        _req(pos is not None and start is not None, "hist needs pos and start")
+        hist_ld = hist.shape[1]
+    e = list(eos)[:4] + [-1] * (4 - min(4, len(eos)))
+    L = lib()
+    ws = _call_scratch(L.da_sample_filtered_ws(B, V), logits)
+    _check(L.da_sample_filtered(_at(logits), f32, B, V, logits.stride(0), T, p, m, max(0, min(int(k), V)), _at(Ts), _at(ps), _at(ms),
+                                _at(ks), _at(u), seed & 0xffffffff, step & 0xffffffff, _at(ctr), _at(ws), _at(out_tok),
+                                _at(out_lp), _at(conf), _at(active), _at(pos), _at(lens), _at(hist), _at(start), hist_ld, *e,
+                                _raw_stream()), "sample_filtered")
+    return out_tok, out_lp
+
+
 def sample_partial(logits, temperature: float, seed: int, v0: int, step: int = 0, ctr=None, out=None):
     """Vocab-parallel sampling, rank side: logits [B, Vl] of the vocabulary slice starting at global
     index v0 -> stats fp32 [B, 8] = (best Gumbel score, best global index as int bits, local max,
@@ -1891,3 +1958,149 @@ def pool_l2norm_f16(h, cu_seqlens, mode: int = 0, out32=None, out16=None):
 from .seq_kernels import (causal_conv, delta_rule, delta_step, delta_step_fits, gated_scan, gemm_any, gemm_heads,  # noqa: E402,F401
                           gemm_partials, latent_attn, latent_flash, latent_flash_fits, latent_gather, latent_prep, partials_fit, rglru_gates,
                           selective_scan, sigmoid_attn, stream_add, stream_final, stream_step)
+
+
+# --------------------------------------------------------------------------- 4-bit key / value cache
+def _cache4(c, Hkv: int, layers: bool = False):
+    """(head dim, slots, max_seq) of a 4-bit cache (one layer's; ``layers``: with the layers in front)."""
+    k, ks, v, vs = c
+    dims = 4 + layers
+    _req(all(t.is_cuda and t.dtype == torch.uint8 and t.is_contiguous() and t.device == k.device for t in c), "cache4: contiguous uint8 on one GPU")
+    _req(k.dim() == dims and k.shape == v.shape and ks.shape == vs.shape == (*k.shape[:-1], SCALE_BYTES), "cache4: codes [slots, Hkv, max_seq, D / 2], scales [.., 4]")
+    D = 2 * k.shape[-1]
+    _req(D in (64, 96, 128), "cache4: head dim 64, 96 or 128")
+    _req(k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0 and ks.data_ptr() % 4 == 0 and vs.data_ptr() % 4 == 0, "cache4: alignment")
+    _req(k.shape[-3] == Hkv and max(k.shape) < 1 << 31, "cache4: KV heads")
+    return D, k.shape[-4], k.shape[-2]
+
+
+def _weight4(weight, c):
+    _req(weight.is_cuda and weight.dtype == torch.float32 and weight.is_contiguous() and weight.shape == c.k.shape[:-1]
+         and weight.device == c.k.device, "weight: contiguous fp32 [slots, Hkv, max_seq] beside its cache")
+
+
+def _rows16(t, name: str, width: int):
+    _bf16_cuda(t, name)
+    _req(t.dim() == 2 and t.shape[1] == width and (t.shape[0] == 1 or (t.stride(0) % 8 == 0 and width <= t.stride(0) < 1 << 31))
+         and t.stride(1) == 1 and t.data_ptr() % 16 == 0, name + ": rows of 16-byte pieces")
+
+
+def _places(T: int, *places):
+    for t in places:
+        _i32(t, "places"); _req(t.numel() >= T, "places: one a token")
+
+
+def cache4_write(k, v, c: Cache4, slot, at, weight=None) -> None:
+    """Keys and values k, v [T, Hkv * D] (bf16, rows of any stride) of T tokens into places ``at`` of slots ``slot`` (int32 [T])
+    of a 4-bit cache, rounded to the nearest code (ties to even). One token a place; a token whose place lies outside the cache
+    is not written. weight (fp32 [slots, Hkv, max_seq]): a written key's accumulated weight begins at 0."""
+    Hkv = c.k.shape[-3]
+    D, slots, max_seq = _cache4(c, Hkv)
+    _rows16(k, "k", Hkv * D); _rows16(v, "v", Hkv * D)
+    T = k.shape[0]
+    _req(v.shape[0] == T, "k and v: the same tokens")
+    _places(T, slot, at)
+    if weight is not None:
+        _weight4(weight, c)
+    _same_device(c.k, k, v, slot, at)
+    _check(lib().da_cache4_write(None, _at(k), _at(v), k.stride(0), v.stride(0), _at(slot), _at(at), None, None, *map(_at, c),
+                                 _at(weight), T, 0, Hkv, D, slots, max_seq, _raw_stream()), "cache4_write")
+
+
+def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4, weight=None):
+    """``rope_cache`` with a 4-bit cache: q and k heads of qkv [T, (H + 2 Hkv) * D] rotated in place (by position ``pos``), k
+    and v written as ``cache4_write`` writes them, to places ``at`` (which are not the positions once keys have been evicted)."""
+    Dc, slots, max_seq = _cache4(c, Hkv)
+    _bf16_cuda(qkv, "qkv"); _i32(pos, "pos")
+    T = qkv.shape[0]
+    _req(Dc == D and qkv.is_contiguous() and qkv.shape[1] == (H + 2 * Hkv) * D and qkv.data_ptr() % 16 == 0, "qkv shape")
+    _req(cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[-1] == 2 and cos_sin.shape[1] == D // 2,
+         "cos_sin must be fp32 [max_pos, D/2, 2]")
+    _places(T, pos, slot, at)
+    if weight is not None:
+        _weight4(weight, c)
+    _same_device(c.k, qkv, pos, slot, at, cos_sin)
+    q = qkv.data_ptr()
+    _check(lib().da_cache4_write(q, q + 2 * H * D, q + 2 * (H + Hkv) * D, qkv.shape[1], qkv.shape[1], _at(slot), _at(at), _at(pos),
+                                 _at(cos_sin), *map(_at, c), _at(weight), T, H, Hkv, D, slots, max_seq, _raw_stream()), "rope_cache4")
+    return qkv
+
+
+def cache4_read(c: Cache4, slot: int, n: int):
+    """The first n keys and values of a slot as bf16 [Hkv, n, D] (exact: what the codes stand for)."""
+    Hkv = c.k.shape[-3]
+    D, slots, max_seq = _cache4(c, Hkv)
+    _req(0 <= slot < slots and 0 <= n <= max_seq, "cache4_read: outside the cache")
+    _same_device(c.k)
+    k, v = torch.empty((2, Hkv, n, D), dtype=torch.bfloat16, device=c.k.device)
+    _check(lib().da_cache4_read(*map(_at, c), Hkv, D, slots, max_seq, slot, n, _at(k), _at(v), _raw_stream()), "cache4_read")
+    return k, v
+
+
+def _same_device(*ts):
+    """Launches go to the current device's stream: tensors of another device are refused."""
+    dev = torch._C._cuda_getDevice()
+    for t in ts:
+        _req(t.get_device() == dev, "tensors must be on the current device")
+
+
+@_rule
+def _attn4_split(B: int, Hkv: int, max_len: int) -> int:
+    """Splits of a row's keys: some 4 workgroups a CU, but 256 keys a split at least."""
+    return max(1, min(-(-1024 // (B * Hkv)), -(-max_len // 256)))
+
+
+def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: int, scale=None, out=None, pre=None, weight=None):
+    """``decode_attn`` over a 4-bit cache: q [B, >= H * D], lens / slot int32 [B], max_len >= every length (host int: fixes the
+    split count, so that the launch is graph-capturable). A row of length 0 gives zeros. Up to 16 query heads on a KV head.
+    pre (int32 [B, 2]: P, slot; P % 64 == 0): the keys [0, P) of a row are those of another slot.
+    weight (fp32 [slots, Hkv, max_seq]; not with pre): each key's probability, summed over the query heads of its KV head, is
+    added to it (what ``cache4_evict`` goes by). Rows then have slots of their own."""
+    Dc, slots, max_seq = _cache4(c, Hkv)
+    _bf16_cuda(q, "q"); _i32(lens, "lens"); _i32(slot, "slot")
+    B = q.shape[0]
+    _req(Dc == D and H % Hkv == 0 and H // Hkv <= 16, "decode_attn4: head dim, query heads")
+    _req(q.dim() == 2 and q.shape[1] >= H * D and q.stride(1) == 1 and (B <= 1 or q.stride(0) % 8 == 0) and q.data_ptr() % 16 == 0, "q layout")
+    _req(lens.numel() >= B and slot.numel() >= B and 1 <= max_len <= max_seq, "lens / slot / max_len")
+    _same_device(c.k, q, lens, slot)
+    if pre is not None:
+        _i32(pre, "pre"); _req(pre.shape == (B, 2) and weight is None, "pre must be int32 [B, 2], without weight")
+    if weight is not None:
+        _weight4(weight, c)
+    if out is None:
+        out = q.new_empty((B, H * D))
+    _req(out.dtype == torch.bfloat16 and out.shape == (B, H * D) and out.stride(1) == 1 and out.device == q.device, "bad out")
+    if B == 0:
+        return out
+    nsplit = _attn4_split(B, Hkv, max_len)
+    L = lib()
+    ws = _call_scratch(L.da_decode_attn4_ws(B, H, D, max_len, nsplit, weight is not None), q)
+    _check(L.da_decode_attn4(_at(q), q.stride(0), *map(_at, c), _at(lens), _at(slot), _at(pre), B, H, Hkv, D, slots, max_seq, max_len,
+                             nsplit, scale if scale is not None else D ** -0.5, _at(ws), _at(weight), _at(out), out.stride(0),
+                             _raw_stream()), "decode_attn4")
+    return out
+
+
+def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None, out=None):
+    """Shorten sequences of more than ``keep`` keys to that many: each KV head of each layer keeps the ``recent`` last keys and of
+    the others those of largest accumulated ``weight`` (fp32 [layers,] slots, Hkv, max_seq; equal ones: the earlier; NaN least),
+    in their order, with their weights. lens / slot int32 [B]; the kept rows go to the front of the same slot, or of slots ``to``
+    (then shorter sequences are copied too). What lies behind them is left as it was. Slots, and those of ``to``, are distinct.
+    c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: not lens itself)."""
+    Hkv = c.k.shape[-3]
+    layered = c.k.dim() == 5
+    D, slots, max_seq = _cache4(c, Hkv, layered)
+    _weight4(weight, c)
+    _i32(lens, "lens"); _i32(slot, "slot")
+    B = lens.numel()
+    _req(slot.numel() >= B and 0 <= recent <= keep, "lens / slot, 0 <= recent <= keep")
+    if to is None:
+        to = slot
+    _i32(to, "to"); _req(to.numel() >= B, "to: one a row")
+    _same_device(c.k, lens, slot, to)
+    if out is None:
+        out = torch.empty_like(lens)
+    _i32(out, "out"); _req(out.numel() >= B and out.data_ptr() != lens.data_ptr(), "out: int32 [B] apart from lens")
+    _check(lib().da_cache4_evict(*map(_at, c), _at(weight), _at(lens), _at(slot), _at(to), _at(out), c.k.shape[0] if layered else 1, B,
+                                 Hkv, D, slots, max_seq, min(keep, max_seq), min(recent, max_seq), _raw_stream()), "cache4_evict")
+    return out

@@ -12,6 +12,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from .cache4 import MAGNITUDES, SCALE_BYTES, Cache4, new_cache4  # noqa: F401
+
 EPI_NONE, EPI_BIAS, EPI_GELU, EPI_SWIGLU, EPI_RESID = 0, 1, 2, 3, 4
 EPI_ROPE = 6  # gemm8p only: QKV + RoPE + KV-cache write
 EPI_REGLU = 7  # EPI_SWIGLU with relu in place of silu
@@ -334,6 +336,42 @@ def sample(logits, temperature, seed, step=0, out_tok=None, out_lp=None, conf=No
     return _bookkeep(B, tok.int(), chosen, logits.device, out_tok, out_lp, conf, active, pos, lens, hist, start, eos)
 
 
+def sample_filtered(logits, temperature, seed=0, step=0, top_k=0, top_p=1.0, min_p=0.0, u=None, out_tok=None, out_lp=None,
+                    conf=None, active=None, ctr=None, pos=None, lens=None, hist=None, start=None, eos=()):
+    """See ops.kernels.sample_filtered: row by row, in 64 bits."""
+    B, V = logits.shape
+    if u is None:
+        u = torch.from_numpy(gumbel_u01(seed, _rkeys(B, step, ctr), 0))
+    of = lambda v, b: float(v[b]) if isinstance(v, torch.Tensor) else float(v)  # noqa: E731
+    x = logits.double().cpu()
+    x = torch.where(x.isnan(), torch.full_like(x, -math.inf), x)
+    tok, chosen = torch.zeros(B, dtype=torch.int32), torch.zeros(B)
+    for b in range(B):
+        z, order = x[b].sort(descending=True, stable=True)
+        if z[0] == -math.inf:
+            chosen[b] = -math.inf
+            continue
+        T, k, p, m = of(temperature, b), int(of(top_k, b)), of(top_p, b), of(min_p, b)
+        d = torch.where(z == z[0], torch.zeros_like(z), z - z[0])  # (z may be inf)
+        n = 1
+        if T > 0:
+            w = torch.exp(d / T)
+            C = w.cumsum(0)
+            n = n_k = k if 0 < k < V else V
+            if p < 1:
+                n = min(n, int((C < p * C[n_k - 1]).sum()) + 1)
+            if m > 0:
+                n = min(n, int((w >= m).sum()))
+            n = max(n, 1)
+        else:
+            C = torch.ones(1, dtype=torch.float64)
+        at = min(int((C[:n] <= float(u[b]) * C[n - 1]).sum()), n - 1)
+        tok[b] = order[at]
+        chosen[b] = d[at] - torch.log1p(torch.exp(d[1:]).sum())
+    return _bookkeep(B, tok.to(logits.device), chosen.to(logits.device), logits.device, out_tok, out_lp, conf, active, pos, lens,
+                     hist, start, eos)
+
+
 def sample_partial(logits, temperature, seed, v0, step=0, ctr=None, out=None):
     """Vocab-parallel sampling, rank side (see ops.kernels.sample_partial): stats fp32 [B, 8]."""
     B, V = logits.shape
@@ -579,3 +617,104 @@ def encoder_layers_fit(rows: int) -> bool:
 from .seq_reference import (causal_conv, delta_rule, delta_step, delta_step_fits, gated_scan, gemm_any,  # noqa: E402,F401
                             gemm_heads, gemm_partials, latent_attn, latent_flash_fits, latent_prep, partials_fit, rglru_gates, selective_scan,
                             sigmoid_attn, stream_add, stream_final, stream_step)
+
+
+# ----------------------------------------------------------------------- 4-bit key / value cache
+def _encode4(x):
+    """[..., D] -> (codes [..., D / 2], scales [..., 4]); csrc/cache4.hip has the format."""
+    D = x.shape[-1]
+    b = x.float().unflatten(-1, (D // 32, 32))
+    bits = b.abs().amax(-1).view(torch.int32)
+    e = (((bits + 0x200000) >> 23) - 2).clamp(min=1)
+    bad = (bits >> 23) >= 255
+    y = (b.double() * torch.exp2(127.0 - e.double()).unsqueeze(-1)).abs()
+    # the nearest magnitude, ties to the even code
+    mid = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64, device=x.device)
+    up, down = torch.bucketize(y, mid, right=True), torch.bucketize(y, mid)
+    code = torch.where(up % 2 == 0, up, down) | (torch.signbit(b).long() << 3)
+    code = code.masked_fill(bad.unsqueeze(-1), 0).flatten(-2).to(torch.uint8)
+    scales = torch.zeros((*x.shape[:-1], SCALE_BYTES), dtype=torch.uint8, device=x.device)
+    scales[..., :D // 32] = e.masked_fill(bad, 255).to(torch.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scales
+
+
+def _decode4(codes, scales, dtype=torch.float32):
+    D = 2 * codes.shape[-1]
+    lut = torch.tensor([*MAGNITUDES, *(-v for v in MAGNITUDES)], dtype=dtype, device=codes.device)
+    s = scales[..., :D // 32]
+    f = torch.exp2(s.to(dtype) - 127).masked_fill(s == 255, float("nan"))
+    x = lut[torch.stack((codes & 15, codes >> 4), -1).flatten(-2).long()]
+    return (x.unflatten(-1, (D // 32, 32)) * f.unsqueeze(-1)).flatten(-2)
+
+
+def cache4_write(k, v, c, slot, at, weight=None):
+    D, T = 2 * c.k.shape[-1], k.shape[0]
+    slots, Hkv, max_seq = c.k.shape[-4:-1]
+    s, a = slot[:T].long(), at[:T].long()
+    ok = (s >= 0) & (s < slots) & (a >= 0) & (a < max_seq)
+    s, a = s[ok], a[ok]
+    for x, codes, scales in ((k, c.k, c.k_scale), (v, c.v, c.v_scale)):
+        new, sc = _encode4(x[ok].reshape(-1, Hkv, D))
+        codes[s, :, a], scales[s, :, a, :D // 32] = new, sc[..., :D // 32]
+    if weight is not None:
+        weight[s, :, a] = 0.0
+
+
+def rope_cache4(qkv, pos, cos_sin, H, Hkv, D, slot, at, c, weight=None):
+    rope_cache(qkv, pos, cos_sin, H, Hkv, D)
+    cache4_write(qkv[:, H * D:(H + Hkv) * D], qkv[:, (H + Hkv) * D:], c, slot, at, weight)
+    return qkv
+
+
+def cache4_read(c, slot: int, n: int):
+    return tuple(_decode4(codes[slot, :, :n], scales[slot, :, :n]).bfloat16() for codes, scales in ((c.k, c.k_scale), (c.v, c.v_scale)))
+
+
+def decode_attn4(q, c, lens, slot, H, Hkv, D, max_len=None, scale=None, out=None, pre=None, weight=None, dtype=torch.float32):
+    B, G = q.shape[0], H // Hkv
+    scale = scale if scale is not None else D ** -0.5
+    res = torch.zeros((B, H * D), dtype=q.dtype if dtype == torch.float32 else dtype, device=q.device)
+    for b in range(B):
+        L, s = int(lens[b]), int(slot[b])
+        if L <= 0 or not 0 <= s < c.k.shape[0]:
+            continue
+        kv = []
+        for codes, scales in ((c.k, c.k_scale), (c.v, c.v_scale)):
+            x = _decode4(codes[s, :, :L], scales[s, :, :L], dtype)
+            if pre is not None and int(pre[b, 0]) > 0:
+                P, ps = int(pre[b, 0]), int(pre[b, 1])
+                x[:, :P] = _decode4(codes[ps, :, :P], scales[ps, :, :P], dtype)
+            kv.append(x)
+        p = (q[b, :H * D].to(dtype).view(Hkv, G, D) @ kv[0].transpose(1, 2) * scale).softmax(-1)
+        res[b] = (p @ kv[1]).reshape(H * D).to(res.dtype)
+        if weight is not None:
+            weight[s, :, :L] += p.sum(1).to(weight.dtype)
+    if out is not None:
+        out.copy_(res)
+        return out
+    return res
+
+
+def cache4_evict(c, weight, lens, slot, keep: int, recent: int, to=None, out=None):
+    layered = c.k.dim() == 5
+    out = torch.empty_like(lens) if out is None else out
+    to = slot if to is None else to
+    for b in range(lens.numel()):
+        n, s, d = int(lens[b]), int(slot[b]), int(to[b])
+        out[b] = min(n, keep)
+        for layer in range(c.k.shape[0] if layered else 1):
+            w = (weight[layer] if layered else weight)
+            one = c.layer(layer) if layered else c
+            for h in range(c.k.shape[-3]):
+                pick = torch.arange(n, device=w.device)
+                if n > keep:
+                    m = n - recent
+                    x = w[s, h, :m]
+                    x = torch.where(x.isnan(), torch.full_like(x, float("-inf")), x)
+                    # NaN least: behind the others of weight -inf
+                    order = torch.argsort(x, descending=True, stable=True)
+                    order = torch.cat((order[~w[s, h, :m][order].isnan()], order[w[s, h, :m][order].isnan()]))
+                    pick = torch.cat((order[:keep - recent].sort()[0], pick[m:]))
+                for t in (*one, w):
+                    t[d, h, :len(pick)] = t[s, h, pick].clone()
+    return out
