@@ -23,8 +23,7 @@ __device__ __forceinline__ unsigned bf2_of4(unsigned w, float scale) {
 }
 
 __device__ __forceinline__ float scale_of(unsigned bytes, int at) {
-  const unsigned s = (bytes >> (8 * at)) & 255;
-  return __uint_as_float(s == 255 ? 0x7fc00000u : s << 23);
+  return __uint_as_float(((bytes >> (8 * at)) & 255) << 23);  // (the conversion takes the exponent; 255 gives NaN)
 }
 
 __device__ __forceinline__ long row_of(const Cache4& c, int slot, int h, int at) {
@@ -135,97 +134,240 @@ DA_EXPORT int da_cache4_read(void* ck, void* cks, void* cv, void* cvs, int Hkv, 
 }
 
 // ------------------------------------------------------------------------------------------- attention
-// One new token a sequence. The G query heads of a KV head are the columns of the products (16, zeros behind G): per 32 keys
-//   S^T[key][g] = K Q^T     A: lane (c, f) has key c and its chunks of 8 elements f CH .. f CH + CH - 1 (CH = D / 32 steps)
-//   O^T[d][g] += V^T P^T    B: P^T straight from S^T's registers (slot j of lane group f is key 16 (j >> 2) + 4 f + (j & 3));
-//                           A: lane (c, f) has the D / 16 elements (D / 16) c .. of those 8 keys, as bytes of two elements,
-//                           and row c of tile i is element (D / 16) c + i
-// so that the order in which a product takes its elements and keys is that of the bytes in memory and nothing is transposed.
+// One new token a sequence. The G query heads of a KV head are the columns of the products (16, zeros behind G): per 16 keys
+//   S^T[key][g] = K Q^T     A: lane (c, f) has chunks f CH .. f CH + CH - 1 of 8 elements (CH = D / 32 steps) of row c, which
+//                           is key 4 (c & 3) + (c >> 2)
+// so that lane (g, f) has the scores of keys 4 i + f (i = 0 .. 3), and per 32 keys
+//   O^T[d][g] += V^T P^T    B: P^T straight from S^T's registers; A: lane (c, f) has the D / 16 elements (D / 16) c .. of those
+//                           8 keys, as bytes of two elements, and row c of tile i is element (D / 16) c + i
+// The order in which a product takes its elements and keys is that of the bytes in memory: nothing is transposed, and the
+// keys' order spreads a wave's reads of V over all LDS banks.
+// A wave walks 64 keys at a time, copied by LDS-DMA (1 KiB an instruction, rows past the end are zeros) into two places of its
+// own: a place is filled again as soon as its codes are in registers, with counted waits and no barrier.
 struct Attn4 {
   const bf16_t* q;
   int ldq;
   Cache4 c;
   const int *lens, *slot, *pre;
-  int B, H, max_len, nsplit, ldo;
+  int B, H, max_len, nsplit, keys, ldo;
   float scale_log2e;
   float *po, *pm, *pl;  // of the splits
-  float* sc;            // scores [B, H, ld_sc] (log2), or null
+  float* sc;            // scores [B, H, ld_sc] (log2; 16 keys as 4 f + i for 4 i + f), or null
   int ld_sc;
   float* weight;
   bf16_t* out;
+  int* cnt;  // tickets [B, Hkv], 0 between launches: the last split of a row's KV head joins them; null: another launch does
 };
 
-constexpr int A4_KEYS = 256;  // keys that a split takes at least
-
-__device__ __forceinline__ int splits4(int L, int nsplit) { return min(nsplit, max(1, (L + A4_KEYS - 1) / A4_KEYS)); }
+// A row's keys evenly over as many splits as hold `keys` of them each: splits of one size whatever the rows' lengths
+__device__ __forceinline__ int splits4(const Attn4& a, int L) { return min(a.nsplit, max(1, (L + a.keys - 1) / a.keys)); }
 
 __device__ __forceinline__ int len4(const Attn4& a, int b) {
   const int s = a.slot[b];
-  return (unsigned)s < (unsigned)a.c.slots ? max(0, min(a.lens[b], a.max_len)) : 0;
+  return __builtin_amdgcn_readfirstlane((unsigned)s < (unsigned)a.c.slots ? max(0, min(a.lens[b], a.max_len)) : 0);
+}
+
+// What splits hand over passes the L2s of the XCDs (agent scope): no fence, only the stores' completion
+__device__ __forceinline__ void put4(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get4(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// One output of a head from its splits' partials, `step` of them beside each other
+template <int D>
+__device__ __forceinline__ void join4(const Attn4& a, long at, int act, int d, int s0, int step, float& M, float& sum, float& acc) {
+  M = -INFINITY, sum = 0.f, acc = 0.f;
+  for (int s = s0; s < act; s += 8 * step) {
+    float ms[8], ls[8], os[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int x = min(s + j * step, act - 1);
+      ms[j] = s + j * step < act ? get4(a.pm + at + x) : -INFINITY;
+      ls[j] = get4(a.pl + at + x);
+      os[j] = get4(a.po + (at + x) * D + d);
+    }
+    float mx = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, ms[j]);
+    if (mx == -INFINITY) continue;
+    const float r = exp2f(M - mx);
+    sum *= r;
+    acc *= r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = exp2f(ms[j] - mx);
+      sum += ls[j] * e;
+      acc += os[j] * e;
+    }
+    M = mx;
+  }
+}
+
+// Reads of a place in LDS as instructions of their own: ahead of an ordinary read hipcc drains the copies that are on their way
+// to the other places. Each waits for itself.
+template <int D>
+__device__ __forceinline__ void read_k4(unsigned at, unsigned at_s, unsigned (&k)[4][D / 32], unsigned (&s)[4]) {
+  if constexpr (D == 128) {
+    u32x4_t x[4];
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\t"
+                 "ds_read_b128 %3, %8 offset:3072\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
+                 "ds_read_b32 %6, %9 offset:128\n\tds_read_b32 %7, %9 offset:192\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+                 : "v"(at), "v"(at_s) : "memory");
+#pragma unroll
+    for (int e = 0; e < 16; ++e) k[e >> 2][e & 3] = x[e >> 2][e & 3];
+  } else if constexpr (D == 64) {
+    u32x2_t x[4];
+    asm volatile("ds_read_b64 %0, %8\n\tds_read_b64 %1, %8 offset:512\n\tds_read_b64 %2, %8 offset:1024\n\t"
+                 "ds_read_b64 %3, %8 offset:1536\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
+                 "ds_read_b32 %6, %9 offset:128\n\tds_read_b32 %7, %9 offset:192\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+                 : "v"(at), "v"(at_s) : "memory");
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e >> 1][e & 1] = x[e >> 1][e & 1];
+  } else {
+    asm volatile("ds_read_b32 %0, %16\n\tds_read_b32 %1, %16 offset:4\n\tds_read_b32 %2, %16 offset:8\n\t"
+                 "ds_read_b32 %3, %16 offset:768\n\tds_read_b32 %4, %16 offset:772\n\tds_read_b32 %5, %16 offset:776\n\t"
+                 "ds_read_b32 %6, %16 offset:1536\n\tds_read_b32 %7, %16 offset:1540\n\tds_read_b32 %8, %16 offset:1544\n\t"
+                 "ds_read_b32 %9, %16 offset:2304\n\tds_read_b32 %10, %16 offset:2308\n\tds_read_b32 %11, %16 offset:2312\n\t"
+                 "ds_read_b32 %12, %17\n\tds_read_b32 %13, %17 offset:64\n\tds_read_b32 %14, %17 offset:128\n\t"
+                 "ds_read_b32 %15, %17 offset:192\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[2][0]),
+                   "=&v"(k[2][1]), "=&v"(k[2][2]), "=&v"(k[3][0]), "=&v"(k[3][1]), "=&v"(k[3][2]), "=&v"(s[0]), "=&v"(s[1]),
+                   "=&v"(s[2]), "=&v"(s[3])
+                 : "v"(at), "v"(at_s) : "memory");
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+#define A4_READ8(op, x, at, o, st)                                                                                          \
+  asm volatile(op " %0, %8 offset:%9\n\t" op " %1, %8 offset:%10\n\t" op " %2, %8 offset:%11\n\t" op " %3, %8 offset:%12\n\t" \
+               op " %4, %8 offset:%13\n\t" op " %5, %8 offset:%14\n\t" op " %6, %8 offset:%15\n\t" op " %7, %8 offset:%16\n\t" \
+               "s_waitcnt lgkmcnt(0)"                                                                                       \
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])      \
+               : "v"(at), "n"(o), "n"(o + 4 * st), "n"(o + 8 * st), "n"(o + 12 * st), "n"(o + 16 * st), "n"(o + 20 * st),   \
+                 "n"(o + 24 * st), "n"(o + 28 * st)                                                                         \
+               : "memory")
+
+// Rows 32 HF + 4 j (+ the lane's f, in the address): slot j is key 16 (j >> 2) + 4 (j & 3) + f
+template <int D, int HF>
+__device__ __forceinline__ void read_v4(unsigned at, unsigned at_s, unsigned (&v)[8], unsigned (&s)[8]) {
+  constexpr int RB = D / 2, O = 32 * HF * RB;
+  if constexpr (D == 64) A4_READ8("ds_read_u16", v, at, O, RB);
+  else A4_READ8("ds_read_b32", v, at, O, RB);
+  A4_READ8("ds_read_b32", s, at_s, 128 * HF, 4);
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 template <int D>
-__global__ void __launch_bounds__(256, 2) decode_attn4_kernel(Attn4 a) {
-  constexpr int CH = D / 32, VB = D / 32, NT = D / 16;
-  __shared__ float so[4][16][D + 1], sm[4][16], sl[4][16];
-  const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = a.H / a.c.Hkv;
-  const int L = len4(a, b), act = splits4(L, a.nsplit);
+__global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
+  constexpr int CH = D / 32, VB = D / 32, NT = D / 16, RB = D / 2, KT = 64;
+  constexpr int ST = 1, ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4, STAGE = 2 * HALF;  // DMA instructions, bytes of K or V
+  typedef __attribute__((address_space(3))) void* lds_t;
+  constexpr int SO = 4 * 16 * (D + 1) * 4, RING = 4 * ST * STAGE;
+  __shared__ __attribute__((aligned(16))) char ring[(SO > RING ? SO : RING) + 16];
+  __shared__ float sm[4][16], sl[4][16];
+  __shared__ int last;
+  const int hk = blockIdx.x, b = blockIdx.y, split = blockIdx.z, G = a.H / a.c.Hkv;
+  const int L = len4(a, b), act = splits4(a, L);
   if (split >= act) return;
-  const int chunk = ((L + act - 1) / act + 127) & ~127;
+  const int chunk = ((L + act - 1) / act + KT - 1) & ~(KT - 1);
   const int kstart = split * chunk, kend = min(L, kstart + chunk);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, f = lane >> 4;
-  const long own = L ? row_of(a.c, a.slot[b], hk, 0) : 0;
-  const int P = a.pre && L ? a.pre[2 * b] : 0;
-  const long head = P ? row_of(a.c, a.pre[2 * b + 1], hk, 0) : own;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, f = lane >> 4;
+  const long own = L ? row_of(a.c, __builtin_amdgcn_readfirstlane(a.slot[b]), hk, 0) : 0;
+  int P = a.pre && L ? __builtin_amdgcn_readfirstlane(a.pre[2 * b]) : 0;
+  long head = own;
+  if (P > 0) {
+    const int s = __builtin_amdgcn_readfirstlane(a.pre[2 * b + 1]);
+    if ((unsigned)s < (unsigned)a.c.slots) head = row_of(a.c, s, hk, 0);
+    else P = 0;
+  }
+  char* mine = ring + w * ST * STAGE;
 
   bf16x8_t qf[CH];
 #pragma unroll
   for (int t = 0; t < CH; ++t)
     qf[t] = c < G ? *(const bf16x8_t*)(a.q + (long)b * a.ldq + (hk * G + c) * D + (f * CH + t) * 8) : bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+
+  // K rows of 64 bytes: the 16-byte pieces of a row are exchanged by its number, so that 16 rows' pieces are in all banks
+  unsigned ko[4];  // (ND of them)
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const unsigned p = i * 64 + lane;
+    ko[i & 3] = D == 128 ? (p & ~3u) * 16 + (((p & 3) ^ ((p >> 4) & 3)) << 4) : p * 16;
+  }
+  auto issue = [&](const uint8_t* codes, const uint8_t* scales, bool swizzled, int t0, char* dst) __attribute__((always_inline)) {
+    const int n = __builtin_amdgcn_readfirstlane(max(0, min(KT, kend - t0)));  // rows (none past kend)
+    const long at = (t0 < P ? head : own) + t0;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(codes + at * RB), (short)0, n * RB, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(scales + at * 4), (short)0, n * 4, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < ND; ++i)  // aux 2: read once a step
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(dst + i * 1024), 16, swizzled ? ko[i & 3] : (i * 64 + lane) * 16, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(dst + KT * RB), 4, lane * 4, 0, 0, 2);
+  };
+  auto landed = [&]() __attribute__((always_inline)) {  // the oldest K or V; the three issued after it may be on their way
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * ST - 1) * PH) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
   f32x4_t o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+  const int kr = 4 * (c & 3) + (c >> 2);  // the lane's key of 16
 
-  for (int t0 = kstart + 32 * w; t0 < kend; t0 += 128) {
-    const long base = t0 < P ? head : own;
-    f32x4_t s[2];
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const long row = base + min(t0 + 16 * tt + c, kend - 1);
-      const unsigned* kp = (const unsigned*)(a.c.k + row * (D / 2)) + f * CH;
-      const unsigned sb = *(const unsigned*)(a.c.ks + row * 4);
+  for (int i = 0; i < ST; ++i) {
+    issue(a.c.k, a.c.ks, true, kstart + (w + 4 * i) * KT, mine + i * STAGE);
+    issue(a.c.v, a.c.vs, false, kstart + (w + 4 * i) * KT, mine + i * STAGE + HALF);
+  }
+#pragma unroll
+  for (int t = 0; t < CH; ++t) asm volatile("" : "+v"(qf[t]));
+  int stage = 0;
+  for (int t0 = kstart + w * KT; t0 < kend; t0 += 4 * KT) {
+    char* kt = mine + stage * STAGE;
+    char* vt = kt + HALF;
+    landed();
+    unsigned kw[4][CH], ks[4];
+    const unsigned kt_at = (unsigned)(size_t)(lds_t)kt;
+    read_k4<D>(kt_at + kr * RB + (D == 128 ? ((f ^ (c & 3)) << 4) : f * CH * 4), kt_at + KT * RB + kr * 4, kw, ks);
+    issue(a.c.k, a.c.ks, true, t0 + 4 * ST * KT, kt);
+    f32x4_t s[4];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
       s[tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < CH; ++t) {
-        const float sc = scale_of(sb, (f * CH + t) >> 2);
-        const u32x4_t kk = {bf2_of4<0>(kp[t], sc), bf2_of4<1>(kp[t], sc), bf2_of4<2>(kp[t], sc), bf2_of4<3>(kp[t], sc)};
+        const float sc = scale_of(ks[tt], (f * CH + t) >> 2);
+        const u32x4_t kk = {bf2_of4<0>(kw[tt][t], sc), bf2_of4<1>(kw[tt][t], sc), bf2_of4<2>(kw[tt][t], sc), bf2_of4<3>(kw[tt][t], sc)};
         s[tt] = mfma16(__builtin_bit_cast(bf16x8_t, kk), qf[t], s[tt]);
       }
     }
     float mx = -INFINITY;
+    const bool whole = t0 + KT <= kend;
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[tt][i] = t0 + 16 * tt + 4 * f + i < kend ? s[tt][i] * a.scale_log2e : -INFINITY;
+        s[tt][i] = whole || t0 + 16 * tt + 4 * i + f < kend ? s[tt][i] * a.scale_log2e : -INFINITY;
         mx = fmaxf(mx, s[tt][i]);
       }
     if (a.sc && c < G) {
       float* to = a.sc + ((long)b * a.H + hk * G + c) * a.ld_sc + t0 + 4 * f;
-      *(f32x4_t*)to = s[0];
-      *(f32x4_t*)(to + 16) = s[1];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) *(f32x4_t*)(to + 16 * tt) = s[tt];
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = max_xhalf(mx);
-    const float mn = fmaxf(m, mx), use = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m - use);
-    m = mn;
-    l *= alpha;
+    if (__ballot(mx > m)) {  // (a new maximum is rare after the first tiles)
+      const float mn = fmaxf(m, mx), alpha = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i] *= alpha;
-    unsigned pw[4];
+      for (int i = 0; i < NT; ++i) o[i] *= alpha;
+    }
+    const float use = m == -INFINITY ? 0.f : m;
+    unsigned pw[8];
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
+    for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - use);
@@ -234,36 +376,48 @@ __global__ void __launch_bounds__(256, 2) decode_attn4_kernel(Attn4 a) {
       pw[2 * tt] = pack_bf2(s[tt][0], s[tt][1]);
       pw[2 * tt + 1] = pack_bf2(s[tt][2], s[tt][3]);
     }
-    const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{pw[0], pw[1], pw[2], pw[3]});
-    unsigned vv[8][VB];  // pairs of elements of 8 keys
+    landed();
+    const unsigned vt_at = (unsigned)(size_t)(lds_t)vt;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const long row = base + min(t0 + 16 * (j >> 2) + 4 * f + (j & 3), kend - 1);
-      const uint8_t* vp = a.c.v + row * (D / 2) + c * VB;
-      const unsigned sb = *(const unsigned*)(a.c.vs + row * 4);
-      unsigned word = 0;
-      __builtin_memcpy(&word, vp, VB);
-      vv[j][0] = bf2_of4<0>(word, scale_of(sb, (c * NT) >> 5));
-      vv[j][1] = bf2_of4<1>(word, scale_of(sb, (c * NT + 2) >> 5));
-      if constexpr (VB > 2) vv[j][2] = bf2_of4<2>(word, scale_of(sb, (c * NT + 4) >> 5));
-      if constexpr (VB > 3) vv[j][3] = bf2_of4<3>(word, scale_of(sb, (c * NT + 6) >> 5));
+    for (int hf = 0; hf < 2; ++hf) {
+      unsigned word[8], vs[8];
+      const unsigned v_at = vt_at + f * RB + c * VB, s_at = vt_at + KT * RB + f * 4;
+      if (hf) {
+        read_v4<D, 1>(v_at, s_at, word, vs);
+        issue(a.c.v, a.c.vs, false, t0 + 4 * ST * KT, vt);
+      } else {
+        read_v4<D, 0>(v_at, s_at, word, vs);
+      }
+      unsigned vv[8][VB];  // pairs of elements of 8 keys
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        vv[j][0] = bf2_of4<0>(word[j], scale_of(vs[j], (c * NT) >> 5));
+        vv[j][1] = bf2_of4<1>(word[j], scale_of(vs[j], (c * NT + 2) >> 5));
+        if constexpr (VB > 2) vv[j][2] = bf2_of4<2>(word[j], scale_of(vs[j], (c * NT + 4) >> 5));
+        if constexpr (VB > 3) vv[j][3] = bf2_of4<3>(word[j], scale_of(vs[j], (c * NT + 6) >> 5));
+      }
+      const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{pw[4 * hf], pw[4 * hf + 1], pw[4 * hf + 2], pw[4 * hf + 3]});
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        u32x4_t va;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          va[e] = __builtin_amdgcn_perm(vv[2 * e + 1][i >> 1], vv[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+        o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pb, o[i]);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      u32x4_t va;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        va[e] = __builtin_amdgcn_perm(vv[2 * e + 1][i >> 1], vv[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
-      o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pb, o[i]);
-    }
+    stage = stage + 1 == ST ? 0 : stage + 1;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (pieces past the end write zeros)
   l += __shfl_xor(l, 16, 64);
   l = sum_xhalf(l);
   if (f == 0) { sm[w][c] = m; sl[w][c] = l; }
+  __syncthreads();  // every wave is done with its places
+  float* so = (float*)ring;  // [4][16][D + 1]
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) so[w][c][NT * (4 * f + r) + i] = o[i][r];
+    for (int r = 0; r < 4; ++r) so[(w * 16 + c) * (D + 1) + NT * (4 * f + r) + i] = o[i][r];
   __syncthreads();
   for (int i = tid; i < G * D; i += 256) {
     const int g = i / D, d = i - g * D;
@@ -272,73 +426,125 @@ __global__ void __launch_bounds__(256, 2) decode_attn4_kernel(Attn4 a) {
 #pragma unroll
     for (int ww = 0; ww < 4; ++ww) {
       const float e = exp2f(sm[ww][g] - use);
-      acc += so[ww][g][d] * e;
+      acc += so[(ww * 16 + g) * (D + 1) + d] * e;
       sum += sl[ww][g] * e;
     }
     const long at = ((long)b * a.H + hk * G + g) * a.nsplit + split;
-    if (a.nsplit == 1) a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(L ? acc / sum : 0.f);
-    else a.po[at * D + d] = acc;
-    if (d == 0) { a.pm[at] = M; a.pl[at] = sum; }
+    if (act == 1) a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(L ? acc / sum : 0.f);
+    else put4(a.po + at * D + d, acc);
+    if (d == 0) { put4(a.pm + at, M); put4(a.pl + at, sum); }
+  }
+  if (act == 1 || !a.cnt) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int* t = a.cnt + b * a.c.Hkv + hk;
+    last = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == act - 1;
+    if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int i = tid; i < G * D; i += 256) {
+    const int g = i / D, d = i - g * D;
+    float M, sum, acc;
+    join4<D>(a, ((long)b * a.H + hk * G + g) * a.nsplit, act, d, 0, 1, M, sum, acc);
+    a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(acc / sum);
   }
 }
 
-// The splits of a head joined, and (weight) its share of each key's weight added: a workgroup per (1024 keys, KV head, row).
+// The second launch of many splits or of weights: workgroup x < G of a row's KV head joins the splits of its head x, the others
+// add the weights of 1024 keys each.
 template <int D>
 __global__ void __launch_bounds__(256) decode_attn4_join_kernel(Attn4 a) {
-  __shared__ float sM[16], sR[16];
-  const int hk = blockIdx.y, b = blockIdx.z, G = a.H / a.c.Hkv, tid = threadIdx.x;
-  const int L = len4(a, b), act = splits4(L, a.nsplit);
-  if (blockIdx.x && (int)blockIdx.x * 1024 >= L) return;
-  if (tid < G) {
-    const long at = ((long)b * a.H + hk * G + tid) * a.nsplit;
+  __shared__ float sM[16], sR[16], part[3][4][D];
+  const int hk = blockIdx.y, b = blockIdx.z, G = a.H / a.c.Hkv, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int L = len4(a, b), act = splits4(a, L);
+  const long first = ((long)b * a.H + hk * G) * a.nsplit;
+  if ((int)blockIdx.x < G) {
+    if (act == 1) return;
+    const int g = blockIdx.x;
+    for (int d = lane; d < D; d += 64) join4<D>(a, first + (long)g * a.nsplit, act, d, w, 4, part[0][w][d], part[1][w][d], part[2][w][d]);
+    __syncthreads();
+    if (tid < D) {
+      const float M = fmaxf(fmaxf(part[0][0][tid], part[0][1][tid]), fmaxf(part[0][2][tid], part[0][3][tid]));
+      float sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = exp2f(part[0][i][tid] - M);
+        sum += part[1][i][tid] * e;
+        acc += part[2][i][tid] * e;
+      }
+      a.out[(long)b * a.ldo + (hk * G + g) * D + tid] = f2bf(acc / sum);
+    }
+    return;
+  }
+  const int k0 = ((int)blockIdx.x - G) * 1024;
+  if (k0 >= L) return;
+  // 4 keys a thread: places 4 f + i of 16 are keys 4 i + f. The scores of 4 heads are on their way beside the sums of the splits
+  const int at = k0 + 4 * tid, key = (at & ~15) + ((at >> 2) & 3);
+  const bool in = key < L;
+  const float* sc = a.sc + ((long)b * a.H + hk * G) * a.ld_sc + at;
+  f32x4_t s[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) s[g] = in ? *(const f32x4_t*)(sc + (long)min(g, G - 1) * a.ld_sc) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int g = tid >> 4; g < G; g += 16) {  // 16 lanes a head
     float M = -INFINITY, sum = 0.f;
-    for (int s = 0; s < act; ++s) M = fmaxf(M, a.pm[at + s]);
-    for (int s = 0; s < act; ++s) sum += a.pl[at + s] * exp2f(a.pm[at + s] - (M == -INFINITY ? 0.f : M));
-    sM[tid] = M == -INFINITY ? 0.f : M;
-    sR[tid] = 1.f / sum;
+    for (int x = tid & 15; x < act; x += 16) {
+      const float m = a.pm[first + (long)g * a.nsplit + x], l = a.pl[first + (long)g * a.nsplit + x], mx = fmaxf(M, m);
+      sum = sum * exp2f(M - mx) + l * exp2f(m - mx);
+      M = mx;
+    }
+    const float mine = M;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 16));
+    sum *= exp2f(mine - M);
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 16);
+    if ((tid & 15) == 0) { sM[g] = M; sR[g] = 1.f / sum; }
   }
   __syncthreads();
-  if (blockIdx.x == 0 && a.nsplit > 1)
-    for (int i = tid; i < G * D; i += 256) {
-      const int g = i / D, d = i - g * D;
-      const long at = ((long)b * a.H + hk * G + g) * a.nsplit;
-      float acc = 0.f;
-      for (int s = 0; s < act; ++s) acc += a.po[(at + s) * D + d] * exp2f(a.pm[at + s] - sM[g]);
-      a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(L ? acc * sR[g] : 0.f);
+  if (!in) return;
+  f32x4_t p = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < G; g0 += 4) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (g0) s[g] = *(const f32x4_t*)(sc + (long)min(g0 + g, G - 1) * a.ld_sc);
+      if (g0 + g < G)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] += exp2f(s[g][i] - sM[g0 + g]) * sR[g0 + g];
     }
-  if (!a.weight) return;
-  float* wt = a.weight + row_of(a.c, a.slot[b], hk, 0);
-  for (int key = blockIdx.x * 1024 + tid; key < min(L, (int)(blockIdx.x + 1) * 1024); key += 256) {
-    float p = 0.f;
-    for (int g = 0; g < G; ++g) p += exp2f(a.sc[((long)b * a.H + hk * G + g) * a.ld_sc + key] - sM[g]) * sR[g];
-    wt[key] += p;
   }
+  float* wt = a.weight + row_of(a.c, a.slot[b], hk, key);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (key + 4 * i < L) wt[4 * i] += p[i];
 }
 
 DA_EXPORT size_t da_decode_attn4_ws(int B, int H, int D, int max_len, int nsplit, int weight) {
-  return 4 * ((size_t)B * H * nsplit * (D + 2) + (weight ? (size_t)B * H * ((max_len + 31) / 32 * 32) : 0));
+  return 4 * ((size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4) + (weight ? (size_t)B * H * ((max_len + 63) / 64 * 64) : 0));
 }
 
 template <int D>
 static int attn4(Attn4& a, hipStream_t st) {
-  decode_attn4_kernel<D><<<dim3(a.nsplit, a.c.Hkv, a.B), 256, 0, st>>>(a);
+  decode_attn4_kernel<D><<<dim3(a.c.Hkv, a.B, a.nsplit), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if (a.nsplit > 1 || a.weight)
-    decode_attn4_join_kernel<D><<<dim3(a.weight ? (a.max_len + 1023) / 1024 : 1, a.c.Hkv, a.B), 256, 0, st>>>(a);
+  if (a.weight || (a.nsplit > 1 && !a.cnt))
+    decode_attn4_join_kernel<D><<<dim3(a.H / a.c.Hkv + (a.weight ? (a.max_len + 1023) / 1024 : 0), a.c.Hkv, a.B), 256, 0, st>>>(a);
   DA_LAUNCH_CHECK();
 }
 
+// counters (ints, B * Hkv of them, 0): the splits are joined in the launch; null (always with weights): in a second one
 DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void* cv, void* cvs, const void* lens, const void* slot,
                               const void* pre, int B, int H, int Hkv, int D, int slots, int max_seq, int max_len, int nsplit,
-                              float scale, void* ws, void* weight, void* out, int ldo, void* stream) {
-  if (Hkv < 1 || H % Hkv || H / Hkv > 16 || max_len < 1 || max_len > max_seq || nsplit < 1 || B > 65535 || Hkv > 65535) return (int)hipErrorInvalidValue;
+                              int keys, float scale, void* ws, void* weight, void* out, int ldo, void* counters, void* stream) {
+  if (Hkv < 1 || H % Hkv || H / Hkv > 16 || max_len < 1 || max_len > max_seq || nsplit < 1 || nsplit > 65535 || keys < 1 || B > 65535) return (int)hipErrorInvalidValue;
   if (B == 0) return 0;
-  const size_t n = (size_t)B * H * nsplit;
+  const size_t n = (size_t)B * H * nsplit, all = (size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4);
   Attn4 a{(const bf16_t*)q, ldq, {(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq},
-          (const int*)lens, (const int*)slot, (const int*)pre, B, H, max_len, nsplit, ldo, scale * 1.44269504f,
-          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), weight ? (float*)ws + n * (D + 2) : nullptr,
-          (max_len + 31) / 32 * 32, (float*)weight, (bf16_t*)out};
+          (const int*)lens, (const int*)slot, (const int*)pre, B, H, max_len, nsplit, keys, ldo, scale * 1.44269504f,
+          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), weight ? (float*)ws + all : nullptr,
+          (max_len + 63) / 64 * 64, (float*)weight, (bf16_t*)out, weight ? nullptr : (int*)counters};
   hipStream_t st = (hipStream_t)stream;
   return D == 64 ? attn4<64>(a, st) : D == 96 ? attn4<96>(a, st) : D == 128 ? attn4<128>(a, st) : (int)hipErrorInvalidValue;
 }

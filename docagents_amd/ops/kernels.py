@@ -126,7 +126,7 @@ _SIGS = {
     "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 9 + [c_int] * 6 + [c_void_p],
     "da_cache4_read": [c_void_p] * 4 + [c_int] * 6 + [c_void_p] * 3,
     "da_cache4_evict": [c_void_p] * 9 + [c_int] * 8 + [c_void_p],
-    "da_decode_attn4": [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_float] + [c_void_p] * 3 + [c_int, c_void_p],
+    "da_decode_attn4": [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 9 + [c_float] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p],
     "da_decode_attn4_ws": [c_int] * 6,
 }
 # the library part (build.py) of each launcher that is not in "kernels"; da_gemm* are in "gemm"
@@ -2044,10 +2044,17 @@ def _same_device(*ts):
         _req(t.get_device() == dev, "tensors must be on the current device")
 
 
+ATTN4_JOINED = (12, 64)  # splits, and partials (splits x query heads of a KV head), that the last split's workgroup joins
+
+
 @_rule
-def _attn4_split(B: int, Hkv: int, max_len: int) -> int:
-    """Splits of a row's keys: some 4 workgroups a CU, but 256 keys a split at least."""
-    return max(1, min(-(-1024 // (B * Hkv)), -(-max_len // 256)))
+def _attn4_split(B: int, Hkv: int, max_len: int):
+    """(splits of the longest row, keys a split): some 6 workgroups a CU, of 256 keys at least, and up to 32 splits a row, whose join
+    costs more than the last CUs' share of the work. us of keys a split, 8 KV heads x 128: 64 rows of 2700 - 8192 keys 512 86 / 1024
+    77 / 2048 76 / 4096 82; 2 of 21000 - 65533 512 41 / 1024 34 / 2048 31 / 4096 32; 24 of 1400 - 4096 with weights 256 32 / 512 30 /
+    1024 31."""
+    keys = max(256, -(-max_len * B * Hkv // 1536 // 64) * 64, -(-max_len // 32 // 64) * 64)
+    return -(-max_len // keys), keys
 
 
 def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: int, scale=None, out=None, pre=None, weight=None):
@@ -2072,12 +2079,16 @@ def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: in
     _req(out.dtype == torch.bfloat16 and out.shape == (B, H * D) and out.stride(1) == 1 and out.device == q.device, "bad out")
     if B == 0:
         return out
-    nsplit = _attn4_split(B, Hkv, max_len)
+    nsplit, keys = _attn4_split(B, Hkv, max_len)
+    stream = _raw_stream()
+    # few partials: the last of a row's splits joins them; else a second launch over all heads does
+    joined = weight is None and 1 < nsplit <= ATTN4_JOINED[0] and nsplit * (H // Hkv) <= ATTN4_JOINED[1] and B * Hkv <= N_COUNTERS
+    cnt = _counters(q.device, stream) if joined else None
     L = lib()
     ws = _call_scratch(L.da_decode_attn4_ws(B, H, D, max_len, nsplit, weight is not None), q)
     _check(L.da_decode_attn4(_at(q), q.stride(0), *map(_at, c), _at(lens), _at(slot), _at(pre), B, H, Hkv, D, slots, max_seq, max_len,
-                             nsplit, scale if scale is not None else D ** -0.5, _at(ws), _at(weight), _at(out), out.stride(0),
-                             _raw_stream()), "decode_attn4")
+                             nsplit, keys, scale if scale is not None else D ** -0.5, _at(ws), _at(weight), _at(out), out.stride(0),
+                             _at(cnt), stream), "decode_attn4")
     return out
 
 
