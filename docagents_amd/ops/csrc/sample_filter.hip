@@ -9,23 +9,24 @@
 // (relative error 2e-13), sums in double or, where they are collected by atomics, in units of 2^-45 (whole numbers: no order
 // changes them).
 //
-// Two launches. The first reads the row once, many workgroups a row: largest entry of each 64 (group), and of each 2048 entries
-// the sums of exp. The second, a workgroup a row, never sorts the row: each filter bounds the kept entries from below before any
-// of them is known,
+// Two launches. The first reads the row once, a wave to 512 entries: the largest entry of each 64 (group) and the sums of exp.
+// The second, a workgroup a row, never sorts the row: each filter bounds the kept entries from below before any of them is known,
 //   top-k  the k-th largest of the groups' largest entries (k groups have an entry as large)
 //   top-p  w >= (1 - p) C(V) / V: entries below it hold less than 1 - p of the mass together
 //   min-p  w >= min_p
-// and only groups whose largest entry passes the bound are read again. Up to CAP entries are sorted in LDS; more of them (flat
-// distributions) are counted into 2048 bins of the ordered 32-bit key, the bin in which a border falls into 2048 of its own,
-// until a bin is one value (three times at most).
+// and only groups whose largest entry passes the bound are read again. Up to CAP entries are sorted in LDS. More of them (flat
+// distributions) are counted into 2048 bins of equal width; a border (of top-k, top-p or u) falls into one bin, and that bin's
+// entries are sorted. If even those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
 #include "common.h"
 #include "sample.h"
 
-constexpr int SF_GROUP = 64, SF_CHUNK = 2048, SF_MAX_V = 1 << 18, SF_CAP = 4096, SF_BINS = 2048;
-constexpr int SF_MAX_GROUPS = SF_MAX_V / SF_GROUP, SF_MAX_CHUNKS = SF_MAX_V / SF_CHUNK;
+constexpr int SF_GROUP = 64, SF_CHUNK = 512, SF_MAX_V = 1 << 18, SF_CAP = 2048, SF_BINS = 2048;
+constexpr int SF_MAX_GROUPS = SF_MAX_V / SF_GROUP;
+static_assert(SF_MAX_V / SF_CHUNK <= 1024 && SF_MAX_GROUPS <= 4096 && SF_CAP <= 2048, "the second launch's 1024 threads");
+typedef unsigned long long u64;
 constexpr double SF_UNIT = 35184372088832.0;  // 2^45: 2^18 weights of 1 fit 64 bits
 
-struct ChunkSum { double zt, z1; float m; int pad; };
+struct ChunkSum { double zt; float rest, m; int n, pad; };  // sums relative to the chunk's largest entry m: n of it, the others' exp
 
 struct FilterArgs {
   double T, p, m;  // of all rows, unless the pointers give each its own
@@ -84,14 +85,37 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return v;
 }
 
+// A wave's reductions on the vector ALU: neighbours, pairs, halves of 8 and of 16 lanes (mirrored), then rows of lanes
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max8(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  return fmaxf(v, dpp<0x141>(v));
+}
+__device__ __forceinline__ float max_8_64(float v) {  // of max8
+  v = fmaxf(v, dpp<0x140>(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_xhalf(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum64(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  v += dpp<0x140>(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return sum_xhalf(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // ------------------------------------------------------------------------------------------- first launch
 template <typename L>
 __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
-  __shared__ float redf[16];
-  __shared__ double redd[2][4];
-  const int b = blockIdx.y, V = a.s.V, tid = threadIdx.x, v0 = blockIdx.x * SF_CHUNK + tid * 8;
+  const int b = blockIdx.y, V = a.s.V, lane = threadIdx.x & 63, chunk = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int NC = (V + SF_CHUNK - 1) / SF_CHUNK, NG = (V + SF_GROUP - 1) / SF_GROUP, v0 = chunk * SF_CHUNK + lane * 8;
+  if (chunk >= NC) return;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
-  const RowOpts o = row_opts(a, b);
   float x[8];
   if (v0 + 8 <= V && (((size_t)(row + v0)) & 15) == 0) {
     if constexpr (sizeof(L) == 2) {
@@ -113,74 +137,52 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     x[e] = entry(x[e]);
     mx = fmaxf(mx, x[e]);
   }
-  float gm = mx;  // a group is 8 lanes
-  gm = fmaxf(gm, __shfl_xor(gm, 1, 64));
-  gm = fmaxf(gm, __shfl_xor(gm, 2, 64));
-  gm = fmaxf(gm, __shfl_xor(gm, 4, 64));
-  const int NG = (V + SF_GROUP - 1) / SF_GROUP;
-  if ((tid & 7) == 0 && v0 < V) a.gmax[(long)b * NG + v0 / SF_GROUP] = key_of(gm);
-  const float top = block_max(mx, redf), use = top == -INFINITY ? 0.f : top;
-  double z1 = 0, zt = 0;
+  mx = max8(mx);  // a group is 8 lanes
+  if ((lane & 7) == 0 && v0 < V) a.gmax[(long)b * NG + v0 / SF_GROUP] = key_of(mx);
+  const float top = max_8_64(mx), use = top == -INFINITY ? 0.f : top;
+  // 2^t with t rounded: 2^-24 |t| of a term, of the log-probability's sum that is
+  float rest = 0.f;
+  int n = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    // exp in fp32 with the product's rounding error put back: 2 ulp for the log-probability's sum
-    const float d = x[e] == use ? 0.f : x[e] - use, t = d * 1.44269504f, lo = fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f;
-    const float q = __builtin_amdgcn_exp2f(t);
-    z1 += t < -150.f ? 0.f : fmaf(q, lo * 0.693147181f, q);
+    const float q = __builtin_amdgcn_exp2f((x[e] - use) * 1.44269504f);
+    const u64 same = __ballot(x[e] == use);
+    n += __popcll(same);
+    rest += x[e] == use ? 0.f : q;
   }
+  rest = sum64(rest);
+  const RowOpts o = row_opts(a, b);
+  double zt = 0;
   if (o.p < 1 && o.k == 0) {
     const double it = 1.0 / o.T;
 #pragma unroll
     for (int e = 0; e < 8; ++e) zt += x[e] == -INFINITY ? 0.0 : weight(x[e], use, it);
+    zt = wave_sum_d(zt);
   }
-  z1 = wave_sum_d(z1);
-  zt = wave_sum_d(zt);
-  if ((tid & 63) == 0) { redd[0][tid >> 6] = z1; redd[1][tid >> 6] = zt; }
-  __syncthreads();
-  if (tid == 0)
-    a.sums[(long)b * gridDim.x + blockIdx.x] = {((redd[1][0] + redd[1][1]) + redd[1][2]) + redd[1][3],
-                                                ((redd[0][0] + redd[0][1]) + redd[0][2]) + redd[0][3], top, 0};
+  if (lane == 0) a.sums[(long)b * NC + chunk] = {zt, rest, top, n, 0};
 }
 
 // ------------------------------------------------------------------------------------------- second launch
-typedef unsigned long long u64;
-
 struct PickLds {
-  u64 list[SF_CAP];  // (key, ~index) of the entries; counted ones: mass[SF_BINS], count[SF_BINS]
+  u64 list[SF_CAP];  // (key, ~index) of entries
   union {
-    double C[SF_CAP];  // of sorted entries
-    struct {           // the groups that pass the bound, and (counted entries) each group's entries of one value
-      unsigned short group[SF_MAX_GROUPS], match[SF_MAX_GROUPS];
-    };
+    double C[SF_CAP];                     // of sorted entries
+    unsigned short match[SF_MAX_GROUPS];  // each listed group's entries of one value
   };
+  u64 mass[SF_BINS];
+  unsigned count[SF_BINS];
+  unsigned short group[SF_MAX_GROUPS];  // the groups that pass the bound
   double redd[2][16];
   unsigned redu[3][16];
   u64 redm[16];
   unsigned kappa, n_group, n_list;
   unsigned bin, c_above, c_at, found;
-  u64 m_above, m_at;
+  u64 m_above;
 };
 
-// The workgroup's inclusive sums over its threads, in order (16 waves)
-__device__ __forceinline__ double scan_d(double v, double* red, double& before) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  double s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(s, o, 64);
-    if (lane >= o) s += t;
-  }
-  __syncthreads();
-  if (lane == 63) red[wv] = s;
-  __syncthreads();
-  double off = 0;
-  for (int i = 0; i < wv; ++i) off += red[i];
-  before = off + (s - v);
-  return off + s;
-}
-
+// The workgroup's sums over its threads, in order (16 waves): before the thread's own
 template <typename T>
-__device__ __forceinline__ T scan_u(T v, T* red) {  // exclusive
+__device__ __forceinline__ T scan_before(T v, T* red) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   T s = v;
 #pragma unroll
@@ -192,8 +194,9 @@ __device__ __forceinline__ T scan_u(T v, T* red) {  // exclusive
   if (lane == 63) red[wv] = s;
   __syncthreads();
   T off = 0;
-  for (int i = 0; i < wv; ++i) off += red[i];
-  return off + s - v;
+#pragma unroll
+  for (int i = 0; i < 15; ++i) off += i < wv ? red[i] : T(0);
+  return off + (s - v);
 }
 
 __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
@@ -203,203 +206,285 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   unsigned t = 0;
+#pragma unroll
   for (int i = 0; i < 16; ++i) t += red[i];
   return t;
 }
 
-// f(key, index) for the entries of the listed groups
-template <typename L, typename F>
+// f(there, key, index) for the entries of the listed groups, by whole waves; U groups of a wave are on their way
+template <int U, typename L, typename F>
 __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S, F f) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, n = S.n_group;
-  for (int g0 = wv * 4; g0 < n; g0 += 64) {
-    float x[4];
-    int v[4];
+  for (int g0 = wv * U; g0 < n; g0 += 16 * U) {
+    float x[U];
+    int v[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = g0 + e < n ? S.group[g0 + e] * SF_GROUP + lane : V;
+    for (int e = 0; e < U; ++e) {
+      v[e] = g0 + e < n ? S.group[min(g0 + e, n - 1)] * SF_GROUP + lane : V;
       x[e] = v[e] < V ? logit_f(row[v[e]]) : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f(v[e] < V, key_of(entry(x[e])), v[e], e, g0 + e);
+    for (int e = 0; e < U; ++e) f(v[e] < V, key_of(entry(x[e])), v[e]);
   }
 }
 
-// A border in the order of a row: the r first entries of value `key`, behind all larger ones (`above` of them, of mass `mass`)
-struct Border { unsigned key, r, above; u64 mass; };
+// Appends (key, ~index) of the lanes that `hit` to the list (n_list of them, those past CAP are only counted)
+__device__ __forceinline__ void append(PickLds& S, bool hit, unsigned key, int v) {
+  const int lane = threadIdx.x & 63;
+  const u64 all = __ballot(hit);
+  if (!all) return;
+  unsigned at = 0;
+  if (lane == 0) at = atomicAdd(&S.n_list, (unsigned)__popcll(all));
+  at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
+  if (hit && at < SF_CAP) S.list[at] = ((u64)key << 32) | (unsigned)~v;
+}
 
-// The entries with lo <= key <= hi into bins, hi's first; then the first bin by which `count` entries (or more than / at least
-// `mass`) are reached, and again within it until it is one key. Nothing reached: the end of the last bin.
-enum { BY_COUNT, BY_MASS, OVER_MASS };
-template <typename L>
-__device__ Border find_border(const L* row, int V, PickLds& S, unsigned lo, unsigned hi, float top, double it, int by,
-                              unsigned count, double mass) {
-  u64* mbin = S.list;
-  unsigned* cbin = (unsigned*)(S.list + SF_BINS);
+// The list in descending order; a key and its index are no other entry's. Returns a power of two >= count, zeros behind.
+__device__ unsigned sort_list(PickLds& S, unsigned count) {
   const int tid = threadIdx.x;
-  unsigned above = 0;
-  u64 m_above = 0;
-  for (;;) {
-    const unsigned range = hi - lo;
-    const int shift = range < SF_BINS ? 0 : 21 - __builtin_clz(range);  // range >> shift < 2048
+  unsigned n2 = 64, p = 16;  // p threads an entry
+  while (n2 < count) n2 *= 2, p /= 2;
+  if (n2 <= 512) {  // each entry's rank by counting the larger ones: n2^2 / 1024 comparisons a thread and no rounds
+    const unsigned i = tid / p;
+    const u64 mine = i < count ? S.list[i] : 0;
+    unsigned rank = 0;
+    for (unsigned j = tid & (p - 1); j < count; j += p) rank += S.list[j] > mine;
+    for (unsigned o = p / 2; o > 0; o >>= 1) rank += __shfl_xor(rank, o, 64);
     __syncthreads();
-    for (int i = tid; i < SF_BINS; i += 1024) { mbin[i] = 0; cbin[i] = 0; }
+    if ((tid & (p - 1)) == 0) S.list[i < count ? rank : i] = mine;
     __syncthreads();
-    each_entry(row, V, S, [&](bool in, unsigned key, int, int, int) {
-      if (!in || key < lo || key > hi) return;
-      const unsigned bin = (hi - key) >> shift;
-      atomicAdd(&cbin[bin], 1u);
-      atomicAdd(&mbin[bin], (u64)rint(weight(of_key(key), top, it) * SF_UNIT));
-    });
-    __syncthreads();
-    const unsigned c0 = cbin[2 * tid], c1 = cbin[2 * tid + 1];
-    const u64 m0 = mbin[2 * tid], m1 = mbin[2 * tid + 1];
-    const unsigned cb = above + scan_u<unsigned>(c0 + c1, S.redu[0]);
-    const u64 mb = m_above + scan_u<u64>(m0 + m1, S.redm);
-    if (tid == 0) S.found = 0;
-    __syncthreads();
-    auto reached = [&](unsigned c, u64 m) {
-      return by == BY_COUNT ? c >= count : by == BY_MASS ? (double)m >= mass : (double)m > mass;
-    };
-    // bins that hold something, the last of them if nothing is reached
-    if (c0 && !reached(cb, mb) && reached(cb + c0, mb + m0)) {
-      S.bin = 2 * tid; S.c_above = cb; S.c_at = c0; S.m_above = mb; S.m_at = m0; S.found = 1;
-    }
-    if (c1 && !reached(cb + c0, mb + m0) && reached(cb + c0 + c1, mb + m0 + m1)) {
-      S.bin = 2 * tid + 1; S.c_above = cb + c0; S.c_at = c1; S.m_above = mb + m0; S.m_at = m1; S.found = 1;
-    }
-    __syncthreads();
-    if (!S.found) {
-      const unsigned all = block_sum_u(c0 + c1, S.redu[1]) + above;
-      if (c0 && cb + c0 == all) { S.bin = 2 * tid; S.c_above = cb; S.c_at = c0; S.m_above = mb; S.m_at = m0; }
-      if (c1 && cb + c0 + c1 == all) { S.bin = 2 * tid + 1; S.c_above = cb + c0; S.c_at = c1; S.m_above = mb + m0; S.m_at = m1; }
-      __syncthreads();
-    }
-    above = S.c_above;
-    m_above = S.m_above;
-    const unsigned bin = S.bin, at = S.c_at;
-    const bool found = S.found;
-    hi -= bin << shift;
-    if (shift == 0) {
-      const double w = rint(weight(of_key(hi), top, it) * SF_UNIT);
-      double r = at;
-      if (found && by == BY_COUNT) r = count - above;
-      else if (found && w > 0) r = by == BY_MASS ? ceil((mass - (double)m_above) / w) : floor((mass - (double)m_above) / w) + 1;
-      return {hi, (unsigned)fmin(fmax(r, 1.0), (double)at), above, m_above};
-    }
-    const unsigned low = hi - ((1u << shift) - 1);
-    if (low > lo && low <= hi) lo = low;
+    return n2;
   }
-}
-
-__device__ __forceinline__ double border_mass(const Border& b, float top, double it) {
-  return (double)(b.mass + (u64)b.r * (u64)rint(weight(of_key(b.key), top, it) * SF_UNIT));
-}
-
-template <typename L>
-__device__ int pick_counted(const L* row, int V, PickLds& S, const RowOpts& o, unsigned kappa, unsigned hi, float top, double it,
-                            double zt, double u) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  unsigned lo = kappa, lo_m = 0;
-  if (o.m > 0) {  // the smallest key of weight min_p or more
-    unsigned a = 0, b = hi;
-    while (a < b) {
-      const unsigned mid = a + (b - a) / 2;
-      if (weight(of_key(mid), top, it) >= o.m) b = mid;
-      else a = mid + 1;
-    }
-    lo_m = a;
-    if (!(o.k && o.p < 1)) lo = max(lo, lo_m);
-  }
-  Border end = find_border(row, V, S, lo, hi, top, it, BY_COUNT, o.k ? (unsigned)o.k : 0xffffffffu, 0.0);
-  if (o.p < 1) {
-    const double mass = o.k ? border_mass(end, top, it) : zt * SF_UNIT;
-    const Border e = find_border(row, V, S, lo, hi, top, it, BY_MASS, 0, fmax(o.p * mass, 1.0));  // (the first entry at least)
-    if (e.key > end.key || (e.key == end.key && e.r < end.r)) end = e;
-  }
-  if (lo_m > end.key) end = find_border(row, V, S, lo_m, hi, top, it, BY_COUNT, 0xffffffffu, 0.0);
-  const Border at = find_border(row, V, S, lo, hi, top, it, OVER_MASS, 0, u * border_mass(end, top, it));
-  unsigned key = at.key, r = at.r;
-  if (key < end.key || (key == end.key && r > end.r)) key = end.key, r = end.r;
-  // the r-th of the entries of that value, by index: each listed group's count, in the groups' order
-  const int NG = (V + SF_GROUP - 1) / SF_GROUP;
-  __syncthreads();
-  for (int g = tid; g < SF_MAX_GROUPS; g += 1024) S.match[g] = 0;
-  __syncthreads();
-  each_entry(row, V, S, [&](bool in, unsigned k, int v, int, int) {
-    const u64 hit = __ballot(in && k == key);
-    if (hit && lane == 0) S.match[v / SF_GROUP] = (unsigned short)__popcll(hit);
-  });
-  __syncthreads();
-  unsigned c[4], sum = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sum += c[e] = 4 * tid + e < NG ? S.match[4 * tid + e] : 0;
-  unsigned before = scan_u<unsigned>(sum, S.redu[0]);
-  if (tid == 0) S.bin = 0, S.c_above = 0;
-  __syncthreads();
-  if (before < r && before + sum >= r) {
-    int e = 0;
-    while (before + c[e] < r) before += c[e++];
-    S.bin = 4 * tid + e;
-    S.c_above = r - before;  // of its matches
-  }
-  __syncthreads();
-  if (wv == 0) {
-    const int v = S.bin * SF_GROUP + lane;
-    const u64 hit = __ballot(v < V && key_of(entry(logit_f(row[min(v, V - 1)]))) == key);
-    const unsigned nth = __popcll(hit & ((2ull << lane) - 1));
-    if ((hit >> lane & 1) && nth == S.c_above) S.bin = v;
-  }
-  __syncthreads();
-  return S.bin;
-}
-
-__device__ int pick_sorted(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
-  const int tid = threadIdx.x;
-  unsigned n2 = 64;
-  while (n2 < count) n2 *= 2;
   for (unsigned i = count + tid; i < n2; i += 1024) S.list[i] = 0;
-  // bitonic, descending; a key and its index are no other entry's
   for (unsigned size = 2; size <= n2; size *= 2)
     for (unsigned step = size / 2; step > 0; step /= 2) {
       __syncthreads();
       for (unsigned i = tid; i < n2 / 2; i += 1024) {
         const unsigned x = 2 * i - (i & (step - 1)), y = x + step;
-        const u64 p = S.list[x], q = S.list[y];
-        if ((p < q) == ((x & size) == 0)) { S.list[x] = q; S.list[y] = p; }
+        const u64 q = S.list[x], r = S.list[y];
+        if ((q < r) == ((x & size) == 0)) { S.list[x] = r; S.list[y] = q; }
       }
     }
   __syncthreads();
-  const unsigned each = n2 > 1024 ? n2 / 1024 : 1;
-  double w[4], sum = 0, before;
-#pragma unroll
-  for (unsigned e = 0; e < 4; ++e) {
-    const unsigned i = tid * each + e;
-    w[e] = e < each && i < count ? weight(of_key((unsigned)(S.list[i] >> 32)), top, it) : 0.0;
-    sum += w[e];
+  return n2;
+}
+
+// A row's entries in their order up to a border: the last one's (key, ~index), their mass in units, how many
+struct Border { u64 last; double mass; unsigned n; };
+enum { BY_COUNT, BY_MASS, OVER_MASS };
+struct Goal {
+  int by;
+  unsigned count;
+  double mass;
+  __device__ bool reached(unsigned c, double m) const { return by == BY_COUNT ? c >= count : by == BY_MASS ? m >= mass : m > mass; }
+};
+
+template <typename L>
+struct Row {
+  const L* x;
+  int V;
+  float top, scale;  // bins a unit of logit
+  double it, least;  // entries of weight >= least count
+  unsigned lo, hi;   // and of these keys
+
+  __device__ double units(unsigned key) const { return rint(weight(of_key(key), top, it) * SF_UNIT); }
+  __device__ unsigned bin(unsigned key) const {
+    const float v = of_key(key), d = v == top ? 0.f : top - v;
+    return (unsigned)fminf(d * scale, (float)(SF_BINS - 1));
   }
-  scan_d(sum, S.redd[0], before);
+  __device__ bool counts(unsigned key) const { return key >= lo && (least <= 0 || weight(of_key(key), top, it) >= least); }
+};
+
+template <typename L, typename Bin>
+__device__ void fill_bins(const Row<L>& r, PickLds& S, Bin bin) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < SF_BINS; i += 1024) { S.mass[i] = 0; S.count[i] = 0; }
+  __syncthreads();
+  each_entry<2>(r.x, r.V, S, [&](bool there, unsigned key, int) {
+    if (!there || key < r.lo || key > r.hi) return;
+    const double w = weight(of_key(key), r.top, r.it);
+    if (w < r.least) return;
+    const unsigned at = bin(key);
+    atomicAdd(&S.count[at], 1u);
+    atomicAdd(&S.mass[at], (u64)rint(w * SF_UNIT));
+  });
+  __syncthreads();
+}
+
+// The first bin by which the goal is reached, from `above` entries of mass `m_above` on (the last that holds something, if none is):
+// S.bin, what is before it, and what it holds
+__device__ void find_bin(PickLds& S, const Goal& goal, unsigned above, u64 m_above) {
+  const int tid = threadIdx.x;
+  const unsigned c0 = S.count[2 * tid], c1 = S.count[2 * tid + 1];
+  const u64 m0 = S.mass[2 * tid], m1 = S.mass[2 * tid + 1];
+  const unsigned cb = above + scan_before<unsigned>(c0 + c1, S.redu[0]);
+  const u64 mb = m_above + scan_before<u64>(m0 + m1, S.redm);
+  if (tid == 0) S.found = 0;
+  __syncthreads();
+  auto take = [&](unsigned i, unsigned c_above, unsigned c_at, u64 mass) { S.bin = i; S.c_above = c_above; S.c_at = c_at; S.m_above = mass; };
+  const bool r0 = goal.reached(cb, (double)mb), r1 = goal.reached(cb + c0, (double)(mb + m0)), r2 = goal.reached(cb + c0 + c1, (double)(mb + m0 + m1));
+  if (c0 && !r0 && r1) take(2 * tid, cb, c0, mb), S.found = 1;
+  if (c1 && !r1 && r2) take(2 * tid + 1, cb + c0, c1, mb + m0), S.found = 1;
+  const unsigned all = block_sum_u(c0 + c1, S.redu[1]) + above;
+  if (!S.found) {
+    if (c0 && cb + c0 == all) take(2 * tid, cb, c0, mb);
+    if (c1 && cb + c0 + c1 == all) take(2 * tid + 1, cb + c0, c1, mb + m0);
+  }
+  __syncthreads();
+}
+
+// Too many entries in one bin: by the key, 11 bits of its range a time, and the last of a value's by their indices. The bins of
+// equal width are gone afterwards.
+template <typename L>
+__device__ Border border_by_key(Row<L> r, PickLds& S, const Goal& goal) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  unsigned above = 0;
+  u64 m_above = 0;
+  int shift;
+  do {
+    const unsigned range = r.hi - r.lo;
+    shift = range < SF_BINS ? 0 : 21 - __builtin_clz(range);  // range >> shift < 2048
+    fill_bins(r, S, [&](unsigned key) { return (r.hi - key) >> shift; });
+    find_bin(S, goal, above, m_above);
+    above = S.c_above;
+    m_above = S.m_above;
+    r.hi -= S.bin << shift;
+    const unsigned low = r.hi - ((1u << shift) - 1);
+    if (low > r.lo && low <= r.hi) r.lo = low;
+  } while (shift);
+  const unsigned key = r.hi, at = S.c_at;
+  const double w = r.units(key);
+  double n = at;  // of that value
+  if (S.found && goal.by == BY_COUNT) n = goal.count - above;
+  else if (S.found && w > 0) n = goal.by == BY_MASS ? ceil((goal.mass - (double)m_above) / w) : floor((goal.mass - (double)m_above) / w) + 1;
+  const unsigned nth = (unsigned)fmin(fmax(n, 1.0), (double)at);
+  __syncthreads();
+  for (int g = tid; g < SF_MAX_GROUPS; g += 1024) S.match[g] = 0;
+  __syncthreads();
+  each_entry<4>(r.x, r.V, S, [&](bool there, unsigned k, int v) {
+    const u64 hit = __ballot(there && k == key);
+    if (hit && lane == 0) S.match[v / SF_GROUP] = (unsigned short)__popcll(hit);
+  });
+  __syncthreads();
+  unsigned c[4], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += c[e] = S.match[4 * tid + e];
+  unsigned before = scan_before<unsigned>(sum, S.redu[0]);
+  if (before < nth && before + sum >= nth) {
+    int e = 0;
+    while (before + c[e] < nth) before += c[e++];
+    S.bin = 4 * tid + e;
+    S.c_at = nth - before;  // of its matches
+  }
+  __syncthreads();
+  const int v = S.bin * SF_GROUP + lane;  // (each wave for itself)
+  const u64 hit = __ballot(v < r.V && key_of(entry(logit_f(r.x[min(v, r.V - 1)]))) == key);
+  const u64 me = __ballot((hit >> lane & 1) && __popcll(hit & ((2ull << lane) - 1)) == S.c_at);
+  const unsigned index = S.bin * SF_GROUP + __builtin_ctzll(me | (1ull << 63));
+  __syncthreads();
+  return {((u64)key << 32) | (unsigned)~index, (double)m_above + nth * w, above + nth};
+}
+
+// The bins of equal width are filled
+template <typename L>
+__device__ Border border(const Row<L>& r, PickLds& S, const Goal& goal) {
+  const int tid = threadIdx.x;
+  find_bin(S, goal, 0, 0);
+  const unsigned bin = S.bin, above = S.c_above, n = S.c_at;
+  const double m_above = (double)S.m_above;
+  if (n > SF_CAP) {
+    const Border b = border_by_key(r, S, goal);
+    fill_bins(r, S, [&](unsigned key) { return r.bin(key); });
+    return b;
+  }
+  if (tid == 0) S.n_list = 0;
+  __syncthreads();
+  each_entry<4>(r.x, r.V, S, [&](bool there, unsigned key, int v) {
+    append(S, there && key >= r.lo && r.bin(key) == bin && r.counts(key), key, v);
+  });
+  __syncthreads();
+  sort_list(S, n);
+  double w[2], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned i = 2 * tid + e;
+    sum += w[e] = i < n ? r.units((unsigned)(S.list[i] >> 32)) : 0.0;
+  }
+  double C = m_above + scan_before<double>(sum, S.redd[0]);
+  unsigned before = 0;  // entries that do not reach the goal
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned i = 2 * tid + e;
+    C += w[e];
+    if (i < n) {
+      S.C[i] = C;
+      before += !goal.reached(above + i + 1, C);
+    }
+  }
+  const unsigned at = min(block_sum_u(before, S.redu[2]), n - 1);
+  const Border b{S.list[at], S.C[at], above + at + 1};
+  __syncthreads();
+  return b;
+}
+
+template <typename L>
+__device__ u64 pick_counted(Row<L>& r, PickLds& S, const RowOpts& o, double zt, double u) {
+  auto bins = [&] { fill_bins(r, S, [&](unsigned key) { return r.bin(key); }); };
+  Border end{0, 0, 0};
+  auto all = [&] {  // every entry that counts
+    find_bin(S, Goal{BY_COUNT, 0xffffffffu, 0.0}, 0, 0);
+    end = {0, (double)(S.m_above + S.mass[S.bin]), 0};
+  };
+  const bool mass_of_k = o.k && o.p < 1;  // the mass of the top k counts, whatever min-p leaves of them
+  r.least = mass_of_k ? 0.0 : o.m;
+  bins();
+  if (o.k) end = border(r, S, Goal{BY_COUNT, (unsigned)o.k, 0.0});
+  if (o.p < 1) {
+    const Border e = border(r, S, Goal{BY_MASS, 0, fmax(o.p * (o.k ? end.mass : zt * SF_UNIT), 1.0)});  // (the first entry at least)
+    if (e.last > end.last) end = e;
+  }
+  if (!o.k && !(o.p < 1)) all();
+  if (mass_of_k && o.m > 0 && weight(of_key((unsigned)(end.last >> 32)), r.top, r.it) < o.m) {
+    r.least = o.m;
+    bins();
+    all();
+  }
+  const Border at = border(r, S, Goal{OVER_MASS, 0, u * end.mass});
+  return at.last > end.last ? at.last : end.last;  // (an earlier entry is larger)
+}
+
+__device__ u64 pick_sorted(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
+  const int tid = threadIdx.x;
+  sort_list(S, count);
+  double w[2], sum = 0;
   unsigned over = 0;
 #pragma unroll
-  for (unsigned e = 0; e < 4; ++e) {
-    const unsigned i = tid * each + e;
-    before += w[e];
-    if (e < each && i < count) S.C[i] = before;
-    over += e < each && i < count && w[e] >= o.m;
+  for (int e = 0; e < 2; ++e) {
+    const unsigned i = 2 * tid + e;
+    sum += w[e] = i < count ? weight(of_key((unsigned)(S.list[i] >> 32)), top, it) : 0.0;
+    over += i < count && w[e] >= o.m;
+  }
+  double C = scan_before<double>(sum, S.redd[0]);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    C += w[e];
+    S.C[2 * tid + e] = C;
   }
   __syncthreads();
   unsigned n = min(o.k ? (unsigned)o.k : count, count);
   if (o.p < 1) {
     const double t = o.p * (o.k ? S.C[n - 1] : zt);
     unsigned c = 0;
-    for (unsigned i = tid; i < count; i += 1024) c += S.C[i] < t;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) c += (unsigned)(2 * tid + e) < count && S.C[2 * tid + e] < t;
     n = min(n, block_sum_u(c, S.redu[0]) + 1);
   }
   if (o.m > 0) n = min(n, max(1u, block_sum_u(over, S.redu[1])));
   const double t = u * S.C[n - 1];
   unsigned c = 0;
-  for (unsigned i = tid; i < n; i += 1024) c += S.C[i] <= t;
-  const unsigned at = min(block_sum_u(c, S.redu[2]), n - 1);
-  return (int)~(unsigned)S.list[at];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) c += (unsigned)(2 * tid + e) < n && S.C[2 * tid + e] <= t;
+  return S.list[min(block_sum_u(c, S.redu[2]), n - 1)];
 }
 
 template <typename L>
@@ -408,9 +493,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   const int b = blockIdx.x, V = a.s.V, tid = threadIdx.x, lane = tid & 63;
   const int NG = (V + SF_GROUP - 1) / SF_GROUP, NC = (V + SF_CHUNK - 1) / SF_CHUNK;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
-  const RowOpts o = row_opts(a, b);
-  const double it = 1.0 / o.T;
-  ChunkSum cs{0, 0, -INFINITY, 0};
+  ChunkSum cs{0, 0.f, -INFINITY, 0, 0};
   if (tid < NC) cs = a.sums[(long)b * NC + tid];
   unsigned gm[4];
   unsigned least = ~0u;
@@ -419,45 +502,60 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     gm[e] = tid + 1024 * e < NG ? a.gmax[(long)b * NG + tid + 1024 * e] : 0;
     if (tid + 1024 * e < NG) least = min(least, gm[e]);
   }
+  const RowOpts o = row_opts(a, b);
+  const double it = 1.0 / o.T;
+  double u;
+  if (a.u) u = a.u[b];
+  else u = u01(a.s.seed, (a.s.ctr ? (unsigned)a.s.ctr[b] : a.s.step) * 131071u + (unsigned)b, 0u);
+  u = fmin(fmax(u, 0.0), 1.0);
+  if (tid == 0) S.kappa = 0, S.n_group = 0, S.n_list = 0;
   const float top = block_max(cs.m, (float*)S.redu[0]);
   if (top == -INFINITY) {
     if (tid == 0) sample_bookkeep(a.s, b, 0, -INFINITY);
     return;
   }
-  double z1 = cs.m == -INFINITY ? 0.0 : cs.z1 * (cs.m == top ? 1.0 : exp_neg((double)cs.m - (double)top)), zt = 0, skip;
-  if (o.p < 1 && o.k == 0) zt = cs.m == -INFINITY ? 0.0 : cs.zt * weight(cs.m, top, it);
-  z1 = wave_sum_d(z1);
-  zt = wave_sum_d(zt);
-  if (lane == 0) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; }
-  if (tid == 0) S.kappa = 0, S.n_group = 0, S.n_list = 0;
-  __syncthreads();
-  z1 = S.redd[0][0] + S.redd[0][1];  // (up to 128 chunks: two waves)
-  zt = S.redd[1][0] + S.redd[1][1];
+  double z1 = 0, zt = 0;
+  if (cs.m != -INFINITY) {
+    z1 = ((double)cs.rest + cs.n) * (cs.m == top ? 1.0 : exp_neg((double)cs.m - (double)top));
+    if (o.p < 1 && o.k == 0) zt = cs.zt * weight(cs.m, top, it);
+  }
+  if (tid < 512) {  // (chunks there are up to 512 of)
+    z1 = wave_sum_d(z1);
+    zt = wave_sum_d(zt);
+    if (lane == 0) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; }
+  }
   const unsigned hi = key_of(top);
   // ---- the bound ----
-  unsigned kappa = 0;
+  unsigned kappa = key_of(-INFINITY);
   if (o.k && o.k <= NG) {
     // the k-th largest group's bin of 1024 between the smallest and the largest
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, x, 64));
-    unsigned* cbin = (unsigned*)S.list;
-    cbin[tid] = 0;
+    S.count[tid] = 0;
     if (lane == 0) S.redu[1][tid >> 6] = least;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < 16; ++i) least = min(least, S.redu[1][i]);
     const unsigned range = hi - least;
     const int shift = range < 1024 ? 0 : 22 - __builtin_clz(range);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (tid + 1024 * e < NG) atomicAdd(&cbin[(hi - gm[e]) >> shift], 1u);
+      if (tid + 1024 * e < NG) atomicAdd(&S.count[(hi - gm[e]) >> shift], 1u);
     __syncthreads();
-    const unsigned mine = cbin[tid], before = scan_u<unsigned>(mine, S.redu[0]);
+    const unsigned mine = S.count[tid], before = scan_before<unsigned>(mine, S.redu[0]);
     if (before < (unsigned)o.k && before + mine >= (unsigned)o.k) {
       const unsigned up = ((unsigned)tid << shift) + ((1u << shift) - 1);
       S.kappa = up >= hi ? 0 : hi - up;
     }
     __syncthreads();
-    kappa = S.kappa;
+    kappa = max(kappa, S.kappa);
+  }
+  __syncthreads();
+  z1 = zt = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    z1 += S.redd[0][i];
+    zt += S.redd[1][i];
   }
   if (!(o.k && o.p < 1)) {  // (with both, the mass of the top k is needed)
     double least_w = o.m;
@@ -469,33 +567,34 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     }
     kappa = min(kappa, hi);
   }
-  __syncthreads();
   // ---- the groups that pass it, in any order, and their entries ----
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (tid + 1024 * e < NG && gm[e] >= kappa) S.group[atomicAdd(&S.n_group, 1u)] = (unsigned short)(tid + 1024 * e);
-  __syncthreads();
-  each_entry(row, V, S, [&](bool in, unsigned key, int v, int, int) {
-    const bool hit = in && key >= kappa;
+  for (int e = 0; e < 4; ++e) {
+    const bool hit = tid + 1024 * e < NG && gm[e] >= kappa;
     const u64 all = __ballot(hit);
-    if (!all) return;
+    if (!all) continue;
     unsigned at = 0;
-    if (lane == 0) at = atomicAdd(&S.n_list, (unsigned)__popcll(all));
+    if (lane == 0) at = atomicAdd(&S.n_group, (unsigned)__popcll(all));
     at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-    if (hit && at < SF_CAP) S.list[at] = ((u64)key << 32) | (unsigned)~v;
-  });
+    if (hit) S.group[at] = (unsigned short)(tid + 1024 * e);
+  }
+  __syncthreads();
+  each_entry<4>(row, V, S, [&](bool there, unsigned key, int v) { append(S, there && key >= kappa, key, v); });
   __syncthreads();
   const unsigned count = S.n_list;
-  double u;
-  if (a.u) u = a.u[b];
-  else u = u01(a.s.seed, (a.s.ctr ? (unsigned)a.s.ctr[b] : a.s.step) * 131071u + (unsigned)b, 0u);
-  u = fmin(fmax(u, 0.0), 1.0);
-  const int tok = count <= SF_CAP ? pick_sorted(S, count, o, top, it, zt, u)
-                                  : pick_counted(row, V, S, o, kappa, hi, top, it, zt, u);
+  u64 at;
+  if (count <= SF_CAP) {
+    at = pick_sorted(S, count, o, top, it, zt, u);
+  } else {
+    // weights below a unit's half need no bins of their own: 32 T below the top
+    const float range = fminf(top - of_key(kappa), (float)(32.0 * o.T));
+    Row<L> r{row, V, top, range > 0.f ? (SF_BINS - 1) / range : 0.f, it, 0.0, kappa, hi};
+    at = pick_counted(r, S, o, zt, u);
+  }
   if (tid == 0) {
-    const float x = entry(logit_f(row[tok]));
+    const float x = of_key((unsigned)(at >> 32));
     const double d = x == top ? 0.0 : (double)x - (double)top;
-    sample_bookkeep(a.s, b, tok, (float)(d - log1p(z1 - 1.0)));
+    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - log1p(z1 - 1.0)));
   }
 }
 
@@ -517,8 +616,8 @@ DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int 
   FilterArgs a{T, p, m, (const float*)Ts, (const float*)ps, (const float*)ms, k, (const int*)ks, (const float*)u,
                (unsigned*)((char*)ws + (size_t)B * NC * sizeof(ChunkSum)), (ChunkSum*)ws, s};
   hipStream_t st = (hipStream_t)stream;
-  if (f32) filter_stats_kernel<float><<<dim3(NC, B), 256, 0, st>>>(a);
-  else filter_stats_kernel<bf16_t><<<dim3(NC, B), 256, 0, st>>>(a);
+  if (f32) filter_stats_kernel<float><<<dim3((NC + 3) / 4, B), 256, 0, st>>>(a);
+  else filter_stats_kernel<bf16_t><<<dim3((NC + 3) / 4, B), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (f32) filter_pick_kernel<float><<<B, 1024, 0, st>>>(a);
