@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
 struct PickLds {
   u64 list[SF_CAP];  // (key, ~index) of entries
   union {
-    double C[SF_CAP];                     // of sorted entries
-    unsigned short match[SF_MAX_GROUPS];  // each listed group's entries of one value
+    double C[SF_CAP];               // of sorted entries
+    unsigned match[SF_MAX_GROUPS];  // each listed group's entries of one value
   };
   u64 mass[SF_BINS];
   unsigned count[SF_BINS];
@@ -176,7 +176,7 @@ struct PickLds {
   unsigned redu[3][16];
   u64 redm[16];
   unsigned kappa, n_group, n_list;
-  unsigned bin, c_above, c_at, found;
+  unsigned bin, c_above, c_at, found, range[2];
   u64 m_above;
 };
 
@@ -211,36 +211,84 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   return t;
 }
 
-// f(there, key, index) for the entries of the listed groups, by whole waves; U groups of a wave are on their way
-template <int U, typename L, typename F>
-__device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S, F f) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, n = S.n_group;
-  for (int g0 = wv * U; g0 < n; g0 += 16 * U) {
-    float x[U];
-    int v[U];
+// The 4 neighbours of lane's in each of two groups of a wave's 8: x, and the first ones' indices (V: none)
+template <typename L>
+__device__ __forceinline__ void load_entries(const L* row, int V, const PickLds& S, int g0, float (&x)[8], int (&v)[2]) {
+  const int lane = threadIdx.x & 63, n = S.n_group;
 #pragma unroll
-    for (int e = 0; e < U; ++e) {
-      v[e] = g0 + e < n ? S.group[min(g0 + e, n - 1)] * SF_GROUP + lane : V;
-      x[e] = v[e] < V ? logit_f(row[v[e]]) : 0.f;
+  for (int h = 0; h < 2; ++h) {
+    const int g = g0 + 4 * h + (lane >> 4);
+    v[h] = g < n ? S.group[g] * SF_GROUP + (lane & 15) * 4 : V;
+    if (v[h] + 4 <= V) {
+      L q[4];
+      __builtin_memcpy(q, row + v[h], sizeof(q));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = logit_f(q[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = v[h] + e < V ? logit_f(row[v[h] + e]) : 0.f;
     }
-#pragma unroll
-    for (int e = 0; e < U; ++e) f(v[e] < V, key_of(entry(x[e])), v[e]);
   }
 }
 
-// Appends (key, ~index) of the lanes that `hit` to the list (n_list of them, those past CAP are only counted)
-__device__ __forceinline__ void append(PickLds& S, bool hit, unsigned key, int v) {
-  const int lane = threadIdx.x & 63;
-  const u64 all = __ballot(hit);
-  if (!all) return;
-  unsigned at = 0;
-  if (lane == 0) at = atomicAdd(&S.n_list, (unsigned)__popcll(all));
-  at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-  if (hit && at < SF_CAP) S.list[at] = ((u64)key << 32) | (unsigned)~v;
+// f(there, key, index) for the entries of the listed groups, by whole waves; one after the other in a loop where f is long: a
+// launch fetches its instructions anew
+template <typename L, typename F>
+__device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S, F f) {
+  for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
+    float x[8];
+    int v[2];
+    load_entries(row, V, S, g0, x, v);
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const int at = e < 4 ? v[0] + e : v[1] + e - 4;
+      f(at < V, key_of(entry(x[0])), at);
+#pragma unroll
+      for (int i = 0; i < 7; ++i) x[i] = x[i + 1];
+    }
+  }
 }
 
-// The list in descending order; a key and its index are no other entry's. Returns a power of two >= count, zeros behind.
-__device__ unsigned sort_list(PickLds& S, unsigned count) {
+// (key, ~index) of the listed groups' entries with lo <= key <= hi into the list (n_list of them; those past CAP are only counted,
+// and with `stop` no longer once they are)
+template <typename L>
+__device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigned lo, unsigned hi, bool stop) {
+  const int lane = threadIdx.x & 63;
+  for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
+    if (stop && *(volatile unsigned*)&S.n_list > SF_CAP) return;
+    float x[8];
+    int v[2];
+    load_entries(row, V, S, g0, x, v);
+    unsigned key[8], hits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      key[e] = key_of(entry(x[e]));
+      const int at = e < 4 ? v[0] + e : v[1] + e - 4;
+      hits |= (unsigned)(at < V && key[e] - lo <= hi - lo) << e;
+    }
+    if (!__ballot(hits)) continue;
+    unsigned at = __popc(hits), all = at;  // before the lane's, of the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned t = __shfl_up(all, o, 64);
+      if (lane >= o) all += t;
+    }
+    at = all - at;
+    all = __builtin_amdgcn_readlane(all, 63);
+    unsigned base = 0;
+    if (lane == 0) base = atomicAdd(&S.n_list, all);
+    at += __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (hits >> e & 1) {
+        if (at < SF_CAP) S.list[at] = ((u64)key[e] << 32) | (unsigned)~(e < 4 ? v[0] + e : v[1] + e - 4);
+        ++at;
+      }
+  }
+}
+
+// The list in descending order; a key and its index are no other entry's
+__device__ __forceinline__ void sort_list(PickLds& S, unsigned count) {
   const int tid = threadIdx.x;
   unsigned n2 = 64, p = 16;  // p threads an entry
   while (n2 < count) n2 *= 2, p /= 2;
@@ -253,7 +301,7 @@ __device__ unsigned sort_list(PickLds& S, unsigned count) {
     __syncthreads();
     if ((tid & (p - 1)) == 0) S.list[i < count ? rank : i] = mine;
     __syncthreads();
-    return n2;
+    return;
   }
   for (unsigned i = count + tid; i < n2; i += 1024) S.list[i] = 0;
   for (unsigned size = 2; size <= n2; size *= 2)
@@ -266,11 +314,10 @@ __device__ unsigned sort_list(PickLds& S, unsigned count) {
       }
     }
   __syncthreads();
-  return n2;
 }
 
-// A row's entries in their order up to a border: the last one's (key, ~index), their mass in units, how many
-struct Border { u64 last; double mass; unsigned n; };
+// A row's entries in their order up to a border: the last one's (key, ~index), their mass in units
+struct Border { u64 last; double mass; };
 enum { BY_COUNT, BY_MASS, OVER_MASS };
 struct Goal {
   int by;
@@ -279,41 +326,48 @@ struct Goal {
   __device__ bool reached(unsigned c, double m) const { return by == BY_COUNT ? c >= count : by == BY_MASS ? m >= mass : m > mass; }
 };
 
-template <typename L>
-struct Row {
-  const L* x;
-  int V;
-  float top, scale;  // bins a unit of logit
-  double it, least;  // entries of weight >= least count
-  unsigned lo, hi;   // and of these keys
+// The entries of a row that are counted, and their bins: of equal width from the top (scale: bins a unit of logit), or (shift >= 0) of
+// 2^shift keys from hi
+struct Bins {
+  float top, scale;
+  double it, least;  // weights below `least` do not count
+  unsigned lo, hi;   // nor do other keys
+  int shift;
 
-  __device__ double units(unsigned key) const { return rint(weight(of_key(key), top, it) * SF_UNIT); }
-  __device__ unsigned bin(unsigned key) const {
+  __device__ unsigned of(unsigned key) const {
+    if (shift >= 0) return (hi - key) >> shift;
     const float v = of_key(key), d = v == top ? 0.f : top - v;
     return (unsigned)fminf(d * scale, (float)(SF_BINS - 1));
   }
-  __device__ bool counts(unsigned key) const { return key >= lo && (least <= 0 || weight(of_key(key), top, it) >= least); }
+  __device__ double weight_of(unsigned key) const { return weight(of_key(key), top, it); }
+  __device__ static u64 units(double w) {  // rint(w 2^45): the low bits of the sum with 2^52
+    return (u64)__double_as_longlong(fma(w, SF_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+  __device__ void split() {  // the keys lo .. hi into 2048 bins or fewer
+    const unsigned range = hi - lo;
+    shift = range < SF_BINS ? 0 : 21 - __builtin_clz(range);
+  }
 };
 
-template <typename L, typename Bin>
-__device__ void fill_bins(const Row<L>& r, PickLds& S, Bin bin) {
+template <typename L>
+__device__ __forceinline__ void fill_bins(const L* row, int V, PickLds& S, const Bins& r) {
   __syncthreads();
   for (int i = threadIdx.x; i < SF_BINS; i += 1024) { S.mass[i] = 0; S.count[i] = 0; }
   __syncthreads();
-  each_entry<2>(r.x, r.V, S, [&](bool there, unsigned key, int) {
+  each_entry(row, V, S, [&](bool there, unsigned key, int) {
     if (!there || key < r.lo || key > r.hi) return;
-    const double w = weight(of_key(key), r.top, r.it);
+    const double w = r.weight_of(key);
     if (w < r.least) return;
-    const unsigned at = bin(key);
+    const unsigned at = r.of(key);
     atomicAdd(&S.count[at], 1u);
-    atomicAdd(&S.mass[at], (u64)rint(w * SF_UNIT));
+    atomicAdd(&S.mass[at], Bins::units(w));
   });
   __syncthreads();
 }
 
 // The first bin by which the goal is reached, from `above` entries of mass `m_above` on (the last that holds something, if none is):
 // S.bin, what is before it, and what it holds
-__device__ void find_bin(PickLds& S, const Goal& goal, unsigned above, u64 m_above) {
+__device__ __forceinline__ void find_bin(PickLds& S, const Goal& goal, unsigned above, u64 m_above) {
   const int tid = threadIdx.x;
   const unsigned c0 = S.count[2 * tid], c1 = S.count[2 * tid + 1];
   const u64 m0 = S.mass[2 * tid], m1 = S.mass[2 * tid + 1];
@@ -333,82 +387,40 @@ __device__ void find_bin(PickLds& S, const Goal& goal, unsigned above, u64 m_abo
   __syncthreads();
 }
 
-// Too many entries in one bin: by the key, 11 bits of its range a time, and the last of a value's by their indices. The bins of
-// equal width are gone afterwards.
+// The border in the bin that was found (of equal width, up to CAP entries): its entries sorted
 template <typename L>
-__device__ Border border_by_key(Row<L> r, PickLds& S, const Goal& goal) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  unsigned above = 0;
-  u64 m_above = 0;
-  int shift;
-  do {
-    const unsigned range = r.hi - r.lo;
-    shift = range < SF_BINS ? 0 : 21 - __builtin_clz(range);  // range >> shift < 2048
-    fill_bins(r, S, [&](unsigned key) { return (r.hi - key) >> shift; });
-    find_bin(S, goal, above, m_above);
-    above = S.c_above;
-    m_above = S.m_above;
-    r.hi -= S.bin << shift;
-    const unsigned low = r.hi - ((1u << shift) - 1);
-    if (low > r.lo && low <= r.hi) r.lo = low;
-  } while (shift);
-  const unsigned key = r.hi, at = S.c_at;
-  const double w = r.units(key);
-  double n = at;  // of that value
-  if (S.found && goal.by == BY_COUNT) n = goal.count - above;
-  else if (S.found && w > 0) n = goal.by == BY_MASS ? ceil((goal.mass - (double)m_above) / w) : floor((goal.mass - (double)m_above) / w) + 1;
-  const unsigned nth = (unsigned)fmin(fmax(n, 1.0), (double)at);
-  __syncthreads();
-  for (int g = tid; g < SF_MAX_GROUPS; g += 1024) S.match[g] = 0;
-  __syncthreads();
-  each_entry<4>(r.x, r.V, S, [&](bool there, unsigned k, int v) {
-    const u64 hit = __ballot(there && k == key);
-    if (hit && lane == 0) S.match[v / SF_GROUP] = (unsigned short)__popcll(hit);
-  });
-  __syncthreads();
-  unsigned c[4], sum = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sum += c[e] = S.match[4 * tid + e];
-  unsigned before = scan_before<unsigned>(sum, S.redu[0]);
-  if (before < nth && before + sum >= nth) {
-    int e = 0;
-    while (before + c[e] < nth) before += c[e++];
-    S.bin = 4 * tid + e;
-    S.c_at = nth - before;  // of its matches
-  }
-  __syncthreads();
-  const int v = S.bin * SF_GROUP + lane;  // (each wave for itself)
-  const u64 hit = __ballot(v < r.V && key_of(entry(logit_f(r.x[min(v, r.V - 1)]))) == key);
-  const u64 me = __ballot((hit >> lane & 1) && __popcll(hit & ((2ull << lane) - 1)) == S.c_at);
-  const unsigned index = S.bin * SF_GROUP + __builtin_ctzll(me | (1ull << 63));
-  __syncthreads();
-  return {((u64)key << 32) | (unsigned)~index, (double)m_above + nth * w, above + nth};
-}
-
-// The bins of equal width are filled
-template <typename L>
-__device__ Border border(const Row<L>& r, PickLds& S, const Goal& goal) {
+__device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S, const Bins& r, const Goal& goal) {
   const int tid = threadIdx.x;
-  find_bin(S, goal, 0, 0);
   const unsigned bin = S.bin, above = S.c_above, n = S.c_at;
   const double m_above = (double)S.m_above;
-  if (n > SF_CAP) {
-    const Border b = border_by_key(r, S, goal);
-    fill_bins(r, S, [&](unsigned key) { return r.bin(key); });
-    return b;
-  }
   if (tid == 0) S.n_list = 0;
+  // the bin's keys, from the first of it to before the first of the bin above: 64 keys of a range at a time
+  if (tid < 128) {
+    const unsigned upto = tid < 64 ? bin : bin - 1;
+    unsigned a = r.lo, b = r.hi;  // the smallest key of bin <= upto, of weight >= least (hi is one, in bin 0)
+    while (a < b && upto < SF_BINS) {
+      const unsigned step = (b - a) / 64 + 1, k = a + (tid & 63) * step;
+      const u64 in = __ballot(k >= a && k < b && r.of(k) <= upto && (r.least <= 0 || r.weight_of(k) >= r.least));
+      if (!in) {  // behind the last key tried
+        a += (b - 1 - a) / step * step + 1;
+        continue;
+      }
+      const unsigned i = __builtin_ctzll(in);
+      b = a + i * step;
+      a = i ? b - step + 1 : a;
+    }
+    if ((tid & 63) == 0) S.range[tid >> 6] = tid < 64 ? a : upto < SF_BINS ? a - 1 : r.hi;
+  }
   __syncthreads();
-  each_entry<4>(r.x, r.V, S, [&](bool there, unsigned key, int v) {
-    append(S, there && key >= r.lo && r.bin(key) == bin && r.counts(key), key, v);
-  });
+  const unsigned from = S.range[0], to = S.range[1];
+  collect(row, V, S, from, to, false);
   __syncthreads();
   sort_list(S, n);
   double w[2], sum = 0;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const unsigned i = 2 * tid + e;
-    sum += w[e] = i < n ? r.units((unsigned)(S.list[i] >> 32)) : 0.0;
+    sum += w[e] = i < n ? (double)Bins::units(r.weight_of((unsigned)(S.list[i] >> 32))) : 0.0;
   }
   double C = m_above + scan_before<double>(sum, S.redd[0]);
   unsigned before = 0;  // entries that do not reach the goal
@@ -422,38 +434,165 @@ __device__ Border border(const Row<L>& r, PickLds& S, const Goal& goal) {
     }
   }
   const unsigned at = min(block_sum_u(before, S.redu[2]), n - 1);
-  const Border b{S.list[at], S.C[at], above + at + 1};
+  const Border b{S.list[at], S.C[at]};
   __syncthreads();
   return b;
 }
 
+// The border among the entries of one value, r.hi, which the bins of one key each have found: the last one's index by counting
 template <typename L>
-__device__ u64 pick_counted(Row<L>& r, PickLds& S, const RowOpts& o, double zt, double u) {
-  auto bins = [&] { fill_bins(r, S, [&](unsigned key) { return r.bin(key); }); };
-  Border end{0, 0, 0};
-  auto all = [&] {  // every entry that counts
-    find_bin(S, Goal{BY_COUNT, 0xffffffffu, 0.0}, 0, 0);
-    end = {0, (double)(S.m_above + S.mass[S.bin]), 0};
-  };
-  const bool mass_of_k = o.k && o.p < 1;  // the mass of the top k counts, whatever min-p leaves of them
-  r.least = mass_of_k ? 0.0 : o.m;
-  bins();
-  if (o.k) end = border(r, S, Goal{BY_COUNT, (unsigned)o.k, 0.0});
-  if (o.p < 1) {
-    const Border e = border(r, S, Goal{BY_MASS, 0, fmax(o.p * (o.k ? end.mass : zt * SF_UNIT), 1.0)});  // (the first entry at least)
-    if (e.last > end.last) end = e;
+__device__ __forceinline__ Border equal_border(const L* row, int V, PickLds& S, const Bins& r, const Goal& goal) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const unsigned key = r.hi, above = S.c_above, at = S.c_at;
+  const double m_above = (double)S.m_above, w = (double)Bins::units(r.weight_of(key));
+  double n = at;  // of that value
+  if (S.found && goal.by == BY_COUNT) n = goal.count - above;
+  else if (S.found && w > 0) n = goal.by == BY_MASS ? ceil((goal.mass - m_above) / w) : floor((goal.mass - m_above) / w) + 1;
+  const unsigned nth = (unsigned)fmin(fmax(n, 1.0), (double)at);
+  __syncthreads();
+  for (int g = tid; g < SF_MAX_GROUPS; g += 1024) S.match[g] = 0;
+  __syncthreads();
+  each_entry(row, V, S, [&](bool there, unsigned k, int v) {
+    if (there && k == key) atomicAdd(&S.match[v / SF_GROUP], 1u);
+  });
+  __syncthreads();
+  unsigned c[4], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += c[e] = S.match[4 * tid + e];
+  unsigned before = scan_before<unsigned>(sum, S.redu[0]);
+  if (before < nth && before + sum >= nth) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (before < nth && before + c[e] >= nth) {
+        S.bin = 4 * tid + e;
+        S.c_at = nth - before;  // of its matches
+      }
+      before += c[e];
+    }
   }
-  if (!o.k && !(o.p < 1)) all();
-  if (mass_of_k && o.m > 0 && weight(of_key((unsigned)(end.last >> 32)), r.top, r.it) < o.m) {
-    r.least = o.m;
-    bins();
-    all();
-  }
-  const Border at = border(r, S, Goal{OVER_MASS, 0, u * end.mass});
-  return at.last > end.last ? at.last : end.last;  // (an earlier entry is larger)
+  __syncthreads();
+  const int v = S.bin * SF_GROUP + lane;  // (each wave for itself)
+  const u64 hit = __ballot(v < V && key_of(entry(logit_f(row[min(v, V - 1)]))) == key);
+  const u64 me = __ballot((hit >> lane & 1) && __popcll(hit & ((2ull << lane) - 1)) == S.c_at);
+  const unsigned index = S.bin * SF_GROUP + __builtin_ctzll(me | (1ull << 63));
+  __syncthreads();
+  return {((u64)key << 32) | (unsigned)~index, m_above + nth * w};
 }
 
-__device__ u64 pick_sorted(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
+// Rows of more entries than the list holds: the borders of top-k and of top-p, then u's. A function of its own, with the LDS as such:
+// inside the kernel its registers were the other rows' too (23 of them went to memory, 6.6 -> 8.3 us for one row of 32064), and
+// through generic pointers it took 95 us for 68 in 33 flat rows of 50257.
+typedef __attribute__((address_space(3))) PickLds* lds_pick_t;
+template <typename L>
+__device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, RowOpts o,
+                                                  Bins all, double zt, double u) {
+  const L* row = (const L*)global;
+  PickLds& S = *(PickLds*)lds;
+  const int tid = threadIdx.x;
+  Border end{0, 0};  // of what is kept (last 0: all that counts)
+  const bool mass_of_k = o.k && o.p < 1;  // the mass of the top k counts, whatever min-p leaves of them
+  Bins r = all;
+  r.least = mass_of_k ? 0.0 : o.m;
+  bool filled = false;
+  int border = o.k ? 0 : o.p < 1 ? 1 : 2;
+  unsigned above = 0;
+  u64 m_above = 0;
+  for (;;) {
+    if (border == 2 && r.shift < 0 && mass_of_k && o.m > r.least && r.weight_of((unsigned)(end.last >> 32)) < o.m) {
+      r.least = o.m;
+      filled = false;
+      end.last = 0;
+    }
+    if (!filled) fill_bins(row, V, S, r);
+    filled = true;
+    if (border == 2 && r.shift < 0 && end.last == 0) {
+      const u64 mine = S.mass[2 * tid] + S.mass[2 * tid + 1], before = scan_before<u64>(mine, S.redm);
+      if (tid == 1023) S.m_above = before + mine;
+      __syncthreads();
+      end.mass = (double)S.m_above;
+    }
+    const Goal goal = border == 0 ? Goal{BY_COUNT, (unsigned)o.k, 0.0}
+                      : border == 1 ? Goal{BY_MASS, 0, fmax(o.p * (o.k ? end.mass : zt * SF_UNIT), 1.0)}  // (the first entry at least)
+                                    : Goal{OVER_MASS, 0, u * end.mass};
+    find_bin(S, goal, above, m_above);
+    Border b;
+    if (r.shift < 0 && S.c_at <= SF_CAP) {
+      b = sorted_border(row, V, S, r, goal);
+    } else {
+      // too many in one bin: all the keys into bins of keys, and again the bin that is found, until it is one key
+      if (r.shift >= 0) {
+        above = S.c_above;
+        m_above = S.m_above;
+        r.hi -= S.bin << r.shift;
+        const unsigned low = r.hi - ((1u << r.shift) - 1);
+        if (low > r.lo && low <= r.hi) r.lo = low;
+      }
+      filled = false;
+      if (r.shift != 0) {
+        r.split();
+        continue;
+      }
+      b = equal_border(row, V, S, r, goal);
+      above = 0;
+      m_above = 0;
+      r.lo = all.lo;
+      r.hi = all.hi;
+      r.shift = -1;
+    }
+    if (b.last > end.last) end = {b.last, border == 2 ? end.mass : b.mass};  // (an earlier entry is larger; u's is no later than the end)
+    if (border == 2) return end.last;
+    border = border == 0 && o.p < 1 ? 1 : 2;
+  }
+}
+
+// Up to 64 NW entries: NW waves (the others have ended), an entry a thread
+template <int NW>
+__device__ __forceinline__ u64 pick_few(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
+  const unsigned tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  auto sync = [] { if constexpr (NW > 1) __syncthreads(); };
+  auto votes = [&](bool v, unsigned* red) {  // threads of the NW waves for which v
+    const unsigned n = __popcll(__ballot(v));
+    if constexpr (NW == 1) return n;
+    if (lane == 0) red[wv] = n;
+    __syncthreads();
+    unsigned all = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) all += red[i];
+    return all;
+  };
+  const u64 mine = tid < count ? S.list[tid] : 0;
+  unsigned rank = 0;
+#pragma unroll 4
+  for (unsigned j = 0; j < count; ++j) rank += S.list[j] > mine;
+  sync();
+  if (tid < count) S.list[rank] = mine;
+  sync();
+  const u64 at = tid < count ? S.list[tid] : 0;
+  const double w = tid < count ? weight(of_key((unsigned)(at >> 32)), top, it) : 0.0;
+  double C = w;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const double t = __shfl_up(C, x, 64);
+    if ((int)lane >= x) C += t;
+  }
+  if constexpr (NW > 1) {
+    if (lane == 63) S.redd[0][wv] = C;
+    __syncthreads();
+    double off = 0;
+#pragma unroll
+    for (int i = 0; i < NW - 1; ++i) off += i < (int)wv ? S.redd[0][i] : 0.0;
+    C += off;
+  }
+  S.C[tid] = C;
+  sync();
+  unsigned n = min(o.k ? (unsigned)o.k : count, count);
+  if (o.p < 1) n = min(n, votes(tid < count && C < o.p * (o.k ? S.C[n - 1] : zt), S.redu[0]) + 1);
+  if (o.m > 0) n = min(n, max(1u, votes(tid < count && w >= o.m, S.redu[1])));
+  const double t = u * S.C[n - 1];
+  return S.list[min(votes(tid < n && C <= t, S.redu[2]), n - 1)];
+}
+
+__device__ __forceinline__ u64 pick_sorted(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
   const int tid = threadIdx.x;
   sort_list(S, count);
   double w[2], sum = 0;
@@ -516,7 +655,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   }
   double z1 = 0, zt = 0;
   if (cs.m != -INFINITY) {
-    z1 = ((double)cs.rest + cs.n) * (cs.m == top ? 1.0 : exp_neg((double)cs.m - (double)top));
+    z1 = ((double)cs.rest + cs.n) * (cs.m == top ? 1.f : __builtin_amdgcn_exp2f((cs.m - top) * 1.44269504f));
     if (o.p < 1 && o.k == 0) zt = cs.zt * weight(cs.m, top, it);
   }
   if (tid < 512) {  // (chunks there are up to 512 of)
@@ -561,8 +700,8 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     double least_w = o.m;
     if (o.p < 1) least_w = fmax(least_w, (1.0 - o.p) * zt / V);
     if (least_w > 0) {
-      const double below = o.T * log(least_w), x = (double)top + fmin(below, 0.0);
-      const float f = (float)(x - 1e-6 * (fabs((double)top) + fabs(below)));  // (safely below what rounding could do)
+      const float below = fminf((float)o.T * __logf((float)least_w), 0.f);
+      const float f = top + below - 1e-5f * (fabsf(top) + fabsf(below) + (float)o.T);  // (safely below what rounding could do)
       if (f == f) kappa = max(kappa, key_of(f));
     }
     kappa = min(kappa, hi);
@@ -579,22 +718,27 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     if (hit) S.group[at] = (unsigned short)(tid + 1024 * e);
   }
   __syncthreads();
-  each_entry<4>(row, V, S, [&](bool there, unsigned key, int v) { append(S, there && key >= kappa, key, v); });
+  collect(row, V, S, kappa, hi, true);  // (too many to sort: the counted way, whatever their number)
   __syncthreads();
   const unsigned count = S.n_list;
   u64 at;
-  if (count <= SF_CAP) {
+  if (count <= 64) {
+    if (tid >= 64) return;
+    at = pick_few<1>(S, count, o, top, it, zt, u);
+  } else if (count <= 256) {
+    if (tid >= 256) return;
+    at = pick_few<4>(S, count, o, top, it, zt, u);
+  } else if (count <= SF_CAP) {
     at = pick_sorted(S, count, o, top, it, zt, u);
   } else {
     // weights below a unit's half need no bins of their own: 32 T below the top
     const float range = fminf(top - of_key(kappa), (float)(32.0 * o.T));
-    Row<L> r{row, V, top, range > 0.f ? (SF_BINS - 1) / range : 0.f, it, 0.0, kappa, hi};
-    at = pick_counted(r, S, o, zt, u);
+    at = pick_counted((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, range > 0.f ? (SF_BINS - 1) / range : 0.f, it, 0.0, kappa, hi, -1}, zt, u);
   }
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));
     const double d = x == top ? 0.0 : (double)x - (double)top;
-    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - log1p(z1 - 1.0)));
+    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - (double)log1pf((float)(z1 - 1.0))));
   }
 }
 
