@@ -1552,12 +1552,10 @@ def sample(logits, temperature: float, seed: int, step: int = 0, out_tok=None, o
 SAMPLE_FILTERED_MAX_V = 1 << 18  # entries of a row that sample_filtered takes (csrc/sample_filter.hip, SF_MAX_V)
 
 
-def _row_option(v, B: int, dtype, dev, name: str):
-    """A sampling option as (number for all rows, tensor with each row's)."""
-    if not isinstance(v, torch.Tensor):
-        return v, None
-    _req(v.is_cuda and v.device == dev and v.dtype == dtype and v.is_contiguous() and v.numel() >= B, name + ": one a row, contiguous, beside the logits")
-    return 0, v
+def _row_option(v, B: int, dtype, dev: int, name: str):
+    """A sampling option that is a tensor, with each row's."""
+    _req(v.dtype is dtype and v.get_device() == dev and v.is_contiguous() and v.numel() >= B, name + ": one a row, contiguous, beside the logits")
+    return v.data_ptr()
 
 
 def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, top_p=1.0, min_p=0.0, u=None, out_tok=None,
@@ -1568,40 +1566,55 @@ def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, 
     [B]. temperature <= 0: greedy; top_k <= 0, top_p >= 1 and min_p <= 0 are off. Ties go to the lower index, NaN counts as -inf, and a
     row of nothing else gives token 0 with log-probability -inf. Returns (tokens, logprobs): the untempered, unfiltered
     distribution's. Bookkeeping as ``sample``'s."""
-    f32 = logits.dtype == torch.float32
-    _req(logits.is_cuda and (f32 or logits.dtype == torch.bfloat16), "logits must be bf16 or fp32 on GPU")
+    f32 = logits.dtype is torch.float32
+    _req(logits.is_cuda and (f32 or logits.dtype is torch.bfloat16), "logits must be bf16 or fp32 on GPU")
     B, V = logits.shape
-    dev = logits.device
+    ld = logits.stride(0)
     _req(logits.stride(1) == 1 or V == 1, "logits layout")
-    _req(1 <= V <= SAMPLE_FILTERED_MAX_V and 0 <= logits.stride(0) < 1 << 31, "sample_filtered: vocabulary")
-    _same_device(logits)
-    T, Ts = _row_option(temperature, B, torch.float32, dev, "temperature")
-    p, ps = _row_option(top_p, B, torch.float32, dev, "top_p")
-    m, ms = _row_option(min_p, B, torch.float32, dev, "min_p")
-    k, ks = _row_option(top_k, B, torch.int32, dev, "top_k")
-    _row_option(u, B, torch.float32, dev, "u")
-    out_tok = torch.empty(B, dtype=torch.int32, device=dev) if out_tok is None else out_tok
-    out_lp = torch.empty(B, dtype=torch.float32, device=dev) if out_lp is None else out_lp
-    _i32(out_tok, "out_tok"); _req(out_tok.numel() >= B, "out_tok too short")
-    _req(out_lp.is_cuda and out_lp.dtype == torch.float32 and out_lp.is_contiguous() and out_lp.numel() >= B, "out_lp must be fp32 [B]")
+    _req(1 <= V <= SAMPLE_FILTERED_MAX_V and 0 <= ld < 1 << 31, "sample_filtered: vocabulary")
+    dev = _same_device(logits)
+    f32s, Ts, ps, ms, ks, us = torch.float32, None, None, None, None, None
+    if isinstance(temperature, torch.Tensor):
+        temperature, Ts = 0.0, _row_option(temperature, B, f32s, dev, "temperature")
+    if isinstance(top_k, torch.Tensor):
+        top_k, ks = 0, _row_option(top_k, B, torch.int32, dev, "top_k")
+    if isinstance(top_p, torch.Tensor):
+        top_p, ps = 0.0, _row_option(top_p, B, f32s, dev, "top_p")
+    if isinstance(min_p, torch.Tensor):
+        min_p, ms = 0.0, _row_option(min_p, B, f32s, dev, "min_p")
+    if u is not None:
+        us = _row_option(u, B, f32s, dev, "u")
+    if out_tok is None:
+        out_tok = logits.new_empty(B, dtype=torch.int32)
+    else:
+        _row_option(out_tok, B, torch.int32, dev, "out_tok")
+    if out_lp is None:
+        out_lp = logits.new_empty(B, dtype=f32s)
+    else:
+        _row_option(out_lp, B, f32s, dev, "out_lp")
     if conf is not None:
-        _req(conf.is_cuda and conf.dtype == torch.float32 and conf.is_contiguous() and conf.shape == (B, 2), "conf must be fp32 [B, 2]")
+        _row_option(conf, B, f32s, dev, "conf"); _req(conf.shape == (B, 2), "conf must be fp32 [B, 2]")
     for t in (active, ctr, pos, lens, start):
         if t is not None:
-            _i32(t, "bookkeeping"); _req(t.numel() >= B, "bookkeeping: one a row")
+            _row_option(t, B, torch.int32, dev, "bookkeeping")
     hist_ld = 0
     if hist is not None:
-        _i32(hist, "hist"); _req(hist.dim() == 2 and hist.shape[0] >= B, "hist [B, n]")
+        _row_option(hist, B, torch.int32, dev, "hist"); _req(hist.dim() == 2 and hist.shape[0] >= B, "hist [B, n]")
         _req(pos is not None and start is not None, "hist needs pos and start")
         hist_ld = hist.shape[1]
-    e = list(eos)[:4] + [-1] * (4 - min(4, len(eos)))
+    e = (*eos[:4], -1, -1, -1, -1)
     L = lib()
-    ws = _call_scratch(L.da_sample_filtered_ws(B, V), logits)
-    _check(L.da_sample_filtered(_at(logits), f32, B, V, logits.stride(0), T, p, m, max(0, min(int(k), V)), _at(Ts), _at(ps), _at(ms),
-                                _at(ks), _at(u), seed & 0xffffffff, step & 0xffffffff, _at(ctr), _at(ws), _at(out_tok),
-                                _at(out_lp), _at(conf), _at(active), _at(pos), _at(lens), _at(hist), _at(start), hist_ld, *e,
-                                _raw_stream()), "sample_filtered")
+    ws = _call_scratch(_filtered_bytes(B, V), logits)
+    _check(L.da_sample_filtered(logits.data_ptr(), f32, B, V, ld, temperature, top_p, min_p, max(0, min(int(top_k), V)), Ts, ps, ms,
+                                ks, us, seed & 0xffffffff, step & 0xffffffff, _at(ctr), ws.data_ptr(), out_tok.data_ptr(),
+                                out_lp.data_ptr(), _at(conf), _at(active), _at(pos), _at(lens), _at(hist), _at(start), hist_ld,
+                                e[0], e[1], e[2], e[3], _raw_stream()), "sample_filtered")
     return out_tok, out_lp
+
+
+@_rule
+def _filtered_bytes(B: int, V: int) -> int:
+    return lib().da_sample_filtered_ws(B, V)
 
 
 def sample_partial(logits, temperature: float, seed: int, v0: int, step: int = 0, ctr=None, out=None):
@@ -1961,100 +1974,100 @@ from .seq_kernels import (causal_conv, delta_rule, delta_step, delta_step_fits, 
 
 
 # --------------------------------------------------------------------------- 4-bit key / value cache
-def _cache4(c, Hkv: int, layers: bool = False):
-    """(head dim, slots, max_seq) of a 4-bit cache (one layer's; ``layers``: with the layers in front)."""
+def _same_device(*ts) -> int:
+    """The current device, where the launch goes: tensors elsewhere are refused."""
+    dev = torch._C._cuda_getDevice()
+    for t in ts:
+        if t.get_device() != dev:
+            raise ValueError("tensors must be on the current device")
+    return dev
+
+
+def _cache4(c, layers: bool = False):
+    """(current device, KV heads, head dim, slots, max_seq) of a 4-bit cache (one layer's; ``layers``: with the layers in front)."""
     k, ks, v, vs = c
-    dims = 4 + layers
-    _req(all(t.is_cuda and t.dtype == torch.uint8 and t.is_contiguous() and t.device == k.device for t in c), "cache4: contiguous uint8 on one GPU")
-    _req(k.dim() == dims and k.shape == v.shape and ks.shape == vs.shape == (*k.shape[:-1], SCALE_BYTES), "cache4: codes [slots, Hkv, max_seq, D / 2], scales [.., 4]")
-    D = 2 * k.shape[-1]
-    _req(D in (64, 96, 128), "cache4: head dim 64, 96 or 128")
-    _req(k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0 and ks.data_ptr() % 4 == 0 and vs.data_ptr() % 4 == 0, "cache4: alignment")
-    _req(k.shape[-3] == Hkv and max(k.shape) < 1 << 31, "cache4: KV heads")
-    return D, k.shape[-4], k.shape[-2]
+    dev = _same_device(k, ks, v, vs)
+    shape, scales = k.shape, ks.shape
+    _req(len(shape) == 4 + layers and v.shape == shape and vs.shape == scales and scales[:-1] == shape[:-1] and scales[-1] == SCALE_BYTES,
+         "cache4: codes [slots, Hkv, max_seq, D / 2], scales [.., 4]")
+    for t in c:
+        _req(t.dtype is torch.uint8 and t.is_contiguous() and t.data_ptr() % 16 == 0, "cache4: contiguous uint8, 16-byte aligned")
+    Hkv, max_seq, D = shape[-3], shape[-2], 2 * shape[-1]
+    _req(D in (64, 96, 128) and max_seq < 1 << 31, "cache4: head dim 64, 96 or 128")
+    return dev, Hkv, D, shape[-4], max_seq
 
 
-def _weight4(weight, c):
-    _req(weight.is_cuda and weight.dtype == torch.float32 and weight.is_contiguous() and weight.shape == c.k.shape[:-1]
-         and weight.device == c.k.device, "weight: contiguous fp32 [slots, Hkv, max_seq] beside its cache")
+def _weight4(weight, c, dev: int):
+    _req(weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.shape == c.k.shape[:-1],
+         "weight: contiguous fp32 [slots, Hkv, max_seq] beside its cache")
+    return weight.data_ptr()
 
 
-def _rows16(t, name: str, width: int):
-    _bf16_cuda(t, name)
-    _req(t.dim() == 2 and t.shape[1] == width and (t.shape[0] == 1 or (t.stride(0) % 8 == 0 and width <= t.stride(0) < 1 << 31))
-         and t.stride(1) == 1 and t.data_ptr() % 16 == 0, name + ": rows of 16-byte pieces")
+def _ints(t, n: int, dev: int, name: str):
+    _req(t.dtype is torch.int32 and t.get_device() == dev and t.is_contiguous() and t.numel() >= n, name + ": contiguous int32 on the current device, one a row")
+    return t.data_ptr()
 
 
-def _places(T: int, *places):
-    for t in places:
-        _i32(t, "places"); _req(t.numel() >= T, "places: one a token")
+def _rows16(t, width: int, dev: int, name: str):
+    """(address, row stride) of bf16 rows in pieces of 16 bytes"""
+    _req(t.dtype is torch.bfloat16 and t.get_device() == dev and t.dim() == 2 and t.shape[1] >= width, name + ": bf16 rows on the current device")
+    at, ld = t.data_ptr(), t.stride(0)
+    _req(t.stride(1) == 1 and at % 16 == 0 and (t.shape[0] <= 1 or (ld % 8 == 0 and 0 <= ld < 1 << 31)), name + ": rows of 16-byte pieces")
+    return at, ld
 
 
 def cache4_write(k, v, c: Cache4, slot, at, weight=None) -> None:
     """Keys and values k, v [T, Hkv * D] (bf16, rows of any stride) of T tokens into places ``at`` of slots ``slot`` (int32 [T])
     of a 4-bit cache, rounded to the nearest code (ties to even). One token a place; a token whose place lies outside the cache
     is not written. weight (fp32 [slots, Hkv, max_seq]): a written key's accumulated weight begins at 0."""
-    Hkv = c.k.shape[-3]
-    D, slots, max_seq = _cache4(c, Hkv)
-    _rows16(k, "k", Hkv * D); _rows16(v, "v", Hkv * D)
+    dev, Hkv, D, slots, max_seq = _cache4(c)
+    (ka, kl), (va, vl) = _rows16(k, Hkv * D, dev, "k"), _rows16(v, Hkv * D, dev, "v")
     T = k.shape[0]
-    _req(v.shape[0] == T, "k and v: the same tokens")
-    _places(T, slot, at)
-    if weight is not None:
-        _weight4(weight, c)
-    _same_device(c.k, k, v, slot, at)
-    _check(lib().da_cache4_write(None, _at(k), _at(v), k.stride(0), v.stride(0), _at(slot), _at(at), None, None, *map(_at, c),
-                                 _at(weight), T, 0, Hkv, D, slots, max_seq, _raw_stream()), "cache4_write")
+    _req(v.shape[0] == T and k.shape[1] == v.shape[1] == Hkv * D, "k and v: the same tokens, [T, Hkv * D]")
+    _check(lib().da_cache4_write(None, ka, va, kl, vl, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"), None, None, *map(_at, c),
+                                 None if weight is None else _weight4(weight, c, dev), T, 0, Hkv, D, slots, max_seq, _raw_stream()),
+           "cache4_write")
 
 
 def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4, weight=None):
     """``rope_cache`` with a 4-bit cache: q and k heads of qkv [T, (H + 2 Hkv) * D] rotated in place (by position ``pos``), k
     and v written as ``cache4_write`` writes them, to places ``at`` (which are not the positions once keys have been evicted)."""
-    Dc, slots, max_seq = _cache4(c, Hkv)
-    _bf16_cuda(qkv, "qkv"); _i32(pos, "pos")
+    dev, Hc, Dc, slots, max_seq = _cache4(c)
+    q, ld = _rows16(qkv, (H + 2 * Hkv) * D, dev, "qkv")
     T = qkv.shape[0]
-    _req(Dc == D and qkv.is_contiguous() and qkv.shape[1] == (H + 2 * Hkv) * D and qkv.data_ptr() % 16 == 0, "qkv shape")
-    _req(cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[-1] == 2 and cos_sin.shape[1] == D // 2,
-         "cos_sin must be fp32 [max_pos, D/2, 2]")
-    _places(T, pos, slot, at)
-    if weight is not None:
-        _weight4(weight, c)
-    _same_device(c.k, qkv, pos, slot, at, cos_sin)
-    q = qkv.data_ptr()
-    _check(lib().da_cache4_write(q, q + 2 * H * D, q + 2 * (H + Hkv) * D, qkv.shape[1], qkv.shape[1], _at(slot), _at(at), _at(pos),
-                                 _at(cos_sin), *map(_at, c), _at(weight), T, H, Hkv, D, slots, max_seq, _raw_stream()), "rope_cache4")
+    _req(Hc == Hkv and Dc == D and qkv.is_contiguous() and qkv.shape[1] == (H + 2 * Hkv) * D, "qkv shape")
+    _req(cos_sin.dtype is torch.float32 and cos_sin.get_device() == dev and cos_sin.is_contiguous() and cos_sin.shape[-1] == 2
+         and cos_sin.shape[1] == D // 2, "cos_sin must be fp32 [max_pos, D/2, 2]")
+    ld = qkv.shape[1]
+    _check(lib().da_cache4_write(q, q + 2 * H * D, q + 2 * (H + Hkv) * D, ld, ld, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"),
+                                 _ints(pos, T, dev, "pos"), cos_sin.data_ptr(), *map(_at, c),
+                                 None if weight is None else _weight4(weight, c, dev), T, H, Hkv, D, slots, max_seq, _raw_stream()),
+           "rope_cache4")
     return qkv
 
 
 def cache4_read(c: Cache4, slot: int, n: int):
     """The first n keys and values of a slot as bf16 [Hkv, n, D] (exact: what the codes stand for)."""
-    Hkv = c.k.shape[-3]
-    D, slots, max_seq = _cache4(c, Hkv)
+    dev, Hkv, D, slots, max_seq = _cache4(c)
     _req(0 <= slot < slots and 0 <= n <= max_seq, "cache4_read: outside the cache")
-    _same_device(c.k)
-    k, v = torch.empty((2, Hkv, n, D), dtype=torch.bfloat16, device=c.k.device)
-    _check(lib().da_cache4_read(*map(_at, c), Hkv, D, slots, max_seq, slot, n, _at(k), _at(v), _raw_stream()), "cache4_read")
+    k = c.k.new_empty((Hkv, n, D), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    _check(lib().da_cache4_read(*map(_at, c), Hkv, D, slots, max_seq, slot, n, k.data_ptr(), v.data_ptr(), _raw_stream()), "cache4_read")
     return k, v
 
 
-def _same_device(*ts):
-    """Launches go to the current device's stream: tensors of another device are refused."""
-    dev = torch._C._cuda_getDevice()
-    for t in ts:
-        _req(t.get_device() == dev, "tensors must be on the current device")
-
-
-ATTN4_JOINED = (12, 64)  # splits, and partials (splits x query heads of a KV head), that the last split's workgroup joins
-
-
 @_rule
-def _attn4_split(B: int, Hkv: int, max_len: int):
-    """(splits of the longest row, keys a split): some 6 workgroups a CU, of 256 keys at least, and up to 32 splits a row, whose join
-    costs more than the last CUs' share of the work. us of keys a split, 8 KV heads x 128: 64 rows of 2700 - 8192 keys 512 86 / 1024
-    77 / 2048 76 / 4096 82; 2 of 21000 - 65533 512 41 / 1024 34 / 2048 31 / 4096 32; 24 of 1400 - 4096 with weights 256 32 / 512 30 /
-    1024 31."""
+def _attn4_split(B: int, H: int, Hkv: int, D: int, max_len: int, weight: bool):
+    """(splits of the longest row, keys a split, whether the last split's workgroup joins them, bytes of scratch): some 6 workgroups a
+    CU, of 256 keys at least, and up to 32 splits a row, whose join costs more than the last CUs' share of the work. us of keys a
+    split, 8 KV heads x 128: 64 rows of 2700 - 8192 keys 512 86 / 1024 77 / 2048 76 / 4096 82; 2 of 21000 - 65533 512 41 / 1024 34 /
+    2048 31 / 4096 32; 24 of 1400 - 4096 with weights 256 32 / 512 30 / 1024 31. Joined inside where a workgroup has few partials (splits
+    x query heads) to read one after the other: 4 x 4 of them 80 -> 76 us in the first case, 16 x 8 in the second 32 -> 38; 12 of a lone
+    row (32 heads x 96) 12.4 -> 12.2, 24 12.3 -> 15.4."""
     keys = max(256, -(-max_len * B * Hkv // 1536 // 64) * 64, -(-max_len // 32 // 64) * 64)
-    return -(-max_len // keys), keys
+    nsplit = -(-max_len // keys)
+    joined = not weight and 1 < nsplit <= 12 and nsplit * (H // Hkv) <= 64 and B * Hkv <= N_COUNTERS
+    return nsplit, keys, joined, lib().da_decode_attn4_ws(B, H, D, max_len, nsplit, weight)
 
 
 def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: int, scale=None, out=None, pre=None, weight=None):
@@ -2063,32 +2076,30 @@ def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: in
     pre (int32 [B, 2]: P, slot; P % 64 == 0): the keys [0, P) of a row are those of another slot.
     weight (fp32 [slots, Hkv, max_seq]; not with pre): each key's probability, summed over the query heads of its KV head, is
     added to it (what ``cache4_evict`` goes by). Rows then have slots of their own."""
-    Dc, slots, max_seq = _cache4(c, Hkv)
-    _bf16_cuda(q, "q"); _i32(lens, "lens"); _i32(slot, "slot")
+    dev, Hc, Dc, slots, max_seq = _cache4(c)
+    _req(Hc == Hkv and Dc == D and H % Hkv == 0 and H // Hkv <= 16, "decode_attn4: head dim, KV heads, query heads")
+    qa, ldq = _rows16(q, H * D, dev, "q")
     B = q.shape[0]
-    _req(Dc == D and H % Hkv == 0 and H // Hkv <= 16, "decode_attn4: head dim, query heads")
-    _req(q.dim() == 2 and q.shape[1] >= H * D and q.stride(1) == 1 and (B <= 1 or q.stride(0) % 8 == 0) and q.data_ptr() % 16 == 0, "q layout")
-    _req(lens.numel() >= B and slot.numel() >= B and 1 <= max_len <= max_seq, "lens / slot / max_len")
-    _same_device(c.k, q, lens, slot)
+    la, sa, pa, wa = _ints(lens, B, dev, "lens"), _ints(slot, B, dev, "slot"), None, None
+    _req(1 <= max_len <= max_seq, "max_len")
     if pre is not None:
-        _i32(pre, "pre"); _req(pre.shape == (B, 2) and weight is None, "pre must be int32 [B, 2], without weight")
+        pa = _ints(pre, 2 * B, dev, "pre"); _req(pre.shape == (B, 2) and weight is None, "pre must be int32 [B, 2], without weight")
     if weight is not None:
-        _weight4(weight, c)
+        wa = _weight4(weight, c, dev)
     if out is None:
         out = q.new_empty((B, H * D))
-    _req(out.dtype == torch.bfloat16 and out.shape == (B, H * D) and out.stride(1) == 1 and out.device == q.device, "bad out")
+    else:
+        _req(out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == (B, H * D) and out.stride(1) == 1
+             and 0 <= out.stride(0) < 1 << 31, "bad out")
     if B == 0:
         return out
-    nsplit, keys = _attn4_split(B, Hkv, max_len)
+    nsplit, keys, joined, nbytes = _attn4_split(B, H, Hkv, D, max_len, weight is not None)
     stream = _raw_stream()
-    # few partials: the last of a row's splits joins them; else a second launch over all heads does
-    joined = weight is None and 1 < nsplit <= ATTN4_JOINED[0] and nsplit * (H // Hkv) <= ATTN4_JOINED[1] and B * Hkv <= N_COUNTERS
-    cnt = _counters(q.device, stream) if joined else None
-    L = lib()
-    ws = _call_scratch(L.da_decode_attn4_ws(B, H, D, max_len, nsplit, weight is not None), q)
-    _check(L.da_decode_attn4(_at(q), q.stride(0), *map(_at, c), _at(lens), _at(slot), _at(pre), B, H, Hkv, D, slots, max_seq, max_len,
-                             nsplit, keys, scale if scale is not None else D ** -0.5, _at(ws), _at(weight), _at(out), out.stride(0),
-                             _at(cnt), stream), "decode_attn4")
+    cnt = _counters(q.device, stream).data_ptr() if joined else None
+    ws = _call_scratch(nbytes, q)
+    _check(lib().da_decode_attn4(qa, ldq, *map(_at, c), la, sa, pa, B, H, Hkv, D, slots, max_seq, max_len, nsplit, keys,
+                                 D ** -0.5 if scale is None else scale, ws.data_ptr(), wa, out.data_ptr(), out.stride(0), cnt, stream),
+           "decode_attn4")
     return out
 
 
@@ -2098,20 +2109,15 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     in their order, with their weights. lens / slot int32 [B]; the kept rows go to the front of the same slot, or of slots ``to``
     (then shorter sequences are copied too). What lies behind them is left as it was. Slots, and those of ``to``, are distinct.
     c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: not lens itself)."""
-    Hkv = c.k.shape[-3]
     layered = c.k.dim() == 5
-    D, slots, max_seq = _cache4(c, Hkv, layered)
-    _weight4(weight, c)
-    _i32(lens, "lens"); _i32(slot, "slot")
+    dev, Hkv, D, slots, max_seq = _cache4(c, layered)
     B = lens.numel()
-    _req(slot.numel() >= B and 0 <= recent <= keep, "lens / slot, 0 <= recent <= keep")
-    if to is None:
-        to = slot
-    _i32(to, "to"); _req(to.numel() >= B, "to: one a row")
-    _same_device(c.k, lens, slot, to)
+    wa, la, sa = _weight4(weight, c, dev), _ints(lens, B, dev, "lens"), _ints(slot, B, dev, "slot")
+    ta = sa if to is None else _ints(to, B, dev, "to")
+    _req(0 <= recent <= keep, "0 <= recent <= keep")
     if out is None:
         out = torch.empty_like(lens)
-    _i32(out, "out"); _req(out.numel() >= B and out.data_ptr() != lens.data_ptr(), "out: int32 [B] apart from lens")
-    _check(lib().da_cache4_evict(*map(_at, c), _at(weight), _at(lens), _at(slot), _at(to), _at(out), c.k.shape[0] if layered else 1, B,
-                                 Hkv, D, slots, max_seq, min(keep, max_seq), min(recent, max_seq), _raw_stream()), "cache4_evict")
+    oa = _ints(out, B, dev, "out"); _req(oa != la or B == 0, "out: int32 [B] apart from lens")
+    _check(lib().da_cache4_evict(*map(_at, c), wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
+                                 min(keep, max_seq), min(recent, max_seq), _raw_stream()), "cache4_evict")
     return out
