@@ -31,25 +31,22 @@ __device__ __forceinline__ long row_of(const Cache4& c, int slot, int h, int at)
 }
 
 // ------------------------------------------------------------------------------------------- write, read
-// 8 consecutive elements a lane, 4 lanes a block; x as bf16 pairs. Returns the codes; the block's scale byte in `sb`.
+// 8 consecutive elements a lane, 4 lanes a block; x as bf16 pairs. Returns the codes (the conversion's rounding: to nearest, ties to
+// the even code, past 6 to 6); the block's scale byte in `sb`.
 __device__ __forceinline__ unsigned encode8(const u32x4_t& x, unsigned& sb) {
   unsigned a = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) a = max(a, max((x[e] << 16) & 0x7fffffffu, x[e] & 0x7fff0000u));
-  a = max(a, (unsigned)__shfl_xor((int)a, 1, 64));
-  a = max(a, (unsigned)__shfl_xor((int)a, 2, 64));
+  a = max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0xB1, 0xf, 0xf, true));  // lanes 1 and 2 away
+  a = max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0x4E, 0xf, 0xf, true));
   sb = (unsigned)max(1, (int)((a + 0x200000u) >> 23) - 2);
-  const bool bad = (a >> 23) >= 255;
-  const float up = __uint_as_float((254u - sb) << 23);
-  unsigned r = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const unsigned w = e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16;
-    const float y = fabsf(__uint_as_float(w) * up);
-    const unsigned code = (y > 0.25f) + (y >= 0.75f) + (y > 1.25f) + (y >= 1.75f) + (y > 2.5f) + (y >= 3.5f) + (y > 5.f);
-    r |= (code | ((w >> 31) << 3)) << (4 * e);
-  }
-  if (bad) { sb = 255; r = 0; }
+  const float scale = __uint_as_float(sb << 23);
+  const unsigned x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];  // (a bit_cast of a vector's element itself is one of its first)
+  unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf2_t, x0), scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf2_t, x1), scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf2_t, x2), scale, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf2_t, x3), scale, 3);
+  if ((a >> 23) >= 255) { sb = 255; r = 0; }
   return r;
 }
 
@@ -62,37 +59,59 @@ struct Write4 {
   Cache4 c;
 };
 
-// A lane per 8 elements. With cs the heads of q and k are rotated in place first (rope_cache's arithmetic, its bits).
+// A lane per 8 elements, 8 (heads of 64) or 16 lanes a row, W4_T tokens a thread, one behind the other in the cache as a rule: their
+// rows share lines. With cs the heads of q and k are rotated in place first (rope_cache's arithmetic, its bits).
+// Bound by memory: 16384 tokens of 32 heads x 96 (258 MB read and written) 107 us with a token a thread, 64-bit divisions, comparisons
+// for the codes and a byte a scale; neighbouring tokens on one XCD and inputs past the caches as well -> 54.
+constexpr int W4_T = 4;
 __global__ void __launch_bounds__(256) cache4_write_kernel(Write4 p) {
-  const int ch = p.D / 8, heads = p.H + 2 * p.c.Hkv;
-  const long item = (long)blockIdx.x * 256 + threadIdx.x;
-  const int t = (int)(item / (heads * ch)), r = (int)(item - (long)t * heads * ch);
-  if (t >= p.T) return;  // (whole blocks: a token has a multiple of 4 items)
-  const int hh = r / ch, c = r - hh * ch;
-  const bool is_q = hh < p.H, is_k = !is_q && hh < p.H + p.c.Hkv;
+  const int wg = xcd_remap(blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y), tb = wg % gridDim.x;
+  const int lg = p.D == 64 ? 3 : 4, r = wg / gridDim.x * 256 + threadIdx.x, hh = r >> lg, c = r & ((1 << lg) - 1);
+  if (hh >= p.H + 2 * p.c.Hkv) return;  // (whole rows)
+  const bool is_q = hh < p.H, is_k = !is_q && hh < p.H + p.c.Hkv, in = c < p.D / 8;
   const int h = is_q ? hh : is_k ? hh - p.H : hh - p.H - p.c.Hkv;
-  bf16_t* src = (is_q ? p.q + (long)t * p.ldk : is_k ? p.k + (long)t * p.ldk : p.v + (long)t * p.ldv) + h * p.D + c * 8;
-  u32x4_t x = *(const u32x4_t*)src;
-  if (p.cs && (is_q || is_k)) {
-    const float* f = p.cs + ((long)p.pos[t] * (p.D / 2) + c * 4) * 2;
-    const f32x4_t c01 = *(const f32x4_t*)f, c23 = *(const f32x4_t*)(f + 4);
-    const float cc[4] = {c01[0], c01[2], c23[0], c23[2]}, sn[4] = {c01[1], c01[3], c23[1], c23[3]};
+  bf16_t* src = (is_q ? p.q : is_k ? p.k : p.v) + h * p.D + c * 8;
+  const long ld = is_q || is_k ? p.ldk : p.ldv;
+  const int t0 = tb * W4_T;
+  u32x4_t x[W4_T];
+  int s[W4_T], at[W4_T];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x1 = bf2f(x[e] & 0xffff), x2 = bf2f(x[e] >> 16);
-      x[e] = pack_bf2(fmaf(x1, cc[e], -(x2 * sn[e])), fmaf(x2, cc[e], x1 * sn[e]));
-    }
-    *(u32x4_t*)src = x;
+  for (int i = 0; i < W4_T; ++i) {
+    const int t = min(t0 + i, p.T - 1);
+    x[i] = in ? __builtin_nontemporal_load((const u32x4_t*)(src + t * ld)) : u32x4_t{0, 0, 0, 0};
+    s[i] = p.slot[t];
+    at[i] = p.at[t];
   }
-  if (is_q) return;
-  unsigned sb;
-  const unsigned codes = encode8(x, sb);
-  const int s = p.slot[t], at = p.at[t];
-  if ((unsigned)s >= (unsigned)p.c.slots || (unsigned)at >= (unsigned)p.c.max_seq) return;
-  const long row = row_of(p.c, s, h, at);
-  *(unsigned*)((is_k ? p.c.k : p.c.v) + row * (p.D / 2) + c * 4) = codes;
-  if ((c & 3) == 0) (is_k ? p.c.ks : p.c.vs)[row * 4 + (c >> 2)] = (uint8_t)sb;
-  if (p.weight && is_k && c == 0) p.weight[row] = 0.f;
+#pragma unroll
+  for (int i = 0; i < W4_T; ++i) {
+    const int t = t0 + i;
+    if (t >= p.T) return;
+    if (p.cs && (is_q || is_k) && in) {
+      const float* f = p.cs + ((long)p.pos[t] * (p.D / 2) + c * 4) * 2;
+      const f32x4_t c01 = *(const f32x4_t*)f, c23 = *(const f32x4_t*)(f + 4);
+      const float cc[4] = {c01[0], c01[2], c23[0], c23[2]}, sn[4] = {c01[1], c01[3], c23[1], c23[3]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x1 = bf2f(x[i][e] & 0xffff), x2 = bf2f(x[i][e] >> 16);
+        x[i][e] = pack_bf2(fmaf(x1, cc[e], -(x2 * sn[e])), fmaf(x2, cc[e], x1 * sn[e]));
+      }
+      *(u32x4_t*)(src + t * ld) = x[i];
+    }
+    if (is_q) continue;
+    unsigned sb;
+    const unsigned codes = encode8(x[i], sb);
+    unsigned all = (c & 3) ? 0 : sb << (8 * (c >> 2));  // the row's scales, in its first lane
+    if (!in) all = 0;
+    if (lg == 4) all |= (unsigned)__shfl_down((int)all, 8, 16);
+    all |= (unsigned)__shfl_down((int)all, 4, 8);
+    if ((unsigned)s[i] >= (unsigned)p.c.slots || (unsigned)at[i] >= (unsigned)p.c.max_seq) continue;
+    const long row = row_of(p.c, s[i], h, at[i]);
+    if (in) *(unsigned*)((is_k ? p.c.k : p.c.v) + row * (p.D / 2) + c * 4) = codes;
+    if (c == 0) {
+      *(unsigned*)((is_k ? p.c.ks : p.c.vs) + row * 4) = all;
+      if (p.weight && is_k) p.weight[row] = 0.f;
+    }
+  }
 }
 
 __global__ void __launch_bounds__(256) cache4_read_kernel(Cache4 c, int slot, int n, int D, bf16_t* k, bf16_t* v) {
@@ -114,11 +133,11 @@ DA_EXPORT int da_cache4_write(void* q, void* k, void* v, int ldk, int ldv, const
                               int D, int slots, int max_seq, void* stream) {
   if (D % 32 || D < 32 || D > 128 || (cs && (!pos || !q)) || (!cs && H)) return (int)hipErrorInvalidValue;
   if (T == 0) return 0;
-  const long items = (long)T * (H + 2 * Hkv) * (D / 8);
-  if ((items + 255) / 256 > 0x7fffffffl) return (int)hipErrorInvalidValue;
+  const long rows = H + 2l * Hkv, wgs = (rows * (D == 64 ? 8 : 16) + 255) / 256;
+  if (wgs > 65535) return (int)hipErrorInvalidValue;
   Write4 p{(bf16_t*)q, (bf16_t*)k, (bf16_t*)v, ldk, ldv, T, H, D, (const int*)slot, (const int*)at, (const int*)pos,
            (const float*)cs, (float*)weight, {(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq}};
-  cache4_write_kernel<<<(unsigned)((items + 255) / 256), 256, 0, (hipStream_t)stream>>>(p);
+  cache4_write_kernel<<<dim3((T + W4_T - 1) / W4_T, (unsigned)wgs), 256, 0, (hipStream_t)stream>>>(p);
   DA_LAUNCH_CHECK();
 }
 

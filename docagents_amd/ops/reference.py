@@ -654,8 +654,7 @@ def cache4_write(k, v, c, slot, at, weight=None):
     ok = (s >= 0) & (s < slots) & (a >= 0) & (a < max_seq)
     s, a = s[ok], a[ok]
     for x, codes, scales in ((k, c.k, c.k_scale), (v, c.v, c.v_scale)):
-        new, sc = _encode4(x[ok].reshape(-1, Hkv, D))
-        codes[s, :, a], scales[s, :, a, :D // 32] = new, sc[..., :D // 32]
+        codes[s, :, a], scales[s, :, a] = _encode4(x[ok].reshape(-1, Hkv, D))
     if weight is not None:
         weight[s, :, a] = 0.0
 
