@@ -571,15 +571,17 @@ DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void*
 // ------------------------------------------------------------------------------------------- eviction
 // Of a sequence's n > keep keys a KV head keeps the `recent` last ones and of the others the keep - recent of largest weight
 // (equal ones: the earlier), in their order, at the front of its slot or of another. A workgroup per (KV head, row, layer):
-//   select  the smallest kept weight as a 32-bit key whose order is the weight's, 8 bits a pass, counted in LDS
-//   move    1024 keys at a time: ranks by a scan over the workgroup, then rows in pieces of 16 bytes, all of a step's reads
-//           before its writes (a row never moves back, so later steps read what is still there)
+//   select  the smallest kept weight as a 32-bit key whose order is the weight's, 11 bits a pass, counted in LDS
+//   list    of 4096 keys at a time the kept ones', by two sums over the workgroup (8 neighbours a thread)
+//   move    their rows, 512 or so at a time, in pieces of 16 bytes. A row moves to the front of where it was or stays: what a step
+//           writes, no later step reads, so the next step's rows are on their way while a step's are written, with one barrier.
+// Bound by memory and by the start of each workgroup.
 struct Evict4 {
   Cache4 c;
   float* weight;
   const int *lens, *slot, *to;
   int* out;
-  int D, keep, recent;
+  int keep, recent;
   long layer;  // rows of a layer
 };
 
@@ -588,131 +590,162 @@ __device__ __forceinline__ unsigned order_key(float x) {  // NaN lowest, -0 as +
   return x != x ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(1024) cache4_evict_kernel(Evict4 p) {
-  __shared__ int hist[256], wsum[16], src[1024], sel[2];
-  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+constexpr int EV_T = 512, EV_LIST = 8 * EV_T;
+
+// before the thread's own, over the workgroup's 8 waves; `all` of them
+__device__ __forceinline__ int scan8(int x, int* red, int& all) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int y = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(y, o, 64);
+    if (lane >= o) y += u;
+  }
+  __syncthreads();
+  if (lane == 63) red[wv] = y;
+  __syncthreads();
+  int off = 0;
+  all = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    off += q < wv ? red[q] : 0;
+    all += red[q];
+  }
+  return off + y - x;
+}
+
+struct Small { unsigned ks, vs, w; };  // a row's scales and weight
+__device__ __forceinline__ void arrived(u32x4_t& x) { asm volatile("" : "+v"(x)); }  // (waits for its load)
+__device__ __forceinline__ void arrived(Small& x) { asm volatile("" : "+v"(x.ks), "+v"(x.vs), "+v"(x.w)); }
+
+// Items 0 .. items - 1 from load(i, x) to store(i, x), EV_T U of them a step
+template <int U, typename T, typename Load, typename Store>
+__device__ __forceinline__ void move_rows(int items, Load load, Store store) {
+  T now[U] = {}, next[U] = {};
+#pragma unroll
+  for (int e = 0; e < U; ++e) load((int)threadIdx.x + EV_T * e, now[e]);
+  for (int i0 = 0; i0 < items; i0 += EV_T * U) {
+#pragma unroll
+    for (int e = 0; e < U; ++e) load(i0 + EV_T * U + (int)threadIdx.x + EV_T * e, next[e]);
+#pragma unroll
+    for (int e = 0; e < U; ++e) arrived(now[e]);
+    __syncthreads();  // the whole step is in registers
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      store(i0 + (int)threadIdx.x + EV_T * e, now[e]);
+      now[e] = next[e];
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
+  constexpr int NP = D / 32, RP = 2 * NP;  // 16-byte pieces of a row's codes, of keys and values
+  __shared__ int hist[2048], red[8], sel[2];
+  __shared__ unsigned short list[EV_LIST];
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int s = p.slot[b], d = p.to[b];
   const int n = (unsigned)s < (unsigned)p.c.slots && (unsigned)d < (unsigned)p.c.slots ? max(0, min(p.lens[b], p.c.max_seq)) : 0;
   const int keep = min(n, p.keep);
   if (blockIdx.z == 0 && hk == 0 && tid == 0) p.out[b] = keep;
-  if (keep == n && s == d) return;
+  if (keep == 0 || (keep == n && s == d)) return;
   const long from = blockIdx.z * p.layer + row_of(p.c, s, hk, 0), to = blockIdx.z * p.layer + row_of(p.c, d, hk, 0);
   const float* wt = p.weight + from;
   const int m = n > keep ? n - p.recent : 0;  // keys that have to earn their place (0: all are kept)
-  unsigned cut = 0;
+  unsigned cut = 0xffffffffu;
   int ties = 0;
-  if (m) {
+  if (m && keep > p.recent) {
     int need = keep - p.recent;
-    for (int sh = 24; need > 0 && sh >= 0; sh -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    cut = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+      for (int i = tid; i < 2048; i += EV_T) hist[i] = 0;
       __syncthreads();
-      for (int i = tid; i < m; i += 1024) {
+      for (int i = tid; i < m; i += EV_T) {
         const unsigned k = order_key(wt[i]);
-        if (sh == 24 || (k >> (sh + 8)) == (cut >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255], 1);
+        if (pass == 0 || (k >> (sh + bits)) == (cut >> (sh + bits))) atomicAdd(&hist[(k >> sh) & (bins - 1)], 1);
       }
       __syncthreads();
-      if (tid < 64) {  // from the largest down: lane t has the bins 255 - 4 t .. 252 - 4 t
-        int v[4], mine = 0;
+      int v[4], mine = 0, all;  // from the largest down: 4 bins a thread
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine += v[e] = hist[255 - 4 * lane - e];
-        int upto = mine;
+      for (int e = 0; e < 4; ++e) mine += v[e] = hist[2047 - 4 * tid - e];
+      int before = scan8(mine, red, all);
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int u = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += u;
-        }
-        int before = upto - mine;
-        if (before < need && upto >= need) {
-          int e = 0;
-          while (before + v[e] < need) before += v[e++];
-          sel[0] = 255 - 4 * lane - e;
+      for (int e = 0; e < 4; ++e) {
+        if (before < need && before + v[e] >= need) {
+          sel[0] = 2047 - 4 * tid - e;
           sel[1] = need - before;
         }
+        before += v[e];
       }
       __syncthreads();
       cut |= (unsigned)sel[0] << sh;
       need = sel[1];
-      __syncthreads();
     }
     ties = need;
-    if (keep == p.recent) cut = 0xffffffffu, ties = 0;
   }
-  const int np = p.D / 32;  // 16-byte pieces of a row's codes
-  int done = 0, tied = 0;   // keys kept, keys equal to the cut so far
-  for (int t0 = 0; t0 < n; t0 += 1024) {
-    const int i = t0 + tid;
-    const unsigned k = i < m ? order_key(wt[i]) : 0;
-    const int tie = i < m && k == cut;
-    auto scan = [&](int x, int& total) {  // exclusive, over the workgroup
-      int y = x;
+  int done = 0, tied = 0;  // keys kept, keys equal to the cut so far
+  for (int t0 = 0; t0 < n; t0 += EV_LIST) {
+    const int i0 = t0 + 8 * tid;
+    unsigned k[8];
+    int equal = 0;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(y, o, 64);
-        if (lane >= o) y += u;
-      }
-      if (lane == 63) wsum[wv] = y;
-      __syncthreads();
-      int off = 0;
-      total = 0;
-      for (int q = 0; q < 16; ++q) {
-        off += q < wv ? wsum[q] : 0;
-        total += wsum[q];
-      }
-      __syncthreads();
-      return off + y - x;
+    for (int e = 0; e < 8; ++e) {
+      k[e] = i0 + e < m ? order_key(wt[i0 + e]) : 0;
+      equal += i0 + e < m && k[e] == cut;
+    }
+    int all, cnt, before = tied + scan8(equal, red, all);
+    tied += all;
+    unsigned kept = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool tie = i0 + e < m && k[e] == cut;
+      if (i0 + e < n && (i0 + e >= m || k[e] > cut || (tie && before < ties))) kept |= 1u << e;
+      before += tie;
+    }
+    int at = scan8(__popc(kept), red, cnt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (kept >> e & 1) list[at++] = (unsigned short)(8 * tid + e);
+    __syncthreads();
+    const long src = from + t0, dst = to + done;
+    auto codes = [&](int i, long row) {
+      const int q = i % RP;
+      return (u32x4_t*)((q < NP ? p.c.k : p.c.v) + row * (D / 2) + (q < NP ? q : q - NP) * 16);
     };
-    int all_ties, cnt;
-    const int before = tied + scan(tie, all_ties);
-    const int kept = i < n && (i >= m || k > cut || (tie && before < ties));
-    tied += all_ties;
-    const int at = scan(kept, cnt);
-    if (kept) src[at] = i;
-    __syncthreads();
-    u32x4_t piece[8];
-    const int pieces = cnt * 2 * np;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int x = tid + 1024 * e;
-      if (x < pieces) {
-        const int row = x / (2 * np), q = x - row * 2 * np;
-        piece[e] = *(const u32x4_t*)((q < np ? p.c.k : p.c.v) + (from + src[row]) * (p.D / 2) + (q < np ? q : q - np) * 16);
-      }
-    }
-    unsigned ks = 0, vs = 0;
-    float w = 0.f;
-    if (tid < cnt) {
-      const long row = from + src[tid];
-      ks = *(const unsigned*)(p.c.ks + row * 4);
-      vs = *(const unsigned*)(p.c.vs + row * 4);
-      w = p.weight[row];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int x = tid + 1024 * e;
-      if (x < pieces) {
-        const int row = x / (2 * np), q = x - row * 2 * np;
-        *(u32x4_t*)((q < np ? p.c.k : p.c.v) + (to + done + row) * (p.D / 2) + (q < np ? q : q - np) * 16) = piece[e];
-      }
-    }
-    if (tid < cnt) {
-      const long row = to + done + tid;
-      *(unsigned*)(p.c.ks + row * 4) = ks;
-      *(unsigned*)(p.c.vs + row * 4) = vs;
-      p.weight[row] = w;
-    }
+    move_rows<4, u32x4_t>(
+        cnt * RP, [&](int i, u32x4_t& x) { if (i < cnt * RP) x = __builtin_nontemporal_load(codes(i, src + list[i / RP])); },
+        [&](int i, const u32x4_t& x) { if (i < cnt * RP) __builtin_nontemporal_store(x, codes(i, dst + i / RP)); });
+    move_rows<1, Small>(
+        cnt,
+        [&](int i, Small& x) {
+          if (i >= cnt) return;
+          const long row = src + list[i];
+          x = {*(const unsigned*)(p.c.ks + row * 4), *(const unsigned*)(p.c.vs + row * 4), __float_as_uint(p.weight[row])};
+        },
+        [&](int i, const Small& x) {
+          if (i >= cnt) return;
+          *(unsigned*)(p.c.ks + (dst + i) * 4) = x.ks;
+          *(unsigned*)(p.c.vs + (dst + i) * 4) = x.vs;
+          p.weight[dst + i] = __uint_as_float(x.w);
+        });
     done += cnt;
-    __syncthreads();
+    __syncthreads();  // the list is written again
   }
 }
 
 DA_EXPORT int da_cache4_evict(void* ck, void* cks, void* cv, void* cvs, void* weight, const void* lens, const void* slot,
                               const void* to, void* out, int layers, int B, int Hkv, int D, int slots, int max_seq, int keep,
                               int recent, void* stream) {
-  if (D % 32 || D < 32 || D > 128 || keep < 0 || recent < 0 || recent > keep || B > 65535 || layers > 65535) return (int)hipErrorInvalidValue;
+  if (D % 32 || D < 64 || D > 128 || keep < 0 || recent < 0 || recent > keep || B > 65535 || layers > 65535) return (int)hipErrorInvalidValue;
   if (B == 0 || layers == 0) return 0;
   Evict4 p{{(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq}, (float*)weight, (const int*)lens,
-           (const int*)slot, (const int*)to, (int*)out, D, keep, recent, (long)slots * Hkv * max_seq};
-  cache4_evict_kernel<<<dim3(Hkv, B, layers), 1024, 0, (hipStream_t)stream>>>(p);
+           (const int*)slot, (const int*)to, (int*)out, keep, recent, (long)slots * Hkv * max_seq};
+  const dim3 grid(Hkv, B, layers);
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 64) cache4_evict_kernel<64><<<grid, EV_T, 0, st>>>(p);
+  else if (D == 96) cache4_evict_kernel<96><<<grid, EV_T, 0, st>>>(p);
+  else cache4_evict_kernel<128><<<grid, EV_T, 0, st>>>(p);
   DA_LAUNCH_CHECK();
 }
