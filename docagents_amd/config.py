@@ -63,6 +63,11 @@ class Config:
     max_new_tokens: int = field(default=64, metadata={"env": "MAX_NEW_TOKENS"})
     summary_max_new_tokens: int = field(default=128, metadata={"env": "SUMMARY_MAX_NEW_TOKENS"})
     temperature: float = field(default=0.2, metadata={"env": "LLM_TEMPERATURE"})
+    # sampling filters (0, 1 and 0: off): the k likeliest tokens, the likeliest with that much of the probability together,
+    # those with at least that share of the likeliest one's
+    top_k: int = field(default=0, metadata={"env": "LLM_TOP_K"})
+    top_p: float = field(default=1.0, metadata={"env": "LLM_TOP_P"})
+    min_p: float = field(default=0.0, metadata={"env": "LLM_MIN_P"})
     weights_path: str = field(default="", metadata={"env": "WEIGHTS_PATH"})
     seed: int = field(default=0, metadata={"env": "SEED"})
     # decode rows of an engine replica; 0 = auto: the largest power of two <= 128 whose KV cache fits
@@ -70,6 +75,11 @@ class Config:
     # 128 rows 40.6 q/s vs 64 rows 38.3 (profiles/r6/stack)
     max_batch: int = field(default=0, metadata={"env": "ENGINE_MAX_BATCH"})
     kv_cache_gb: float = field(default=0.0, metadata={"env": "KV_CACHE_GB"})  # 0 -> auto
+    # keys and values of a Llama / Phi-3 decoder's cache: 16 (bf16) or 4 bits; with 4, KV_KEEP > 0 shortens a sequence that has
+    # filled its slot to that many keys a KV head (the KV_RECENT last ones and those attended to most)
+    kv_bits: int = field(default=16, metadata={"env": "KV_BITS"})
+    kv_keep: int = field(default=0, metadata={"env": "KV_KEEP"})
+    kv_recent: int = field(default=0, metadata={"env": "KV_RECENT"})
     fault_spec: str = field(default="", metadata={"env": "DA_FAULT"})
     # --- new keys: engine supervision / observability ---
     engine_step_timeout: float = field(default=300.0, metadata={"env": "ENGINE_STEP_TIMEOUT"})
@@ -148,6 +158,12 @@ class Config:
             raise ValueError(f"DTYPE={self.dtype!r} is not supported (choose one of {', '.join(self.ENGINE_DTYPES)})")
         if self.llm_dtype not in self.LLM_DTYPES:
             raise ValueError(f"LLM_DTYPE={self.llm_dtype!r} is not supported (choose one of {', '.join(self.LLM_DTYPES)})")
+        if self.kv_bits not in (4, 16):
+            raise ValueError(f"KV_BITS={self.kv_bits} is not supported (4 | 16)")
+        if self.kv_keep and (self.kv_bits != 4 or not 0 <= self.kv_recent <= self.kv_keep):
+            raise ValueError(f"KV_KEEP={self.kv_keep}, KV_RECENT={self.kv_recent} need KV_BITS=4 and 0 <= KV_RECENT <= KV_KEEP")
+        if self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1:
+            raise ValueError(f"LLM_TOP_K={self.top_k}, LLM_TOP_P={self.top_p}, LLM_MIN_P={self.min_p}: want k >= 0, 0 < p <= 1, 0 <= min_p <= 1")
         if self.index_kind not in ("flat", "ivfflat"):
             raise ValueError(f"INDEX_KIND={self.index_kind!r} is not supported (flat | ivfflat)")
         if self.tp_size < 1:

@@ -44,7 +44,8 @@ class Engine:
                  ivf_lists: int = 100, ivf_probes: int = 1, load_llm: bool = True, load_encoder: bool = True,
                  use_graphs: bool = True, embed_max_tokens: int = 65536, enc_dtype: str = "bf16",
                  share_prefix: bool = True, overlap_waves: bool = False, kv_cache_gb: float = 0.0,
-                 llm_dtype: str = "bf16"):
+                 llm_dtype: str = "bf16", top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, kv_bits: int = 16,
+                 kv_keep: int = 0, kv_recent: int = 0):
         self.device = torch.device(device)
         self.lock = threading.RLock()      # the decoder / generator (one GPU thread drives it)
         self.enc_lock = threading.RLock()  # the encoder: the fast embed lane and the batcher share it
@@ -66,7 +67,8 @@ class Engine:
         self.decoder = None
         self.gen = None
         if load_llm:
-            self.decoder = make_decoder(self.dec_cfg, self.device, seed=seed, tp=tp, dtype=llm_dtype)
+            self.decoder = make_decoder(self.dec_cfg, self.device, seed=seed, tp=tp, dtype=llm_dtype, kv_bits=kv_bits,
+                                        kv_keep=kv_keep, kv_recent=kv_recent)
             if max_batch <= 0:
                 max_batch = self.auto_batch(max_seq, overlap_waves, kv_gb=kv_cache_gb)
             # + 1 dummy slot (padded graph rows) + 2 prompt-head slots (ContinuousScheduler heads)
@@ -75,7 +77,7 @@ class Engine:
             self.decoder.alloc_cache((2 if overlap_waves else 1) * max_batch + 4, max_seq)
             self.gen = Generator(self.decoder, max_batch=max_batch, max_seq=max_seq, temperature=temperature,
                                  seed=seed, eos=sorted(self.chat.eos_ids), use_graphs=use_graphs,
-                                 share_prefix=share_prefix)
+                                 share_prefix=share_prefix, top_k=top_k, top_p=top_p, min_p=min_p)
         from ..index import make_index
         self.index = make_index(index_kind, self.enc_cfg.hidden, self.device, lists=ivf_lists, probes=ivf_probes)
         self._prefix_cache: dict[str, list[int]] = {}
@@ -199,7 +201,8 @@ class Engine:
         return v
 
     def context_budget(self, max_new: int) -> int:
-        return self.gen.cache.max_seq - max_new - 8
+        most = self.gen.cache.max_seq - max_new - 8
+        return min(most, self.gen.evict_above) if self.gen.evict_above else most
 
     def _answer_tail(self, question: str) -> str:
         return f"\nQuestion: {question}<|end|>\n<|assistant|>\n"

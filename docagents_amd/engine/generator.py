@@ -39,13 +39,17 @@ class GenResult:
 class Generator:
     def __init__(self, model, max_batch: int = 64, max_seq: int = 4096, temperature: float = 0.2,
                  seed: int = 0, eos=(), use_graphs: bool = True, max_prefill_tokens: int = 65536,
-                 check_every: int = 16, share_prefix: bool = True, min_shared_prefix: int = 64):
+                 check_every: int = 16, share_prefix: bool = True, min_shared_prefix: int = 64, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0):
         self.model = model
         # prompts of one wave that start with the same tokens (the Answer / Summarize system prompt:
         # ~260 tokens of every QA prompt) prefill that head once; see _generate_wave
         self.share_prefix, self.min_shared_prefix = share_prefix and model.prefix_sharing, min_shared_prefix
         self.max_batch = max_batch
         self.temperature, self.seed = temperature, seed
+        # None: the sampler without filters (its numbers are another function of the seed than the filtered one's)
+        on = top_k > 0 or top_p < 1 or min_p > 0
+        self.filters = {"top_k": top_k, "top_p": top_p, "min_p": min_p} if on else None
         self.eos = tuple(e for e in eos if e is not None)[:4]
         self.is_cuda = model.device.type == "cuda"
         self.use_graphs = use_graphs and self.is_cuda
@@ -57,6 +61,12 @@ class Generator:
             # one extra slot: the dummy slot for padded rows of a bucket
             model.alloc_cache(max_batch + 1, max_seq)
         self.cache = model.cache
+        # a model that shortens its sequences does so between steps, at most check_every of them apart: those that by then
+        # could be out of places
+        self.evict_above = self.cache.max_seq - check_every if model.kv_keep else 0
+        if model.kv_keep and not model.kv_keep < self.evict_above:
+            raise ValueError(f"kv_keep={model.kv_keep}: slots of {self.cache.max_seq} places leave room for fewer "
+                             f"than {max(0, self.evict_above)}")
         self.dummy_slot = self.cache.acquire(1, [1])[0]
         self.head = None  # {"tokens", "P", "slot"}: the last wave's shared prompt head, kept in its own slot
         self.states: dict[tuple, DecodeState] = {}
@@ -98,9 +108,26 @@ class Generator:
         key = (B, max_new, lane)
         st = self.states.get(key)
         if st is None:
-            st = DecodeState(self.model, B, max_new, self.temperature, self.seed, self.eos)
+            st = DecodeState(self.model, B, max_new, self.temperature, self.seed, self.eos, self.filters)
             self.states[key] = st
         return st
+
+    def check_context(self, n: int, max_new: int):
+        """Raises unless a prompt of n tokens and max_new generated ones fit: the slot, or, where sequences are shortened, the
+        prompt the slot and all of it the model's positions."""
+        if self.evict_above:
+            if n > self.evict_above:
+                raise ValueError(f"prompt of {n} tokens exceeds the {self.evict_above} places of a slot")
+            most = self.model.cfg.max_pos
+        else:
+            most = self.cache.capacity()
+        if n + max_new > most:
+            raise ValueError(f"prompt of {n} tokens + {max_new} new exceeds the context ({most})")
+
+    def evict(self, st: DecodeState):
+        """Between steps, at most check_every of them apart: shorten the sequences that need it (models with kv_keep)."""
+        if self.evict_above:
+            self.model.evict(st, self.evict_above)
 
     def _capture(self, st: DecodeState):
         # warm up on a side stream (allocator + lazy init), then capture one step
@@ -167,7 +194,7 @@ class Generator:
             logits = m.prefill(to(flat), to(pos), to(slot_tok), to(cu), int(lens.max()), to(last), prefix=prefix,
                                local_logits=True, lens=lens.tolist())
             r0, r1 = row0 + i, row0 + j
-            m.sample(logits, self.temperature, self.seed, 0, out_tok=st.tokens[r0:r1], out_lp=st.lp[r0:r1],
+            m.sample(logits, self.temperature, self.seed, 0, filters=self.filters, out_tok=st.tokens[r0:r1], out_lp=st.lp[r0:r1],
                      conf=st.conf[r0:r1], active=st.active[r0:r1], ctr=st.pos[r0:r1], pos=st.pos[r0:r1],
                      lens=st.lens[r0:r1], hist=st.hist[r0:r1], start=st.start[r0:r1], eos=self.eos)
             self.stats["prefill_tokens"] += int(tot)
@@ -210,9 +237,7 @@ class Generator:
         n = len(prompts)
         max_new = max(1, max_new)
         for p in prompts:
-            if len(p) + max_new > self.cache.capacity():
-                raise ValueError(f"prompt of {len(p)} tokens + {max_new} new exceeds the context "
-                                 f"({self.cache.capacity()})")
+            self.check_context(len(p), max_new)
             if len(p) == 0:
                 raise ValueError("empty prompt")
         B = min(_bucket(n), self.max_batch) if self.use_graphs else n
@@ -305,6 +330,8 @@ class Generator:
                     # padded rows never advance past the dummy slot's capacity
                 done += k
                 self.stats["decode_steps"] += k
+                if done < steps:
+                    self.evict(st)
                 if done < steps and int(st.active[:n].sum().item()) == 0:
                     break
                 if B > n:
@@ -480,7 +507,7 @@ class ContinuousScheduler:
         # prompts (a batch of summaries) joins in one or two ticks instead of trickling in at one
         # prefill chunk per tick, which would stretch the decode of the last-admitted rows
         self.max_admit_tokens = max_admit_tokens or 131072  # 4 x 32k-token chunks (deploy-stack tuning)
-        self.st = DecodeState(self.m, self.B, self.cap, gen.temperature, gen.seed, gen.eos)
+        self.st = DecodeState(self.m, self.B, self.cap, gen.temperature, gen.seed, gen.eos, gen.filters)
         # row buckets (powers of two up to B): a tick replays the graph of the smallest bucket that
         # holds every occupied row — an unloaded request decodes at batch-1 cost (the GEMV path), not
         # in the full B-row graph. Admission fills the lowest free rows, so occupancy stays compact.
@@ -496,9 +523,7 @@ class ContinuousScheduler:
         max_new = max(1, min(int(max_new), self.cap))
         if not prompt:
             raise ValueError("empty prompt")
-        if len(prompt) + max_new > self.gen.cache.capacity():
-            raise ValueError(f"prompt of {len(prompt)} tokens + {max_new} new exceeds the context "
-                             f"({self.gen.cache.capacity()})")
+        self.gen.check_context(len(prompt), max_new)
         self.pending.append((list(prompt), max_new, tag))
 
     def busy(self) -> bool:
@@ -536,6 +561,8 @@ class ContinuousScheduler:
             ahead: collections.deque = collections.deque()
             track = stop is not None and k > 1 and st.graph is not None
             while ran < k:
+                if ran % self.gen.check_every == 0:
+                    self.gen.evict(st)
                 if st.graph is not None:
                     st.graph.replay()
                 else:
@@ -771,7 +798,7 @@ class ContinuousScheduler:
         idx = h2d(np.asarray(live, dtype=np.int64), dev)
         names = ("tokens", "lp", "conf", "active", "pos", "lens", "hist", "start")
         s = {n: getattr(st, n).index_select(0, idx) for n in names}
-        self.m.sample(logits, self.gen.temperature, self.gen.seed, 0, out_tok=s["tokens"], out_lp=s["lp"], conf=s["conf"],
+        self.m.sample(logits, self.gen.temperature, self.gen.seed, 0, filters=self.gen.filters, out_tok=s["tokens"], out_lp=s["lp"], conf=s["conf"],
                       active=s["active"], ctr=s["pos"], pos=s["pos"], lens=s["lens"], hist=s["hist"], start=s["start"],
                       eos=self.gen.eos)
         for n in names:

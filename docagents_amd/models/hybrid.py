@@ -158,6 +158,7 @@ class _Layer:
 
 
 class HybridDecoder:
+    kv_keep = 0             # no sequence is shortened
     prefix_sharing = False  # a prompt head's recurrent state is not shared between sequences
     portion_steps = 8192    # a step runs any portions; prompts are cut at this many tokens by default
     stateful_step = True    # running a step twice advances a sequence twice (graph warm-up uses a spare slot)
@@ -290,11 +291,13 @@ class HybridDecoder:
         iota, = st.rows_iota
         m = SeqBatch(iota[:st.B + 1], st.slot, st.pos, iota[:st.B], st.B, st.B, 1, self.cache.row_pages * PAGE)
         logits = self._logits(self._forward(m, st.tokens), out=st.logits)
-        self.sample(logits, st.temperature, st.seed, 0, out_tok=st.tokens, out_lp=st.lp, conf=st.conf, active=st.active,
+        self.sample(logits, st.temperature, st.seed, 0, filters=st.filters, out_tok=st.tokens, out_lp=st.lp, conf=st.conf, active=st.active,
                     ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
         return st.tokens
 
-    def sample(self, logits, temperature: float, seed: int, step: int = 0, **kw):
+    def sample(self, logits, temperature: float, seed: int, step: int = 0, filters=None, **kw):
+        if filters:
+            return self.ops.sample_filtered(logits, temperature, seed, step, **filters, **kw)
         return self.ops.sample(logits, temperature, seed, step, **kw)
 
     def prefill_flops(self, lens) -> float:

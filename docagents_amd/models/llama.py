@@ -27,6 +27,7 @@ import numpy as np
 import torch
 
 from ..ops import get_ops
+from ..ops.cache4 import Cache4, cache4_bytes, new_cache4
 from ..ops.reference import interleave_gate_up, rope_table
 from .configs import DecoderConfig
 
@@ -109,9 +110,13 @@ class TPContext:
         return out.view(self.size, t.shape[0], -1).permute(1, 0, 2).reshape(t.shape[0], -1)
 
 
-def tp_sample(ops, tp: TPContext, logits, temperature: float, seed: int, step: int = 0, **kw):
+def tp_sample(ops, tp: TPContext, logits, temperature: float, seed: int, step: int = 0, filters=None, **kw):
     """Sampling over a vocab-parallel LM head (see LlamaDecoder.sample): partial stats of this rank's
-    slice [B, V/t] (global indices from rank * V/t), one all-gather of [B, 8] fp32, finalize."""
+    slice [B, V/t] (global indices from rank * V/t), one all-gather of [B, 8] fp32, finalize.
+    filters (top_k, top_p, min_p: ``ops.sample_filtered``'s) are borders in the whole distribution: the
+    slices are gathered for them."""
+    if filters:
+        return ops.sample_filtered(tp.all_gather_cols(logits), temperature, seed, step, **filters, **kw)
     if tp.size == 1:
         return ops.sample(logits, temperature, seed, step, **kw)
     ctr = kw.pop("ctr", None)
@@ -195,14 +200,11 @@ def decode_workspace_bytes(cfg: DecoderConfig, heads_local: int, tp: int, max_ba
                8 * max_batch * max(cfg.ffn * 2 // tp, cfg.vocab) * 4)
 
 
-class KVCache:
-    """Contiguous per-slot KV cache: k/v [layers][slots, Hkv_local, max_seq, D] (one allocation)."""
+class _Slots:
+    """Places for whole sequences, up to ``max_seq`` keys each."""
 
-    def __init__(self, cfg: DecoderConfig, slots: int, max_seq: int, tp_size: int, device):
+    def __init__(self, slots: int, max_seq: int):
         self.slots, self.max_seq = slots, max_seq
-        self.hkv = cfg.kv_heads // tp_size
-        self.buf = torch.zeros((cfg.layers, 2, slots, self.hkv, max_seq, cfg.head_dim), dtype=torch.bfloat16,
-                               device=device)
         self.free = list(range(slots - 1, -1, -1))
 
     def fits(self, tokens: list[int]) -> bool:
@@ -213,12 +215,6 @@ class KVCache:
         """The longest sequence the cache could hold."""
         return self.max_seq
 
-    def k(self, layer):
-        return self.buf[layer, 0]
-
-    def v(self, layer):
-        return self.buf[layer, 1]
-
     def acquire(self, n: int, tokens: list[int] | None = None) -> list[int]:
         if n > len(self.free):
             raise RuntimeError(f"KV cache exhausted: want {n} slots, {len(self.free)} free")
@@ -227,9 +223,48 @@ class KVCache:
     def release(self, ids):
         self.free.extend(ids)
 
+
+class KVCache(_Slots):
+    """Contiguous per-slot KV cache: k/v [layers][slots, Hkv_local, max_seq, D] (one allocation)."""
+
+    def __init__(self, cfg: DecoderConfig, slots: int, max_seq: int, tp_size: int, device):
+        super().__init__(slots, max_seq)
+        self.hkv = cfg.kv_heads // tp_size
+        self.buf = torch.zeros((cfg.layers, 2, slots, self.hkv, max_seq, cfg.head_dim), dtype=torch.bfloat16,
+                               device=device)
+
+    def k(self, layer):
+        return self.buf[layer, 0]
+
+    def v(self, layer):
+        return self.buf[layer, 1]
+
     @staticmethod
     def bytes_for(cfg: DecoderConfig, slots: int, max_seq: int, tp_size: int = 1) -> int:
         return cfg.layers * 2 * slots * (cfg.kv_heads // tp_size) * max_seq * cfg.head_dim * 2
+
+
+class KVCache4(_Slots):
+    """The slots' keys and values in 4 bits (``ops.cache4``: 68 bytes of 256 for a key of 128), and, if sequences are to be
+    shortened, each key's accumulated attention weight (fp32 [layers, slots, Hkv_local, max_seq])."""
+
+    def __init__(self, cfg: DecoderConfig, slots: int, max_seq: int, tp_size: int, device, weights: bool):
+        super().__init__(slots, max_seq)
+        hkv = cfg.kv_heads // tp_size
+        self.all = new_cache4(slots, hkv, max_seq, cfg.head_dim, device, layers=cfg.layers)
+        self.weight = torch.zeros((cfg.layers, slots, hkv, max_seq), device=device) if weights else None
+
+    def layer(self, i: int) -> Cache4:
+        return self.all.layer(i)
+
+    def weight_of(self, i: int):
+        return None if self.weight is None else self.weight[i]
+
+    @staticmethod
+    def bytes_for(cfg: DecoderConfig, slots: int, max_seq: int, tp_size: int = 1, weights: bool = False) -> int:
+        hkv = cfg.kv_heads // tp_size
+        return (cache4_bytes(slots, hkv, max_seq, cfg.head_dim, cfg.layers)
+                + (4 * cfg.layers * slots * hkv * max_seq if weights else 0))
 
 
 class LlamaDecoder:
@@ -240,7 +275,19 @@ class LlamaDecoder:
     stateful_step = False   # running a decode step twice leaves a sequence as running it once
 
     def __init__(self, cfg: DecoderConfig, device="cuda", seed: int = 0, tp: TPContext | None = None,
-                 weights: dict | None = None):
+                 weights: dict | None = None, kv_bits: int = 16, kv_keep: int = 0, kv_recent: int = 0):
+        """kv_bits: of the cache's keys and values (16: bf16; 4: ``ops.cache4``). kv_keep (4 bits only; 0: off): a sequence
+        that fills its slot is shortened to that many keys a KV head, the ``kv_recent`` last ones and of the others those that
+        were attended to most, and goes on to the model's last position (``evict``)."""
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits={kv_bits}: 4 or 16")
+        if kv_bits == 4 and cfg.head_dim not in (64, 96, 128):
+            raise ValueError(f"{cfg.name}: a 4-bit cache holds heads of 64, 96 or 128, not {cfg.head_dim}")
+        if kv_keep and (kv_bits != 4 or not 0 <= kv_recent <= kv_keep):
+            raise ValueError(f"kv_keep={kv_keep}, kv_recent={kv_recent}: a 4-bit cache, 0 <= kv_recent <= kv_keep")
+        self.kv_bits, self.kv_keep, self.kv_recent = kv_bits, kv_keep, kv_recent
+        if kv_keep:  # a head's keys are not another sequence's to drop, and a step adds to the keys' weights
+            self.prefix_sharing, self.stateful_step = False, True
         self.cfg = cfg
         self.device = torch.device(device)
         self.ops = get_ops(self.device)
@@ -273,13 +320,21 @@ class LlamaDecoder:
         """The gain a fused batch-1 GEMV norm streams: none once the gains are folded."""
         return None if self.unit_gains else g
 
-    def alloc_cache(self, slots: int, max_seq: int) -> KVCache:
+    def alloc_cache(self, slots: int, max_seq: int) -> KVCache | KVCache4:
         max_seq = min(max_seq, self.cfg.max_pos)
-        self.cache = KVCache(self.cfg, slots, max_seq, self.tp.size, self.device)
+        args = (self.cfg, slots, max_seq, self.tp.size, self.device)
+        self.cache = KVCache4(*args, weights=self.kv_keep > 0) if self.kv_bits == 4 else KVCache(*args)
         return self.cache
 
     def cache_bytes(self, slots: int, max_seq: int) -> int:
-        return KVCache.bytes_for(self.cfg, slots, min(max_seq, self.cfg.max_pos), self.tp.size)
+        args = (self.cfg, slots, min(max_seq, self.cfg.max_pos), self.tp.size)
+        return KVCache4.bytes_for(*args, weights=self.kv_keep > 0) if self.kv_bits == 4 else KVCache.bytes_for(*args)
+
+    def evict(self, st: "DecodeState", above: int) -> None:
+        """Shorten the rows of a decode state whose sequences have more than ``above`` keys to ``kv_keep`` (all layers; the
+        lengths follow, the positions go on)."""
+        c = self.cache
+        st.lens.copy_(self.ops.cache4_evict(c.all, c.weight, st.lens, st.slot, self.kv_keep, self.kv_recent, above=above))
 
     def workspace_bytes(self, max_batch: int, max_seq: int) -> int:
         return decode_workspace_bytes(self.cfg, self.hl, self.tp.size, max_batch, max_seq)
@@ -287,7 +342,8 @@ class LlamaDecoder:
     def decode_buffers(self, B: int) -> dict:
         """Static buffers of a decode state; tuples are shared as they are by views of fewer rows."""
         c, b16 = self.cfg, dict(dtype=torch.bfloat16, device=self.device)
-        return {"x": torch.zeros(B, c.hidden, **b16), "h": torch.zeros(B, c.hidden, **b16),
+        return {**({"at": torch.zeros(B, dtype=torch.int32, device=self.device)} if self.kv_keep else {}),
+                "x": torch.zeros(B, c.hidden, **b16), "h": torch.zeros(B, c.hidden, **b16),
                 "qkv": torch.zeros(B, (self.hl + 2 * self.kl) * c.head_dim, **b16),
                 "attn": torch.zeros(B, self.hl * c.head_dim, **b16),
                 "logits": torch.zeros(B, c.vocab // self.tp.size, **b16),  # this rank's slice
@@ -351,7 +407,8 @@ class LlamaDecoder:
         D, hl, kl = c.head_dim, self.hl, self.kl
         x = o.embed(ids, self.w["embed"])
         hook = self.layer_hook
-        kv_from_cache = bool(getattr(o, "flash_kv_cache_ok", lambda *_: False)(D, True))
+        four = self.kv_bits == 4
+        kv_from_cache = not four and bool(getattr(o, "flash_kv_cache_ok", lambda *_: False)(D, True))
         # up to 64 tokens: the decode step's products, which have the norms and the rotation in them: seven launches a layer for nine,
         # which the host takes longer for than the device (52 tokens through a 3.8B 3493 -> 2558 us, 38 through an 8B 3689 -> 3486)
         few = self._dk_decode(x.shape[0]) and o.dk_rope_fits(x.shape[0], *self.w["layers"][0]["wqkv"].shape, x.stride(0))
@@ -363,7 +420,11 @@ class LlamaDecoder:
                 hook(li)
             # QKV projection + RoPE + KV-cache write in one kernel (gemm8p EPI_ROPE epilogue, gemm_dk's); where the
             # attention reads its keys from the cache (Phi-3's D = 96), k / v go to the cache only
-            if few:
+            if four:  # attention over the prompt's own keys as they are, over a shared head's as the cache holds them
+                h = x if few and li else o.rmsnorm(x, L["ln_attn"], c.eps)
+                qkv = o.gemm_dk(h, L["wqkv"], norm_in=norm) if few else o.gemm(h, L["wqkv"])
+                o.rope_cache4(qkv, pos, self.cos_sin, hl, kl, D, slot_tok, pos, cache.layer(li), cache.weight_of(li))
+            elif few:
                 h = x if li else o.rmsnorm(x, L["ln_attn"], c.eps)
                 qkv = o.gemm_dk_rope(h, L["wqkv"], pos, self.cos_sin, hl, kl, D, slot_tok, cache.k(li), cache.v(li),
                                      norm_in=norm, kv_out=not kv_from_cache)
@@ -371,7 +432,12 @@ class LlamaDecoder:
                 h = o.rmsnorm(x, L["ln_attn"], c.eps)
                 qkv = o.gemm_rope(h, L["wqkv"], pos, self.cos_sin, hl, kl, D, slot_tok, cache.k(li), cache.v(li),
                                   kv_out=not kv_from_cache)
-            pre = None if prefix is None else (cache.k(li)[prefix[0]], cache.v(li)[prefix[0]], prefix[1])
+            if prefix is None:
+                pre = None
+            elif four:
+                pre = (*o.cache4_read(cache.layer(li), *prefix), prefix[1])
+            else:
+                pre = (cache.k(li)[prefix[0]], cache.v(li)[prefix[0]], prefix[1])
             if kv_from_cache:
                 a = o.flash_attn_varlen(qkv[:, :hl * D], None, None, cu, max_seqlen, hl, kl, D, causal=True,
                                         prefix=pre, kv_cache=(cache.k(li), cache.v(li), slot_tok, pos))
@@ -393,6 +459,8 @@ class LlamaDecoder:
         c, o, cache = self.cfg, self.ops, self.cache
         D, hl, kl = c.head_dim, self.hl, self.kl
         x = o.embed(st.tokens, self.w["embed"], out=st.x)
+        if self.kv_keep:
+            torch.sub(st.lens, 1, out=st.at)  # the new key's place: not its position once keys have been evicted
         if self._dk_decode(x.shape[0]):
             return self._decode_step_dk(st, x)
         if self._norm_fusable(x.shape[0]):
@@ -411,7 +479,7 @@ class LlamaDecoder:
         logits = self._logits(x, gather=False, out=st.logits)  # straight into the state (no copy launch)
         if logits.data_ptr() != st.logits.data_ptr():
             st.logits.copy_(logits)
-        self.sample(st.logits, st.temperature, st.seed, 0, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
+        self.sample(st.logits, st.temperature, st.seed, 0, filters=st.filters, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
                     active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
         return st.tokens
 
@@ -421,6 +489,11 @@ class LlamaDecoder:
         kernel, for rows whose projection does not rotate them itself (``dk_rope_fits``: one row, more than 64, a TP slice)."""
         c, o, cache = self.cfg, self.ops, self.cache
         D, hl, kl = c.head_dim, self.hl, self.kl
+        if self.kv_bits == 4:
+            c4, w = cache.layer(li), cache.weight_of(li)
+            o.rope_cache4(qkv, st.pos, self.cos_sin, hl, kl, D, st.slot, st.pos if w is None else st.at, c4, w)
+            return o.decode_attn4(qkv, c4, st.lens, st.slot, hl, kl, D, max_len=cache.max_seq, out=st.attn,
+                                  pre=st.pre if w is None else None, weight=w)
         if hl == kl and _FUSED_ROPE_DECODE:
             return o.decode_attn(qkv, cache.k(li), cache.v(li), st.lens, st.slot, hl, kl, D, max_len=cache.max_seq,
                                  pre=st.pre, rope=(self.cos_sin, st.pos), out=st.attn)
@@ -457,7 +530,7 @@ class LlamaDecoder:
         a_in, norm = o.rmsnorm(x, layers[0]["ln_attn"], c.eps, out=st.h), None
         D, hl, kl, cache = c.head_dim, self.hl, self.kl, self.cache
         # GQA: the rotation and the cache write ride in the projection (MHA: in the attention kernel)
-        rotated = hl != kl and _FUSED_ROPE_DECODE and o.dk_rope_fits(x.shape[0], *layers[0]["wqkv"].shape, a_in.stride(0))
+        rotated = self.kv_bits == 16 and hl != kl and _FUSED_ROPE_DECODE and o.dk_rope_fits(x.shape[0], *layers[0]["wqkv"].shape, a_in.stride(0))
         for li, L in enumerate(layers):
             if rotated:
                 qkv = o.gemm_dk_rope(a_in, L["wqkv"], st.pos, self.cos_sin, hl, kl, D, st.slot, cache.k(li), cache.v(li),
@@ -472,8 +545,8 @@ class LlamaDecoder:
             o.gemm_dk(g, L["w_down"], epi=EPI_RESID, resid=x, out=x, ssq_out=sb)           # x += mlp
             a_in, norm = x, (sb, parts, c.eps)
         o.gemm_dk(x, self.w["lm_head"], out=st.logits, norm_in=norm)                      # final norm deferred
-        o.sample(st.logits, st.temperature, st.seed, 0, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
-                 active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
+        self.sample(st.logits, st.temperature, st.seed, 0, filters=st.filters, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
+                    active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
         return st.tokens
 
     def _decode_step_fused_norms(self, st: "DecodeState", x: torch.Tensor) -> torch.Tensor:
@@ -489,8 +562,8 @@ class LlamaDecoder:
             nxt = layers[li + 1]["ln_attn"] if li + 1 < len(layers) else self.w["norm"]
             h = o.gemm_resid_norm(g, L["w_down"], x, nxt, c.eps, out=x, h_out=st.h)       # x += mlp; h = norm(x)
         st.logits.copy_(o.gemm(h, self.w["lm_head"]))  # h already carries the final norm
-        o.sample(st.logits, st.temperature, st.seed, 0, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
-                 active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
+        self.sample(st.logits, st.temperature, st.seed, 0, filters=st.filters, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
+                    active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
         return st.tokens
 
     def _decode_step_tp_fused_norms(self, st: "DecodeState", x: torch.Tensor) -> torch.Tensor:
@@ -517,7 +590,7 @@ class LlamaDecoder:
             nxt = layers[li + 1]["ln_attn"] if li + 1 < len(layers) else self.w["norm"]
             h = tp.all_reduce_norm_(x, nxt, c.eps, st.h, o)
         st.logits.copy_(o.gemm(h, self.w["lm_head"]))  # h already carries the final norm; local vocab slice
-        self.sample(st.logits, st.temperature, st.seed, 0, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
+        self.sample(st.logits, st.temperature, st.seed, 0, filters=st.filters, out_tok=st.tokens, out_lp=st.lp, conf=st.conf,
                     active=st.active, ctr=st.pos, pos=st.pos, lens=st.lens, hist=st.hist, start=st.start, eos=st.eos)
         return st.tokens
 
@@ -534,7 +607,7 @@ class LlamaDecoder:
 class DecodeState:
     """Static device buffers for a batch bucket of B sequences (HIP-graph friendly)."""
 
-    def __init__(self, model, B: int, max_new: int, temperature: float, seed: int, eos=()):
+    def __init__(self, model, B: int, max_new: int, temperature: float, seed: int, eos=(), filters=None):
         dev = model.device
         i32 = dict(dtype=torch.int32, device=dev)
         self.B = B
@@ -550,6 +623,7 @@ class DecodeState:
         self.lp = torch.zeros(B, dtype=torch.float32, device=dev)
         self.__dict__.update(model.decode_buffers(B))
         self.temperature, self.seed, self.eos = temperature, seed, tuple(eos)[:4]
+        self.filters = filters  # top_k / top_p / min_p of the sampler, None without
         self.graph = None
 
     def rows(self, b: int) -> "DecodeState":

@@ -569,7 +569,7 @@ DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void*
 }
 
 // ------------------------------------------------------------------------------------------- eviction
-// Of a sequence's n > keep keys a KV head keeps the `recent` last ones and of the others the keep - recent of largest weight
+// Of the n keys of a sequence that is too long a KV head keeps the `recent` last ones and of the others the keep - recent of largest weight
 // (equal ones: the earlier), in their order, at the front of its slot or of another. A workgroup per (KV head, row, layer):
 //   select  the smallest kept weight as a 32-bit key whose order is the weight's, 11 bits a pass, counted in LDS
 //   list    of 4096 keys at a time the kept ones', by two sums over the workgroup (8 neighbours a thread)
@@ -581,7 +581,7 @@ struct Evict4 {
   float* weight;
   const int *lens, *slot, *to;
   int* out;
-  int keep, recent;
+  int keep, recent, above;  // sequences of more than `above` keys are shortened to `keep`
   long layer;  // rows of a layer
 };
 
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int s = p.slot[b], d = p.to[b];
   const int n = (unsigned)s < (unsigned)p.c.slots && (unsigned)d < (unsigned)p.c.slots ? max(0, min(p.lens[b], p.c.max_seq)) : 0;
-  const int keep = min(n, p.keep);
+  const int keep = n > p.above ? min(n, p.keep) : n;
   if (blockIdx.z == 0 && hk == 0 && tid == 0) p.out[b] = keep;
   if (keep == 0 || (keep == n && s == d)) return;
   const long from = blockIdx.z * p.layer + row_of(p.c, s, hk, 0), to = blockIdx.z * p.layer + row_of(p.c, d, hk, 0);
@@ -737,11 +737,11 @@ __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
 
 DA_EXPORT int da_cache4_evict(void* ck, void* cks, void* cv, void* cvs, void* weight, const void* lens, const void* slot,
                               const void* to, void* out, int layers, int B, int Hkv, int D, int slots, int max_seq, int keep,
-                              int recent, void* stream) {
-  if (D % 32 || D < 64 || D > 128 || keep < 0 || recent < 0 || recent > keep || B > 65535 || layers > 65535) return (int)hipErrorInvalidValue;
+                              int recent, int above, void* stream) {
+  if (D % 32 || D < 64 || D > 128 || keep < 0 || recent < 0 || recent > keep || above < keep || B > 65535 || layers > 65535) return (int)hipErrorInvalidValue;
   if (B == 0 || layers == 0) return 0;
   Evict4 p{{(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq}, (float*)weight, (const int*)lens,
-           (const int*)slot, (const int*)to, (int*)out, keep, recent, (long)slots * Hkv * max_seq};
+           (const int*)slot, (const int*)to, (int*)out, keep, recent, above, (long)slots * Hkv * max_seq};
   const dim3 grid(Hkv, B, layers);
   hipStream_t st = (hipStream_t)stream;
   if (D == 64) cache4_evict_kernel<64><<<grid, EV_T, 0, st>>>(p);

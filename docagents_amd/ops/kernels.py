@@ -125,7 +125,7 @@ _SIGS = {
     "da_sample_filtered_ws": [c_int] * 2,
     "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 9 + [c_int] * 6 + [c_void_p],
     "da_cache4_read": [c_void_p] * 4 + [c_int] * 6 + [c_void_p] * 3,
-    "da_cache4_evict": [c_void_p] * 9 + [c_int] * 8 + [c_void_p],
+    "da_cache4_evict": [c_void_p] * 9 + [c_int] * 9 + [c_void_p],
     "da_decode_attn4": [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 9 + [c_float] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p],
     "da_decode_attn4_ws": [c_int] * 6,
 }
@@ -2103,8 +2103,8 @@ def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: in
     return out
 
 
-def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None, out=None):
-    """Shorten sequences of more than ``keep`` keys to that many: each KV head of each layer keeps the ``recent`` last keys and of
+def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None, out=None, above: int | None = None):
+    """Shorten sequences of more than ``above`` (None: ``keep``) keys to ``keep``: each KV head of each layer keeps the ``recent`` last keys and of
     the others those of largest accumulated ``weight`` (fp32 [layers,] slots, Hkv, max_seq; equal ones: the earlier; NaN least),
     in their order, with their weights. lens / slot int32 [B]; the kept rows go to the front of the same slot, or of slots ``to``
     (then shorter sequences are copied too). What lies behind them is left as it was. Slots, and those of ``to``, are distinct.
@@ -2114,10 +2114,11 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     B = lens.numel()
     wa, la, sa = _weight4(weight, c, dev), _ints(lens, B, dev, "lens"), _ints(slot, B, dev, "slot")
     ta = sa if to is None else _ints(to, B, dev, "to")
-    _req(0 <= recent <= keep, "0 <= recent <= keep")
+    above = keep if above is None else above
+    _req(0 <= recent <= keep <= above, "0 <= recent <= keep <= above")
     if out is None:
         out = torch.empty_like(lens)
     oa = _ints(out, B, dev, "out"); _req(oa != la or B == 0, "out: int32 [B] apart from lens")
     _check(lib().da_cache4_evict(*map(_at, c), wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
-                                 min(keep, max_seq), min(recent, max_seq), _raw_stream()), "cache4_evict")
+                                 min(keep, max_seq), min(recent, max_seq), min(above, max_seq), _raw_stream()), "cache4_evict")
     return out

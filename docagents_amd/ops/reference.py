@@ -694,19 +694,20 @@ def decode_attn4(q, c, lens, slot, H, Hkv, D, max_len=None, scale=None, out=None
     return res
 
 
-def cache4_evict(c, weight, lens, slot, keep: int, recent: int, to=None, out=None):
+def cache4_evict(c, weight, lens, slot, keep: int, recent: int, to=None, out=None, above=None):
     layered = c.k.dim() == 5
     out = torch.empty_like(lens) if out is None else out
     to = slot if to is None else to
     for b in range(lens.numel()):
         n, s, d = int(lens[b]), int(slot[b]), int(to[b])
-        out[b] = min(n, keep)
+        n_kept = min(n, keep) if n > (keep if above is None else above) else n
+        out[b] = n_kept
         for layer in range(c.k.shape[0] if layered else 1):
             w = (weight[layer] if layered else weight)
             one = c.layer(layer) if layered else c
             for h in range(c.k.shape[-3]):
                 pick = torch.arange(n, device=w.device)
-                if n > keep:
+                if n > n_kept:
                     m = n - recent
                     x = w[s, h, :m]
                     x = torch.where(x.isnan(), torch.full_like(x, float("-inf")), x)

@@ -1,0 +1,99 @@
+"""A decode step's operators over a long context as they are used together: decoders with a 4-bit cache, shortened sequences and
+filtered sampling, on captured graphs."""
+import pytest
+import torch
+
+from docagents_amd.engine.generator import ContinuousScheduler, Generator
+from docagents_amd.models import make_decoder
+from docagents_amd.models.configs import DecoderConfig
+from docagents_amd.ops import reference as R
+
+pytestmark = pytest.mark.gpu
+
+# heads of 64, 96 and 128; with and without shared KV heads
+CFGS = {D: DecoderConfig(f"tiny-{D}", vocab=1024, hidden=4 * D, layers=2, heads=4, kv_heads=kv, ffn=256, max_pos=1024, rope_theta=1e4)
+        for D, kv in ((64, 2), (96, 4), (128, 1))}
+
+
+def _decoder(D, **kw):
+    return make_decoder(CFGS[D], "cuda", seed=3, **kw)
+
+
+def _prompts(n):
+    g = torch.Generator().manual_seed(n)
+    return [torch.randint(0, 1024, (k,), generator=g).tolist() for k in (1, 7, 70, 33)[:n]]
+
+
+@pytest.mark.parametrize("D", sorted(CFGS))
+def test_a_step_is_the_oracles(D):
+    """One layer's new key and its attention in the decoder's own cache against the oracle's on a copy of that cache."""
+    from docagents_amd.ops import kernels as K
+    m = _decoder(D, kv_bits=4, kv_keep=400, kv_recent=20)
+    c, g = CFGS[D], torch.Generator().manual_seed(D)
+    gen = Generator(m, max_batch=4, max_seq=512, temperature=0.0, use_graphs=False)
+    gen.generate(_prompts(4), 6)
+    cache = m.cache.layer(1)
+    one = R.Cache4(*(t.cpu().clone() for t in cache))
+    w, wg = m.cache.weight[1].cpu().clone(), m.cache.weight[1].clone()
+    hl, kl = c.heads, c.kv_heads
+    qkv = torch.randn(3, (hl + 2 * kl) * D, generator=g).bfloat16()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    pos, at, slot, lens = i32(70, 300, 12), i32(70, 30, 12), i32(0, 1, 2), i32(71, 31, 13)
+    want_q = R.rope_cache4(qkv.clone(), pos, m.cos_sin.cpu(), hl, kl, D, slot, at, one, w)
+    want = R.decode_attn4(want_q, one, lens, slot, hl, kl, D, weight=w)
+    got_q = K.rope_cache4(qkv.cuda(), pos.cuda(), m.cos_sin, hl, kl, D, slot.cuda(), at.cuda(), cache, wg)
+    got = K.decode_attn4(got_q, cache, lens.cuda(), slot.cuda(), hl, kl, D, 512, weight=wg)
+    # the rotation's last bit may round the other way (2^-8 of a value), and a code with it: a key's score moves by 2^-8 of |q||k|
+    # at most, small against what the two roundings of the output and of the weights allow together
+    assert (got_q.cpu().float() - want_q.float()).abs().max() <= 2 ** -7 * want_q.float().abs().max()
+    assert torch.allclose(got.cpu().float(), want.float(), rtol=2 ** -6, atol=2 ** -6 * float(want.float().abs().max()))
+    assert torch.allclose(wg.cpu(), w, rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("D", sorted(CFGS))
+def test_graphs_and_scheduler_give_the_eager_tokens(D):
+    kw = dict(max_batch=4, max_seq=512, temperature=0.9, seed=5, top_k=30, top_p=0.9, min_p=0.01)
+    eager = [r.tokens for r in Generator(_decoder(D, kv_bits=4), use_graphs=False, **kw).generate(_prompts(4), 12)]
+    gen = Generator(_decoder(D, kv_bits=4), **kw)
+    for _ in range(3):  # (the graph's own replays, with other work between them)
+        assert [r.tokens for r in gen.generate(_prompts(4), 12)] == eager
+        torch.cuda.synchronize()
+        gen.generate(_prompts(1), 3)
+    m = _decoder(D, kv_bits=4)
+    m.alloc_cache(8, 512)
+    sched = ContinuousScheduler(Generator(m, **kw), B=4, max_new_cap=16)
+    assert all(len(r.tokens) >= 1 for r in sched.run_all(_prompts(4), 12))
+
+
+@pytest.mark.parametrize("D", sorted(CFGS))
+def test_sequences_past_their_slots(D):
+    """Slots of 96 places, 200 tokens: eager and captured steps shorten at the same steps and give the same tokens."""
+    kw = dict(max_batch=4, max_seq=96, temperature=0.7, seed=2, top_p=0.95)
+    keep = dict(kv_bits=4, kv_keep=48, kv_recent=16)
+    eager = Generator(_decoder(D, **keep), use_graphs=False, **kw).generate(_prompts(4), 200)
+    gen = Generator(_decoder(D, **keep), **kw)
+    got = gen.generate(_prompts(4), 200)
+    assert [r.tokens for r in got] == [r.tokens for r in eager]
+    assert [r.n_tokens for r in got] == [200] * 4
+    for st in gen.states.values():
+        assert int(st.lens.max()) <= 96
+    m = _decoder(D, **keep)
+    m.alloc_cache(8, 96)
+    sched = ContinuousScheduler(Generator(m, **kw), B=4, max_new_cap=200)
+    assert [r.n_tokens for r in sched.run_all(_prompts(4), 200)] == [200] * 4
+
+
+def test_a_shared_head_in_four_bits():
+    head = list(range(100, 100 + 128))
+    prompts = [head + p for p in _prompts(3)]
+    m = _decoder(128, kv_bits=4)
+    gen = Generator(m, max_batch=4, max_seq=512, temperature=0.0)
+    got = gen.generate(prompts, 6)
+    assert gen.stats["shared_prefix_tokens"] > 0 and all(r.n_tokens == 6 for r in got)
+
+
+def test_first_tokens_are_those_of_a_bf16_cache():
+    """A prompt's attention is over its own keys as they are: the first token does not depend on the cache's bits."""
+    for D in sorted(CFGS):
+        a, b = (Generator(_decoder(D, kv_bits=bits), max_batch=4, max_seq=256, temperature=0.0).generate(_prompts(4), 1) for bits in (4, 16))
+        assert [r.tokens for r in a] == [r.tokens for r in b]
