@@ -332,9 +332,11 @@ class LlamaDecoder:
 
     def evict(self, st: "DecodeState", above: int) -> None:
         """Shorten the rows of a decode state whose sequences have more than ``above`` keys to ``kv_keep`` (all layers; the
-        lengths follow, the positions go on)."""
+        lengths follow, the positions go on). A row's length counts the token that the next step will write."""
         c = self.cache
-        st.lens.copy_(self.ops.cache4_evict(c.all, c.weight, st.lens, st.slot, self.kv_keep, self.kv_recent, above=above))
+        torch.sub(st.lens, 1, out=st.at)
+        n = self.ops.cache4_evict(c.all, c.weight, st.at, st.slot, self.kv_keep, self.kv_recent, above=above)
+        torch.add(n, 1, out=st.lens)
 
     def workspace_bytes(self, max_batch: int, max_seq: int) -> int:
         return decode_workspace_bytes(self.cfg, self.hl, self.tp.size, max_batch, max_seq)

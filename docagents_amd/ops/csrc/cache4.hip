@@ -52,7 +52,7 @@ __device__ __forceinline__ unsigned encode8(const u32x4_t& x, unsigned& sb) {
 
 struct Write4 {
   bf16_t *q, *k, *v;  // rows of T tokens; q only with cs
-  int ldk, ldv, T, H, D;
+  int ldk, ldv, T, H, D, npos;  // npos: rows of cs
   const int *slot, *at, *pos;
   const float* cs;
   float* weight;
@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(256) cache4_write_kernel(Write4 p) {
   for (int i = 0; i < W4_T; ++i) {
     const int t = t0 + i;
     if (t >= p.T) return;
+    if (p.cs && (unsigned)p.pos[t] >= (unsigned)p.npos) continue;
     if (p.cs && (is_q || is_k) && in) {
       const float* f = p.cs + ((long)p.pos[t] * (p.D / 2) + c * 4) * 2;
       const f32x4_t c01 = *(const f32x4_t*)f, c23 = *(const f32x4_t*)(f + 4);
@@ -129,13 +130,13 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(Cache4 c, int slot, in
 }
 
 DA_EXPORT int da_cache4_write(void* q, void* k, void* v, int ldk, int ldv, const void* slot, const void* at, const void* pos,
-                              const void* cs, void* ck, void* cks, void* cv, void* cvs, void* weight, int T, int H, int Hkv,
-                              int D, int slots, int max_seq, void* stream) {
+                              const void* cs, int npos, void* ck, void* cks, void* cv, void* cvs, void* weight, int T, int H,
+                              int Hkv, int D, int slots, int max_seq, void* stream) {
   if (D % 32 || D < 32 || D > 128 || (cs && (!pos || !q)) || (!cs && H)) return (int)hipErrorInvalidValue;
   if (T == 0) return 0;
   const long rows = H + 2l * Hkv, wgs = (rows * (D == 64 ? 8 : 16) + 255) / 256;
   if (wgs > 65535) return (int)hipErrorInvalidValue;
-  Write4 p{(bf16_t*)q, (bf16_t*)k, (bf16_t*)v, ldk, ldv, T, H, D, (const int*)slot, (const int*)at, (const int*)pos,
+  Write4 p{(bf16_t*)q, (bf16_t*)k, (bf16_t*)v, ldk, ldv, T, H, D, npos, (const int*)slot, (const int*)at, (const int*)pos,
            (const float*)cs, (float*)weight, {(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq}};
   cache4_write_kernel<<<dim3((T + W4_T - 1) / W4_T, (unsigned)wgs), 256, 0, (hipStream_t)stream>>>(p);
   DA_LAUNCH_CHECK();
@@ -194,10 +195,11 @@ __device__ __forceinline__ float get4(const float* p) { return __hip_atomic_load
 template <int D>
 __device__ __forceinline__ void join4(const Attn4& a, long at, int act, int d, int s0, int step, float& M, float& sum, float& acc) {
   M = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int s = s0; s < act; s += 8 * step) {
-    float ms[8], ls[8], os[8];
+  constexpr int U = 12;  // splits that are joined in the launch have one round trip
+  for (int s = s0; s < act; s += U * step) {
+    float ms[U], ls[U], os[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < U; ++j) {
       const int x = min(s + j * step, act - 1);
       ms[j] = s + j * step < act ? get4(a.pm + at + x) : -INFINITY;
       ls[j] = get4(a.pl + at + x);
@@ -205,13 +207,13 @@ __device__ __forceinline__ void join4(const Attn4& a, long at, int act, int d, i
     }
     float mx = M;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, ms[j]);
+    for (int j = 0; j < U; ++j) mx = fmaxf(mx, ms[j]);
     if (mx == -INFINITY) continue;
     const float r = exp2f(M - mx);
     sum *= r;
     acc *= r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < U; ++j) {
       const float e = exp2f(ms[j] - mx);
       sum += ls[j] * e;
       acc += os[j] * e;

@@ -123,7 +123,7 @@ _SIGS = {
     "da_sample_filtered": [c_void_p] + [c_int] * 4 + [ctypes.c_double] * 3 + [c_int] + [c_void_p] * 5 + [c_uint, c_uint] + [c_void_p] * 10
                           + [c_int] * 5 + [c_void_p],
     "da_sample_filtered_ws": [c_int] * 2,
-    "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 9 + [c_int] * 6 + [c_void_p],
+    "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_int] * 6 + [c_void_p],
     "da_cache4_read": [c_void_p] * 4 + [c_int] * 6 + [c_void_p] * 3,
     "da_cache4_evict": [c_void_p] * 9 + [c_int] * 9 + [c_void_p],
     "da_decode_attn4": [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 9 + [c_float] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p],
@@ -2024,14 +2024,15 @@ def cache4_write(k, v, c: Cache4, slot, at, weight=None) -> None:
     (ka, kl), (va, vl) = _rows16(k, Hkv * D, dev, "k"), _rows16(v, Hkv * D, dev, "v")
     T = k.shape[0]
     _req(v.shape[0] == T and k.shape[1] == v.shape[1] == Hkv * D, "k and v: the same tokens, [T, Hkv * D]")
-    _check(lib().da_cache4_write(None, ka, va, kl, vl, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"), None, None, *map(_at, c),
+    _check(lib().da_cache4_write(None, ka, va, kl, vl, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"), None, None, 0, *map(_at, c),
                                  None if weight is None else _weight4(weight, c, dev), T, 0, Hkv, D, slots, max_seq, _raw_stream()),
            "cache4_write")
 
 
 def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4, weight=None):
     """``rope_cache`` with a 4-bit cache: q and k heads of qkv [T, (H + 2 Hkv) * D] rotated in place (by position ``pos``), k
-    and v written as ``cache4_write`` writes them, to places ``at`` (which are not the positions once keys have been evicted)."""
+    and v written as ``cache4_write`` writes them, to places ``at`` (which are not the positions once keys have been evicted).
+    A token whose position lies outside the table is left as it is, and not written."""
     dev, Hc, Dc, slots, max_seq = _cache4(c)
     q, ld = _rows16(qkv, (H + 2 * Hkv) * D, dev, "qkv")
     T = qkv.shape[0]
@@ -2040,7 +2041,7 @@ def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4
          and cos_sin.shape[1] == D // 2, "cos_sin must be fp32 [max_pos, D/2, 2]")
     ld = qkv.shape[1]
     _check(lib().da_cache4_write(q, q + 2 * H * D, q + 2 * (H + Hkv) * D, ld, ld, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"),
-                                 _ints(pos, T, dev, "pos"), cos_sin.data_ptr(), *map(_at, c),
+                                 _ints(pos, T, dev, "pos"), cos_sin.data_ptr(), cos_sin.shape[0], *map(_at, c),
                                  None if weight is None else _weight4(weight, c, dev), T, H, Hkv, D, slots, max_seq, _raw_stream()),
            "rope_cache4")
     return qkv

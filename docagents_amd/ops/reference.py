@@ -660,8 +660,10 @@ def cache4_write(k, v, c, slot, at, weight=None):
 
 
 def rope_cache4(qkv, pos, cos_sin, H, Hkv, D, slot, at, c, weight=None):
-    rope_cache(qkv, pos, cos_sin, H, Hkv, D)
-    cache4_write(qkv[:, H * D:(H + Hkv) * D], qkv[:, (H + Hkv) * D:], c, slot, at, weight)
+    T = qkv.shape[0]
+    ok = (pos[:T] >= 0) & (pos[:T] < cos_sin.shape[0])
+    qkv[ok] = rope_cache(qkv[ok], pos[:T][ok], cos_sin, H, Hkv, D)
+    cache4_write(qkv[ok][:, H * D:(H + Hkv) * D], qkv[ok][:, (H + Hkv) * D:], c, slot[:T][ok], at[:T][ok], weight)
     return qkv
 
 

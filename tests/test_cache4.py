@@ -175,7 +175,7 @@ def test_generation_past_the_slot():
     out = gen.generate([[5, 9, 2, 77, 31], [4] * 30], 70)
     assert [r.n_tokens for r in out] == [70, 70]
     st = next(iter(gen.states.values()))
-    assert int(st.lens.max()) <= 48 and int(st.pos[0]) >= 70
+    assert int(st.lens.max()) <= 49 and int(st.pos[0]) >= 70  # (with the token that the next step would write)
     m2 = _decoder(**kw)
     m2.alloc_cache(6, 48)
     sched = ContinuousScheduler(Generator(m2, max_batch=2, max_seq=48, temperature=0.0, check_every=8), B=2, max_new_cap=70)
@@ -184,6 +184,29 @@ def test_generation_past_the_slot():
     # until the first eviction (more than 40 keys) the tokens are those of a slot that holds everything
     big = Generator(_decoder(kv_bits=4), max_batch=2, max_seq=256, temperature=0.0).generate([[5, 9, 2, 77, 31]], 30)[0]
     assert out[0].tokens[:30] == big.tokens
+
+
+@pytest.mark.parametrize("recent", [0, 1, 8])
+def test_only_written_keys_are_kept(recent):
+    """Between steps the last place of a sequence is empty (the next step's); what lies there from before is no key."""
+    m = _decoder(kv_bits=4, kv_keep=12, kv_recent=recent)
+    gen = Generator(m, max_batch=1, max_seq=64, temperature=0.0, check_every=64 - 13)
+    gen.evict_above = 64  # (this test shortens by itself)
+    gen.generate([[5, 9, 2, 77, 31]], 26)
+    st = next(iter(gen.states.values()))
+    n, slot = int(st.lens[0]) - 1, int(st.slot[0])
+    assert n == int(st.pos[0]) == 30
+    for t in (m.cache.weight,):
+        t[:, slot, :, n:] = 1e9  # another sequence's, behind the end
+    before = m.cache.all.k[:, slot, :, :n].clone()
+    w = m.cache.weight[:, slot, :, :n].clone()
+    m.evict(st, 20)
+    assert int(st.lens[0]) == 13 and int(st.pos[0]) == 30
+    after = m.cache.all.k[:, slot, :, :12]
+    for layer in range(m.cfg.layers):
+        x = w[layer, 0]
+        want = sorted([*torch.argsort(x[:n - recent], descending=True, stable=True)[:12 - recent].tolist(), *range(n - recent, n)])
+        assert torch.equal(after[layer, 0], before[layer, 0, want])
 
 
 def test_what_does_not_fit_is_refused():

@@ -103,6 +103,21 @@ def test_rope_write_is_rope_cache_and_write(K, H, Hkv, D):
         assert torch.equal(x, y)
 
 
+def test_positions_outside_the_table(K):
+    """Neither rotated nor written; the others are."""
+    g = torch.Generator().manual_seed(8)
+    H, Hkv, D = 4, 2, 64
+    qkv = torch.randn(6, (H + 2 * Hkv) * D, generator=g).bfloat16()
+    pos = torch.tensor([3, -1, 31, 32, 10 ** 6, 0], dtype=torch.int32)
+    cs, z = R.rope_table(32, D, 10000.0), torch.zeros(6, dtype=torch.int32)
+    at = torch.arange(6, dtype=torch.int32)
+    c = K.new_cache4(1, Hkv, 8, D, DEV)
+    got = K.rope_cache4(qkv.to(DEV), pos.to(DEV), cs.to(DEV), H, Hkv, D, z.to(DEV), at.to(DEV), c)
+    bad = [1, 3, 4]
+    assert torch.equal(got[bad].cpu(), qkv[bad]) and not c.k[0, :, bad].any() and not c.v_scale[0, :, bad].any()
+    assert (got.cpu()[[0, 2]] != qkv[[0, 2]]).any(1).all() and all(c.k[0, 0, i].any() for i in (0, 2, 5))
+
+
 def _attend(K, g, B, Hkv, G, D, lens, max_seq, max_len, pre=None, weight=False):
     H = Hkv * G
     c, cg = _filled(K, g, B + 1, Hkv, max_seq, D)
@@ -222,3 +237,51 @@ def test_places_past_32_bits(K):
     for a, b in zip(K.cache4_read(c, slots - 1, 100), K.cache4_read(small, 0, 100)):
         assert torch.equal(a, b)
     assert torch.equal(w[-1, :, :100], ws[0, :, :100])
+
+
+def test_what_is_refused(K):
+    c = K.new_cache4(2, 2, 64, 64, DEV)
+    i = torch.zeros(4, dtype=torch.int32, device=DEV)
+    x = torch.zeros(4, 128, device=DEV).bfloat16()
+    w = torch.zeros(2, 2, 64, device=DEV)
+    q = torch.zeros(4, 256, device=DEV).bfloat16()
+    bad = [lambda: K.cache4_write(x.float(), x, c, i, i), lambda: K.cache4_write(x, x[:2], c, i, i), lambda: K.cache4_write(x, x, c, i[:3], i),
+           lambda: K.cache4_write(x, x, c, i.long(), i), lambda: K.cache4_write(x[:, :64], x, c, i, i), lambda: K.cache4_write(x.cpu(), x, c, i, i),
+           lambda: K.cache4_write(x, x, c, i, i, weight=w[:1]), lambda: K.cache4_write(x, x, c._replace(k=c.k[:, :1]), i, i),
+           lambda: K.cache4_write(x, x, c._replace(k_scale=c.k_scale[..., :2]), i, i),
+           lambda: K.cache4_write(x.view(-1)[4:388].view(3, 128), x[:3], c, i, i),
+           lambda: K.cache4_read(c, 2, 1), lambda: K.cache4_read(c, 0, 65), lambda: K.cache4_read(c, -1, 1),
+           lambda: K.decode_attn4(q, c, i, i, 4, 2, 128, 64), lambda: K.decode_attn4(q, c, i, i, 3, 2, 64, 64),
+           lambda: K.decode_attn4(q, c, i, i, 4, 2, 64, 65), lambda: K.decode_attn4(q, c, i, i, 4, 2, 64, 0),
+           lambda: K.decode_attn4(q, c, i[:3], i, 4, 2, 64, 64), lambda: K.decode_attn4(q, c, i, i, 68, 2, 64, 64),
+           lambda: K.decode_attn4(q, c, i, i, 4, 2, 64, 64, weight=w, pre=torch.zeros(4, 2, dtype=torch.int32, device=DEV)),
+           lambda: K.decode_attn4(q, c, i, i, 4, 2, 64, 64, weight=w.half()), lambda: K.decode_attn4(q, c, i, i, 4, 2, 64, 64, out=q[:, :128]),
+           lambda: K.cache4_evict(c, w, i, i, 4, 5), lambda: K.cache4_evict(c, w, i, i, 4, 2, above=3), lambda: K.cache4_evict(c, w, i, i[:2], 4, 2),
+           lambda: K.cache4_evict(c, w, i, i, 4, 2, out=i), lambda: K.cache4_evict(c, w[:, :1], i, i, 4, 2)]
+    for n, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("not refused:", n)
+    assert K.decode_attn4(q[:0], c, i[:0], i[:0], 4, 2, 64, 64).shape == (0, 256)
+    K.cache4_write(x[:0], x[:0], c, i[:0], i[:0])
+    assert K.cache4_evict(c, w, i[:0], i[:0], 4, 2).numel() == 0
+
+
+def test_evict_leaves_sequences_below_the_line(K):
+    g = torch.Generator().manual_seed(4)
+    c, cg = _filled(K, g, 3, 1, 300, 64)
+    w = torch.rand(3, 1, 300, generator=g)
+    lens, slot = torch.tensor([150, 200, 201], dtype=torch.int32), torch.tensor([2, 0, 1], dtype=torch.int32)
+    wg = w.to(DEV)
+    n = K.cache4_evict(cg, wg, lens.to(DEV), slot.to(DEV), 100, 10, above=200)
+    want = R.cache4_evict(c, w, lens, slot, 100, 10, above=200)
+    assert n.tolist() == want.tolist() == [150, 200, 100]
+    for a, b in zip((*c, w), (*cg, wg)):
+        assert torch.equal(a, b.cpu())
+
+
+def test_rows_without_a_slot_give_zeros(K):
+    c = K.new_cache4(2, 1, 64, 128, DEV)
+    q = torch.randn(3, 128, device=DEV).bfloat16()
+    n, s = torch.tensor([5, 64, 0], dtype=torch.int32, device=DEV), torch.tensor([-1, 2, 0], dtype=torch.int32, device=DEV)
+    assert not K.decode_attn4(q, c, n, s, 1, 1, 128, 64).any()

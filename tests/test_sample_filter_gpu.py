@@ -121,6 +121,32 @@ def test_rows_of_any_stride_and_address(K, f32):
         _same(K, x, torch.rand(4, generator=g), xg=xg, temperature=0.9, top_k=60, top_p=0.95)
 
 
+@pytest.mark.parametrize("V", [262143, 262144])
+def test_the_largest_vocabulary(K, V):
+    g = torch.Generator().manual_seed(V)
+    for f32 in (False, True):
+        x = _logits(g, 2, V, f32, 1.5)
+        for opts in (dict(top_k=50, top_p=0.9), dict(top_p=0.99), dict(), dict(top_k=100000)):
+            _same(K, x, torch.rand(2, generator=g), temperature=1.1, **opts)
+    with pytest.raises(ValueError, match="vocabulary"):
+        K.sample_filtered(torch.zeros(1, (1 << 18) + 1, device=DEV), 1.0, top_k=3)
+
+
+def test_what_is_refused(K):
+    x = torch.randn(3, 100, device=DEV)
+    for kw in (dict(temperature=torch.ones(3)), dict(temperature=torch.ones(2, device=DEV)), dict(temperature=1.0, top_k=torch.ones(3, device=DEV)),
+               dict(temperature=1.0, u=torch.rand(3, device=DEV, dtype=torch.float64)), dict(temperature=1.0, u=torch.rand(3)),
+               dict(temperature=1.0, out_tok=torch.zeros(3, device=DEV)), dict(temperature=1.0, conf=torch.zeros(3, 3, device=DEV)),
+               dict(temperature=1.0, hist=torch.zeros(3, 4, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            K.sample_filtered(x, **kw)
+    for y in (x.half(), x.double(), x[:, ::2], x.cpu()):
+        with pytest.raises(ValueError):
+            K.sample_filtered(y, 1.0, top_k=3)
+    tok, lp = K.sample_filtered(x[:0], 1.0, top_k=3)
+    assert tok.numel() == lp.numel() == 0
+
+
 def test_own_numbers_and_bookkeeping(K):
     """Without u: the oracle's counter-based numbers; inactive rows stay as they were."""
     g = torch.Generator().manual_seed(13)
