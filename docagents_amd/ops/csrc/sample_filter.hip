@@ -43,7 +43,7 @@ struct RowOpts { double T, p, m; int k; };  // k 0, p 1, m 0: off
 
 __device__ __forceinline__ RowOpts row_opts(const FilterArgs& a, int b) {
   RowOpts o{a.Ts ? (double)a.Ts[b] : a.T, a.ps ? (double)a.ps[b] : a.p, a.ms ? (double)a.ms[b] : a.m, a.ks ? a.ks[b] : a.k};
-  if (!(o.T > 0)) o = {1.0, 1.0, 0.0, 1};  // greedy: the first entry
+  if (!(o.T > 0) || o.m > 1) o = {1.0, 1.0, 0.0, 1};  // the first entry: greedy, or no weight passes min-p (which bins could not hold)
   if (o.k <= 0 || o.k >= a.s.V) o.k = 0;
   if (!(o.p < 1)) o.p = 1;
   if (!(o.m > 0)) o.m = 0;
@@ -391,7 +391,7 @@ __device__ __forceinline__ void find_bin(PickLds& S, const Goal& goal, unsigned 
 template <typename L>
 __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S, const Bins& r, const Goal& goal) {
   const int tid = threadIdx.x;
-  const unsigned bin = S.bin, above = S.c_above, n = S.c_at;
+  const unsigned bin = S.bin, above = S.c_above;
   const double m_above = (double)S.m_above;
   if (tid == 0) S.n_list = 0;
   // the bin's keys, from the first of it to before the first of the bin above: 64 keys of a range at a time
@@ -415,6 +415,7 @@ __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S,
   const unsigned from = S.range[0], to = S.range[1];
   collect(row, V, S, from, to, false);
   __syncthreads();
+  const unsigned n = min(S.n_list, (unsigned)SF_CAP);
   sort_list(S, n);
   double w[2], sum = 0;
 #pragma unroll

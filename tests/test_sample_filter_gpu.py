@@ -76,7 +76,8 @@ def test_equal_logits(K, f32):
     x[4, ::2] = -0.0
     x[5, 17000:] = 3.0
     x = x if f32 else x.bfloat16()
-    for opts in (dict(), dict(top_k=5), dict(top_k=9000), dict(top_p=0.5), dict(top_p=0.25, top_k=8000), dict(min_p=0.9), dict(top_k=15000, top_p=0.9, min_p=0.3)):
+    for opts in (dict(), dict(top_k=5), dict(top_k=9000), dict(top_p=0.5), dict(top_p=0.25, top_k=8000), dict(min_p=0.9), dict(min_p=1.0), dict(min_p=1.5),
+                 dict(top_k=15000, top_p=0.9, min_p=0.3), dict(top_k=15000, top_p=0.9, min_p=1.5)):
         for _ in range(2):
             _same(K, x, torch.rand(B, generator=g), temperature=1.0, **opts)
 
