@@ -22,8 +22,9 @@ __device__ __forceinline__ unsigned bf2_of4(unsigned w, float scale) {
   return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, B));
 }
 
+// Byte `at` as the scale of a conversion: turned to where an exponent is; what else is in the word does not count
 __device__ __forceinline__ float scale_of(unsigned bytes, int at) {
-  return __uint_as_float(((bytes >> (8 * at)) & 255) << 23);  // (the conversion takes the exponent; 255 gives NaN)
+  return __uint_as_float(__builtin_amdgcn_alignbit(bytes, bytes, (8 * at + 9) & 31));  // (the conversion takes bits 23 - 30; 255: NaN)
 }
 
 __device__ __forceinline__ long row_of(const Cache4& c, int slot, int h, int at) {
@@ -172,6 +173,7 @@ struct Attn4 {
   int B, H, max_len, nsplit, keys, ldo;
   float scale_log2e;
   float *po, *pm, *pl;  // of the splits
+  float* plw;           // their sums of unrounded weights, or null
   float* sc;            // scores [B, H, ld_sc] (log2; 16 keys as 4 f + i for 4 i + f), or null
   int ld_sc;
   float* weight;
@@ -278,14 +280,14 @@ __device__ __forceinline__ void read_v4(unsigned at, unsigned at_s, unsigned (&v
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int D>
+template <int D, bool W>
 __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   constexpr int CH = D / 32, VB = D / 32, NT = D / 16, RB = D / 2, KT = 64;
   constexpr int ST = 1, ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4, STAGE = 2 * HALF;  // DMA instructions, bytes of K or V
   typedef __attribute__((address_space(3))) void* lds_t;
   constexpr int SO = 4 * 16 * (D + 1) * 4, RING = 4 * ST * STAGE;
   __shared__ __attribute__((aligned(16))) char ring[(SO > RING ? SO : RING) + 16];
-  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float sm[4][16], sl[4][16], slw[W ? 4 : 1][16];
   __shared__ int last;
   const int hk = blockIdx.x, b = blockIdx.y, split = blockIdx.z, G = a.H / a.c.Hkv;
   const int L = len4(a, b), act = splits4(a, L);
@@ -306,7 +308,10 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   bf16x8_t qf[CH];
 #pragma unroll
   for (int t = 0; t < CH; ++t)
-    qf[t] = c < G ? *(const bf16x8_t*)(a.q + (long)b * a.ldq + (hk * G + c) * D + (f * CH + t) * 8) : bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    qf[t] = c < G && a.scale_log2e != 0.f ? *(const bf16x8_t*)(a.q + (long)b * a.ldq + (hk * G + c) * D + (f * CH + t) * 8) : bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+  // the scale is applied behind the largest score's choice: a positive one (q takes the sign, and the 0)
+  const float scale = a.scale_log2e != 0.f ? fabsf(a.scale_log2e) : 1.f;
+  const short flip = a.scale_log2e < 0.f ? (short)0x8000 : (short)0;
 
   // K rows of 64 bytes: the 16-byte pieces of a row are exchanged by its number, so that 16 rows' pieces are in all banks
   unsigned ko[4];  // (ND of them)
@@ -332,7 +337,8 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   f32x4_t o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  f32x4_t ol = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // m of the scores before their scale
   const int kr = 4 * (c & 3) + (c >> 2);  // the lane's key of 16
 
 #pragma unroll
@@ -341,7 +347,10 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     issue(a.c.v, a.c.vs, false, kstart + (w + 4 * i) * KT, mine + i * STAGE + HALF);
   }
 #pragma unroll
-  for (int t = 0; t < CH; ++t) asm volatile("" : "+v"(qf[t]));
+  for (int t = 0; t < CH; ++t) {
+    qf[t] ^= bf16x8_t{flip, flip, flip, flip, flip, flip, flip, flip};
+    asm volatile("" : "+v"(qf[t]));
+  }
   int stage = 0;
   for (int t0 = kstart + w * KT; t0 < kend; t0 += 4 * KT) {
     char* kt = mine + stage * STAGE;
@@ -368,31 +377,32 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[tt][i] = whole || t0 + 16 * tt + 4 * i + f < kend ? s[tt][i] * a.scale_log2e : -INFINITY;
+        if (!whole && t0 + 16 * tt + 4 * i + f >= kend) s[tt][i] = -INFINITY;
         mx = fmaxf(mx, s[tt][i]);
       }
-    if (a.sc && c < G) {
+    if (W && c < G) {
       float* to = a.sc + ((long)b * a.H + hk * G + c) * a.ld_sc + t0 + 4 * f;
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) *(f32x4_t*)(to + 16 * tt) = s[tt];
+      for (int tt = 0; tt < 4; ++tt) *(f32x4_t*)(to + 16 * tt) = s[tt] * scale;
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = max_xhalf(mx);
     if (__ballot(mx > m)) {  // (a new maximum is rare after the first tiles)
-      const float mn = fmaxf(m, mx), alpha = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      const float mn = fmaxf(m, mx), alpha = exp2f((m - (mn == -INFINITY ? 0.f : mn)) * scale);
       m = mn;
-      l *= alpha;
+      if constexpr (W) l *= alpha;
+      ol *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
-    const float use = m == -INFINITY ? 0.f : m;
+    const float use = m == -INFINITY ? 0.f : m * scale;
     unsigned pw[8];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - use);
-        l += s[tt][i];
+        s[tt][i] = __builtin_amdgcn_exp2f(fmaf(s[tt][i], scale, -use));
+        if constexpr (W) l += s[tt][i];
       }
       pw[2 * tt] = pack_bf2(s[tt][0], s[tt][1]);
       pw[2 * tt + 1] = pack_bf2(s[tt][2], s[tt][3]);
@@ -418,6 +428,8 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         if constexpr (VB > 3) vv[j][3] = bf2_of4<3>(word[j], scale_of(vs[j], (c * NT + 6) >> 5));
       }
       const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{pw[4 * hf], pw[4 * hf + 1], pw[4 * hf + 2], pw[4 * hf + 3]});
+      // the weights' sum as a product with ones, of the weights as they are rounded for V (the accumulated ones are divided by their own)
+      ol = mfma16(bf16x8_t{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80}, pb, ol);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         u32x4_t va;
@@ -430,9 +442,15 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     stage = stage + 1 == ST ? 0 : stage + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (pieces past the end write zeros)
-  l += __shfl_xor(l, 16, 64);
-  l = sum_xhalf(l);
-  if (f == 0) { sm[w][c] = m; sl[w][c] = l; }
+  if constexpr (W) {
+    l += __shfl_xor(l, 16, 64);
+    l = sum_xhalf(l);
+  }
+  if (f == 0) {
+    sm[w][c] = m * scale;
+    sl[w][c] = ol[0];
+    if constexpr (W) slw[w][c] = l;
+  }
   __syncthreads();  // every wave is done with its places
   float* so = (float*)ring;  // [4][16][D + 1]
 #pragma unroll
@@ -443,17 +461,22 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   for (int i = tid; i < G * D; i += 256) {
     const int g = i / D, d = i - g * D;
     const float M = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g])), use = M == -INFINITY ? 0.f : M;
-    float acc = 0.f, sum = 0.f;
+    float acc = 0.f, sum = 0.f, sumw = 0.f;
 #pragma unroll
     for (int ww = 0; ww < 4; ++ww) {
       const float e = exp2f(sm[ww][g] - use);
       acc += so[(ww * 16 + g) * (D + 1) + d] * e;
       sum += sl[ww][g] * e;
+      if constexpr (W) sumw += slw[ww][g] * e;
     }
     const long at = ((long)b * a.H + hk * G + g) * a.nsplit + split;
     if (act == 1) a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(L ? acc / sum : 0.f);
     else put4(a.po + at * D + d, acc);
-    if (d == 0) { put4(a.pm + at, M); put4(a.pl + at, sum); }
+    if (d == 0) {
+      put4(a.pm + at, M);
+      put4(a.pl + at, sum);
+      if constexpr (W) a.plw[at] = sumw;
+    }
   }
   if (act == 1 || !a.cnt) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -511,7 +534,7 @@ __global__ void __launch_bounds__(256) decode_attn4_join_kernel(Attn4 a) {
   for (int g = tid >> 4; g < G; g += 16) {  // 16 lanes a head
     float M = -INFINITY, sum = 0.f;
     for (int x = tid & 15; x < act; x += 16) {
-      const float m = a.pm[first + (long)g * a.nsplit + x], l = a.pl[first + (long)g * a.nsplit + x], mx = fmaxf(M, m);
+      const float m = a.pm[first + (long)g * a.nsplit + x], l = a.plw[first + (long)g * a.nsplit + x], mx = fmaxf(M, m);
       sum = sum * exp2f(M - mx) + l * exp2f(m - mx);
       M = mx;
     }
@@ -542,12 +565,14 @@ __global__ void __launch_bounds__(256) decode_attn4_join_kernel(Attn4 a) {
 }
 
 DA_EXPORT size_t da_decode_attn4_ws(int B, int H, int D, int max_len, int nsplit, int weight) {
-  return 4 * ((size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4) + (weight ? (size_t)B * H * ((max_len + 63) / 64 * 64) : 0));
+  return 4 * ((size_t)B * H * ((nsplit * (D + 3) + 3) / 4 * 4) + (weight ? (size_t)B * H * ((max_len + 63) / 64 * 64) : 0));
 }
 
 template <int D>
 static int attn4(Attn4& a, hipStream_t st) {
-  decode_attn4_kernel<D><<<dim3(a.c.Hkv, a.B, a.nsplit), 256, 0, st>>>(a);
+  const dim3 grid(a.c.Hkv, a.B, a.nsplit);
+  if (a.weight) decode_attn4_kernel<D, true><<<grid, 256, 0, st>>>(a);
+  else decode_attn4_kernel<D, false><<<grid, 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (a.weight || (a.nsplit > 1 && !a.cnt))
@@ -561,10 +586,10 @@ DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void*
                               int keys, float scale, void* ws, void* weight, void* out, int ldo, void* counters, void* stream) {
   if (Hkv < 1 || H % Hkv || H / Hkv > 16 || max_len < 1 || max_len > max_seq || nsplit < 1 || nsplit > 65535 || keys < 1 || B > 65535) return (int)hipErrorInvalidValue;
   if (B == 0) return 0;
-  const size_t n = (size_t)B * H * nsplit, all = (size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4);
+  const size_t n = (size_t)B * H * nsplit, all = (size_t)B * H * ((nsplit * (D + 3) + 3) / 4 * 4);
   Attn4 a{(const bf16_t*)q, ldq, {(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq},
           (const int*)lens, (const int*)slot, (const int*)pre, B, H, max_len, nsplit, keys, ldo, scale * 1.44269504f,
-          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), weight ? (float*)ws + all : nullptr,
+          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), (float*)ws + n * (D + 2), weight ? (float*)ws + all : nullptr,
           (max_len + 63) / 64 * 64, (float*)weight, (bf16_t*)out, weight ? nullptr : (int*)counters};
   hipStream_t st = (hipStream_t)stream;
   return D == 64 ? attn4<64>(a, st) : D == 96 ? attn4<96>(a, st) : D == 128 ? attn4<128>(a, st) : (int)hipErrorInvalidValue;
