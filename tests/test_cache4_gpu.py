@@ -280,6 +280,35 @@ def test_evict_leaves_sequences_below_the_line(K):
         assert torch.equal(a, b.cpu())
 
 
+def test_blocks_that_are_no_numbers_stay_with_their_row(K):
+    """A key's block: its KV head's query heads of that row; a value's: 32 of their elements. Nothing else."""
+    g = torch.Generator().manual_seed(6)
+    c, cg = _filled(K, g, 3, 2, 200, 128)
+    for t in (c.k_scale, cg.k_scale):
+        t[0, 1, 77, 2] = 255
+    for t in (c.v_scale, cg.v_scale):
+        t[1, 0, 130, 3] = 255
+    q = torch.randn(3, 8 * 128, generator=g).bfloat16()
+    lens, slot = torch.tensor([150, 150, 150], dtype=torch.int32), torch.tensor([0, 1, 2], dtype=torch.int32)
+    got = K.decode_attn4(q.to(DEV), cg, lens.to(DEV), slot.to(DEV), 8, 2, 128, 200).cpu().view(3, 8, 128)
+    want = torch.zeros(3, 8, 128, dtype=torch.bool)
+    want[0, 4:] = True
+    want[1, :4, 96:] = True
+    assert torch.equal(got.isnan(), want)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.5])
+def test_any_scale(K, scale):
+    g = torch.Generator().manual_seed(7)
+    c, cg = _filled(K, g, 2, 2, 300, 64)
+    q = torch.randn(2, 4 * 64, generator=g).bfloat16()
+    lens, slot = torch.tensor([300, 41], dtype=torch.int32), torch.tensor([1, 0], dtype=torch.int32)
+    got = K.decode_attn4(q.to(DEV), cg, lens.to(DEV), slot.to(DEV), 4, 2, 64, 300, scale=scale).cpu().double()
+    want = R.decode_attn4(q, c, lens, slot, 4, 2, 64, scale=scale, dtype=torch.float64)
+    most = R.decode_attn4(q, c._replace(v=c.v & 0x77), lens, slot, 4, 2, 64, scale=scale, dtype=torch.float64)
+    assert ((got - want).abs() <= 2 ** -8 * want.abs() + (2 ** -8 + 5e-5) * most).all()
+
+
 def test_rows_without_a_slot_give_zeros(K):
     c = K.new_cache4(2, 1, 64, 128, DEV)
     q = torch.randn(3, 128, device=DEV).bfloat16()
