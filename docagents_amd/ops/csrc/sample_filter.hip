@@ -55,6 +55,9 @@ __device__ __forceinline__ unsigned key_of(float x) {  // ordered as the values 
   const unsigned u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// (a range's last key as a value: -0's, which no entry has, would be +0)
+__device__ __forceinline__ float of_key(unsigned k);
+__device__ __forceinline__ float of_last(unsigned k) { return of_key(k - (k == 0x7fffffffu)); }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // e^a for a <= 0: 2^n by the exponent, e^r (|r| <= ln 2 / 2) by its series
@@ -79,10 +82,38 @@ __device__ __forceinline__ double weight(float x, float top, double inv_t) {
   return x == top ? 1.0 : exp_neg(((double)x - (double)top) * inv_t);
 }
 
-__device__ __forceinline__ double wave_sum_d(double v) {
+// v of the lane that CTRL names (0 where there is none, or in the rows that are left out)
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T moved(T v) {
+  constexpr int N = sizeof(T) / 4;
+  int q[N];
+  __builtin_memcpy(q, &v, sizeof(T));
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int i = 0; i < N; ++i) q[i] = __builtin_amdgcn_update_dpp(0, q[i], CTRL, ROWS, 0xf, false);
+  __builtin_memcpy(&v, q, sizeof(T));
   return v;
+}
+
+// A wave's smallest value, in lane 63 (complements: lanes that are moved from nowhere hold 0)
+__device__ __forceinline__ unsigned wave_min(unsigned s) {
+  s = ~s;
+  s = max(s, moved<0x111, 0xf>(s));
+  s = max(s, moved<0x112, 0xf>(s));
+  s = max(s, moved<0x114, 0xf>(s));
+  s = max(s, moved<0x118, 0xf>(s));
+  s = max(s, moved<0x142, 0xa>(s));
+  return ~max(s, moved<0x143, 0xc>(s));
+}
+
+// A wave's sums over its lanes, in order, with the lane's own
+template <typename T>
+__device__ __forceinline__ T wave_scan(T s) {
+  s += moved<0x111, 0xf>(s);
+  s += moved<0x112, 0xf>(s);
+  s += moved<0x114, 0xf>(s);
+  s += moved<0x118, 0xf>(s);
+  s += moved<0x142, 0xa>(s);
+  return s + moved<0x143, 0xc>(s);
 }
 
 // A wave's reductions on the vector ALU: neighbours, pairs, halves of 8 and of 16 lanes (mirrored), then rows of lanes
@@ -157,9 +188,9 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     const double it = 1.0 / o.T;
 #pragma unroll
     for (int e = 0; e < 8; ++e) zt += x[e] == -INFINITY ? 0.0 : weight(x[e], use, it);
-    zt = wave_sum_d(zt);
+    zt = wave_scan(zt);
   }
-  if (lane == 0) a.sums[(long)b * NC + chunk] = {zt, rest, top, n, 0};
+  if (lane == 63) a.sums[(long)b * NC + chunk] = {zt, rest, top, n, 0};
 }
 
 // ------------------------------------------------------------------------------------------- second launch
@@ -174,6 +205,7 @@ struct PickLds {
   unsigned short group[SF_MAX_GROUPS];  // the groups that pass the bound
   double redd[2][16];
   unsigned redu[3][16];
+  float topw[16];
   u64 redm[16];
   unsigned kappa, n_group, n_list;
   unsigned bin, c_above, c_at, found, range[2];
@@ -184,12 +216,7 @@ struct PickLds {
 template <typename T>
 __device__ __forceinline__ T scan_before(T v, T* red) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  T s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T t = __shfl_up(s, o, 64);
-    if (lane >= o) s += t;
-  }
+  const T s = wave_scan(v);
   __syncthreads();
   if (lane == 63) red[wv] = s;
   __syncthreads();
@@ -200,10 +227,9 @@ __device__ __forceinline__ T scan_before(T v, T* red) {
 }
 
 __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = wave_scan(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
   unsigned t = 0;
 #pragma unroll
@@ -211,7 +237,7 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   return t;
 }
 
-// The 4 neighbours of lane's in each of two groups of a wave's 8: x, and the first ones' indices (V: none)
+// The 4 neighbours of lane's in each of two groups of a wave's 8: x (NaN as -inf, NaN where there is none), the first ones' indices
 template <typename L>
 __device__ __forceinline__ void load_entries(const L* row, int V, const PickLds& S, int g0, float (&x)[8], int (&v)[2]) {
   const int lane = threadIdx.x & 63, n = S.n_group;
@@ -223,16 +249,16 @@ __device__ __forceinline__ void load_entries(const L* row, int V, const PickLds&
       L q[4];
       __builtin_memcpy(q, row + v[h], sizeof(q));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * h + e] = logit_f(q[e]);
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = __builtin_amdgcn_fmed3f(logit_f(q[e]), -INFINITY, INFINITY);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * h + e] = v[h] + e < V ? logit_f(row[v[h] + e]) : 0.f;
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = v[h] + e < V ? entry(logit_f(row[v[h] + e])) : __builtin_nanf("");
     }
   }
 }
 
-// f(there, key, index) for the entries of the listed groups, by whole waves; one after the other in a loop where f is long: a
-// launch fetches its instructions anew
+// f(x, index) for the entries of the listed groups (and x = NaN), by whole waves; in a loop where f is long: a launch fetches its
+// instructions anew
 template <typename L, typename F>
 __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S, F f) {
   for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
@@ -240,11 +266,11 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
     int v[2];
     load_entries(row, V, S, g0, x, v);
 #pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      const int at = e < 4 ? v[0] + e : v[1] + e - 4;
-      f(at < V, key_of(entry(x[0])), at);
+    for (int e = 0; e < 4; ++e) {
+      f(x[0], v[0] + e);
+      f(x[4], v[1] + e);
 #pragma unroll
-      for (int i = 0; i < 7; ++i) x[i] = x[i + 1];
+      for (int i = 0; i < 3; ++i) { x[i] = x[i + 1]; x[4 + i] = x[5 + i]; }
     }
   }
 }
@@ -253,35 +279,25 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
 // and with `stop` no longer once they are)
 template <typename L>
 __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigned lo, unsigned hi, bool stop) {
-  const int lane = threadIdx.x & 63;
+  const float from = of_key(lo), to = of_last(hi);
   for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
     if (stop && *(volatile unsigned*)&S.n_list > SF_CAP) return;
     float x[8];
     int v[2];
     load_entries(row, V, S, g0, x, v);
-    unsigned key[8], hits = 0;
+    unsigned hits = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      key[e] = key_of(entry(x[e]));
-      const int at = e < 4 ? v[0] + e : v[1] + e - 4;
-      hits |= (unsigned)(at < V && key[e] - lo <= hi - lo) << e;
-    }
+    for (int e = 0; e < 8; ++e) hits |= __builtin_amdgcn_fmed3f(x[e], from, to) == x[e] ? 1u << e : 0u;
     if (!__ballot(hits)) continue;
-    unsigned at = __popc(hits), all = at;  // before the lane's, of the wave
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned t = __shfl_up(all, o, 64);
-      if (lane >= o) all += t;
-    }
-    at = all - at;
+    unsigned all = wave_scan((unsigned)__popc(hits)), at = all - __popc(hits);  // of the wave, before the lane's
     all = __builtin_amdgcn_readlane(all, 63);
     unsigned base = 0;
-    if (lane == 0) base = atomicAdd(&S.n_list, all);
+    if ((threadIdx.x & 63) == 0) base = atomicAdd(&S.n_list, all);
     at += __builtin_amdgcn_readfirstlane(base);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (hits >> e & 1) {
-        if (at < SF_CAP) S.list[at] = ((u64)key[e] << 32) | (unsigned)~(e < 4 ? v[0] + e : v[1] + e - 4);
+        if (at < SF_CAP) S.list[at] = ((u64)key_of(x[e]) << 32) | (unsigned)~(e < 4 ? v[0] + e : v[1] + e - 4);
         ++at;
       }
   }
@@ -334,12 +350,13 @@ struct Bins {
   unsigned lo, hi;   // nor do other keys
   int shift;
 
-  __device__ unsigned of(unsigned key) const {
-    if (shift >= 0) return (hi - key) >> shift;
-    const float v = of_key(key), d = v == top ? 0.f : top - v;
+  __device__ unsigned of(float x) const {
+    if (shift >= 0) return (hi - key_of(x)) >> shift;
+    const float d = x == top ? 0.f : top - x;
     return (unsigned)fminf(d * scale, (float)(SF_BINS - 1));
   }
-  __device__ double weight_of(unsigned key) const { return weight(of_key(key), top, it); }
+  __device__ double weight_of(float x) const { return weight(x, top, it); }
+  __device__ double weight_of(unsigned key) const { return weight_of(of_key(key)); }
   __device__ static u64 units(double w) {  // rint(w 2^45): the low bits of the sum with 2^52
     return (u64)__double_as_longlong(fma(w, SF_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
   }
@@ -354,11 +371,12 @@ __device__ __forceinline__ void fill_bins(const L* row, int V, PickLds& S, const
   __syncthreads();
   for (int i = threadIdx.x; i < SF_BINS; i += 1024) { S.mass[i] = 0; S.count[i] = 0; }
   __syncthreads();
-  each_entry(row, V, S, [&](bool there, unsigned key, int) {
-    if (!there || key < r.lo || key > r.hi) return;
-    const double w = r.weight_of(key);
+  const float from = of_key(r.lo), to = of_last(r.hi);
+  each_entry(row, V, S, [&](float x, int) {
+    if (__builtin_amdgcn_fmed3f(x, from, to) != x) return;
+    const double w = r.weight_of(x);
     if (w < r.least) return;
-    const unsigned at = r.of(key);
+    const unsigned at = r.of(x);
     atomicAdd(&S.count[at], 1u);
     atomicAdd(&S.mass[at], Bins::units(w));
   });
@@ -368,18 +386,28 @@ __device__ __forceinline__ void fill_bins(const L* row, int V, PickLds& S, const
 // The first bin by which the goal is reached, from `above` entries of mass `m_above` on (the last that holds something, if none is):
 // S.bin, what is before it, and what it holds
 __device__ __forceinline__ void find_bin(PickLds& S, const Goal& goal, unsigned above, u64 m_above) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const unsigned c0 = S.count[2 * tid], c1 = S.count[2 * tid + 1];
   const u64 m0 = S.mass[2 * tid], m1 = S.mass[2 * tid + 1];
-  const unsigned cb = above + scan_before<unsigned>(c0 + c1, S.redu[0]);
-  const u64 mb = m_above + scan_before<u64>(m0 + m1, S.redm);
+  const unsigned cs = wave_scan(c0 + c1);
+  const u64 ms = wave_scan(m0 + m1);
+  __syncthreads();
+  if (lane == 63) { S.redu[0][wv] = cs; S.redm[wv] = ms; }
   if (tid == 0) S.found = 0;
   __syncthreads();
+  unsigned all = above, cb = above + cs - (c0 + c1);
+  u64 mb = m_above + ms - (m0 + m1);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    all += S.redu[0][i];
+    cb += i < wv ? S.redu[0][i] : 0;
+    mb += i < wv ? S.redm[i] : 0;
+  }
   auto take = [&](unsigned i, unsigned c_above, unsigned c_at, u64 mass) { S.bin = i; S.c_above = c_above; S.c_at = c_at; S.m_above = mass; };
   const bool r0 = goal.reached(cb, (double)mb), r1 = goal.reached(cb + c0, (double)(mb + m0)), r2 = goal.reached(cb + c0 + c1, (double)(mb + m0 + m1));
   if (c0 && !r0 && r1) take(2 * tid, cb, c0, mb), S.found = 1;
   if (c1 && !r1 && r2) take(2 * tid + 1, cb + c0, c1, mb + m0), S.found = 1;
-  const unsigned all = block_sum_u(c0 + c1, S.redu[1]) + above;
+  __syncthreads();
   if (!S.found) {
     if (c0 && cb + c0 == all) take(2 * tid, cb, c0, mb);
     if (c1 && cb + c0 + c1 == all) take(2 * tid + 1, cb + c0, c1, mb + m0);
@@ -400,7 +428,7 @@ __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S,
     unsigned a = r.lo, b = r.hi;  // the smallest key of bin <= upto, of weight >= least (hi is one, in bin 0)
     while (a < b && upto < SF_BINS) {
       const unsigned step = (b - a) / 64 + 1, k = a + (tid & 63) * step;
-      const u64 in = __ballot(k >= a && k < b && r.of(k) <= upto && (r.least <= 0 || r.weight_of(k) >= r.least));
+      const u64 in = __ballot(k >= a && k < b && r.of(of_key(k)) <= upto && (r.least <= 0 || r.weight_of(k) >= r.least));
       if (!in) {  // behind the last key tried
         a += (b - 1 - a) / step * step + 1;
         continue;
@@ -453,8 +481,9 @@ __device__ __forceinline__ Border equal_border(const L* row, int V, PickLds& S, 
   __syncthreads();
   for (int g = tid; g < SF_MAX_GROUPS; g += 1024) S.match[g] = 0;
   __syncthreads();
-  each_entry(row, V, S, [&](bool there, unsigned k, int v) {
-    if (there && k == key) atomicAdd(&S.match[v / SF_GROUP], 1u);
+  const float value = of_key(key);
+  each_entry(row, V, S, [&](float x, int v) {
+    if (x == value) atomicAdd(&S.match[v / SF_GROUP], 1u);
   });
   __syncthreads();
   unsigned c[4], sum = 0;
@@ -570,12 +599,7 @@ __device__ __forceinline__ u64 pick_few(PickLds& S, unsigned count, const RowOpt
   sync();
   const u64 at = tid < count ? S.list[tid] : 0;
   const double w = tid < count ? weight(of_key((unsigned)(at >> 32)), top, it) : 0.0;
-  double C = w;
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) {
-    const double t = __shfl_up(C, x, 64);
-    if ((int)lane >= x) C += t;
-  }
+  double C = wave_scan(w);
   if constexpr (NW > 1) {
     if (lane == 63) S.redd[0][wv] = C;
     __syncthreads();
@@ -649,7 +673,14 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   else u = u01(a.s.seed, (a.s.ctr ? (unsigned)a.s.ctr[b] : a.s.step) * 131071u + (unsigned)b, 0u);
   u = fmin(fmax(u, 0.0), 1.0);
   if (tid == 0) S.kappa = 0, S.n_group = 0, S.n_list = 0;
-  const float top = block_max(cs.m, (float*)S.redu[0]);
+  S.count[tid] = 0;
+  const float tops = max_8_64(max8(cs.m));
+  least = wave_min(least);
+  if (lane == 63) { S.topw[tid >> 6] = tops; S.redu[1][tid >> 6] = least; }
+  __syncthreads();
+  float top = S.topw[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, S.topw[i]);  // (chunks there are up to 512 of)
   if (top == -INFINITY) {
     if (tid == 0) sample_bookkeep(a.s, b, 0, -INFINITY);
     return;
@@ -659,21 +690,16 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     z1 = ((double)cs.rest + cs.n) * (cs.m == top ? 1.f : __builtin_amdgcn_exp2f((cs.m - top) * 1.44269504f));
     if (o.p < 1 && o.k == 0) zt = cs.zt * weight(cs.m, top, it);
   }
-  if (tid < 512) {  // (chunks there are up to 512 of)
-    z1 = wave_sum_d(z1);
-    zt = wave_sum_d(zt);
-    if (lane == 0) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; }
+  if (tid < 512) {
+    z1 = wave_scan(z1);
+    zt = wave_scan(zt);
+    if (lane == 63) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; }
   }
   const unsigned hi = key_of(top);
   // ---- the bound ----
   unsigned kappa = key_of(-INFINITY);
   if (o.k && o.k <= NG) {
     // the k-th largest group's bin of 1024 between the smallest and the largest
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, x, 64));
-    S.count[tid] = 0;
-    if (lane == 0) S.redu[1][tid >> 6] = least;
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 16; ++i) least = min(least, S.redu[1][i]);
     const unsigned range = hi - least;
