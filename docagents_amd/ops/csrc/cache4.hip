@@ -622,12 +622,7 @@ constexpr int EV_T = 512, EV_LIST = 8 * EV_T;
 // before the thread's own, over the workgroup's 8 waves; `all` of them
 __device__ __forceinline__ int scan8(int x, int* red, int& all) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int y = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(y, o, 64);
-    if (lane >= o) y += u;
-  }
+  const int y = wave_scan(x);
   __syncthreads();
   if (lane == 63) red[wv] = y;
   __syncthreads();

@@ -181,6 +181,29 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return t;
 }
 
+// v of the lane that CTRL names (0 where there is none, or in the rows that are left out)
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T moved(T v) {
+  constexpr int N = sizeof(T) / 4;
+  int q[N];
+  __builtin_memcpy(q, &v, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = __builtin_amdgcn_update_dpp(0, q[i], CTRL, ROWS, 0xf, false);
+  __builtin_memcpy(&v, q, sizeof(T));
+  return v;
+}
+
+// A wave's sums over its lanes, in order, with the lane's own (on the vector ALU; every lane of the wave takes part)
+template <typename T>
+__device__ __forceinline__ T wave_scan(T s) {
+  s += moved<0x111, 0xf>(s);
+  s += moved<0x112, 0xf>(s);
+  s += moved<0x114, 0xf>(s);
+  s += moved<0x118, 0xf>(s);
+  s += moved<0x142, 0xa>(s);
+  return s + moved<0x143, 0xc>(s);
+}
+
 __device__ __forceinline__ float block_max(float v, float* red) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, nw = blockDim.x >> 6;
   v = wave_max(v);

@@ -82,18 +82,6 @@ __device__ __forceinline__ double weight(float x, float top, double inv_t) {
   return x == top ? 1.0 : exp_neg(((double)x - (double)top) * inv_t);
 }
 
-// v of the lane that CTRL names (0 where there is none, or in the rows that are left out)
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T moved(T v) {
-  constexpr int N = sizeof(T) / 4;
-  int q[N];
-  __builtin_memcpy(q, &v, sizeof(T));
-#pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = __builtin_amdgcn_update_dpp(0, q[i], CTRL, ROWS, 0xf, false);
-  __builtin_memcpy(&v, q, sizeof(T));
-  return v;
-}
-
 // A wave's smallest value, in lane 63 (complements: lanes that are moved from nowhere hold 0)
 __device__ __forceinline__ unsigned wave_min(unsigned s) {
   s = ~s;
@@ -103,17 +91,6 @@ __device__ __forceinline__ unsigned wave_min(unsigned s) {
   s = max(s, moved<0x118, 0xf>(s));
   s = max(s, moved<0x142, 0xa>(s));
   return ~max(s, moved<0x143, 0xc>(s));
-}
-
-// A wave's sums over its lanes, in order, with the lane's own
-template <typename T>
-__device__ __forceinline__ T wave_scan(T s) {
-  s += moved<0x111, 0xf>(s);
-  s += moved<0x112, 0xf>(s);
-  s += moved<0x114, 0xf>(s);
-  s += moved<0x118, 0xf>(s);
-  s += moved<0x142, 0xa>(s);
-  return s + moved<0x143, 0xc>(s);
 }
 
 // A wave's reductions on the vector ALU: neighbours, pairs, halves of 8 and of 16 lanes (mirrored), then rows of lanes
