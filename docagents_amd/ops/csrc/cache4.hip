@@ -599,10 +599,12 @@ DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void*
 // Of the n keys of a sequence that is too long a KV head keeps the `recent` last ones and of the others the keep - recent of largest weight
 // (equal ones: the earlier), in their order, at the front of its slot or of another. A workgroup per (KV head, row, layer):
 //   select  the smallest kept weight as a 32-bit key whose order is the weight's, 11 bits a pass, counted in LDS
-//   list    of 4096 keys at a time the kept ones', by two sums over the workgroup (8 neighbours a thread)
+//   list    of 4096 keys at a time the kept ones', by votes of 64 and two sums over the workgroup's waves
 //   move    their rows, 512 or so at a time, in pieces of 16 bytes. A row moves to the front of where it was or stays: what a step
 //           writes, no later step reads, so the next step's rows are on their way while a step's are written, with one barrier.
-// Bound by memory and by the start of each workgroup.
+// Bound by memory: 12 sequences of 8192 keys to 4096, 8 heads x 128, four layers (452 MB read and written) 110 us, of which 14 go
+// by before the first row is moved (its weights asked for ahead of the selection: the same); 700 keys to 500, 8 heads x 64, two
+// layers 9 us, latencies of the four steps one after the other.
 struct Evict4 {
   Cache4 c;
   float* weight;
@@ -617,6 +619,7 @@ __device__ __forceinline__ unsigned order_key(float x) {  // NaN lowest, -0 as +
   return x != x ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+typedef unsigned long long u64;
 constexpr int EV_T = 512, EV_LIST = 8 * EV_T;
 
 // before the thread's own, over the workgroup's 8 waves; `all` of them
@@ -663,7 +666,7 @@ __device__ __forceinline__ void move_rows(int items, Load load, Store store) {
 template <int D>
 __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
   constexpr int NP = D / 32, RP = 2 * NP;  // 16-byte pieces of a row's codes, of keys and values
-  __shared__ int hist[2048], red[8], sel[2];
+  __shared__ int hist[2048], red[2][8], sel[2];
   __shared__ unsigned short list[EV_LIST];
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int s = p.slot[b], d = p.to[b];
@@ -674,6 +677,7 @@ __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
   const long from = blockIdx.z * p.layer + row_of(p.c, s, hk, 0), to = blockIdx.z * p.layer + row_of(p.c, d, hk, 0);
   const float* wt = p.weight + from;
   const int m = n > keep ? n - p.recent : 0;  // keys that have to earn their place (0: all are kept)
+  const int lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned cut = 0xffffffffu;
   int ties = 0;
   if (m && keep > p.recent) {
@@ -684,15 +688,21 @@ __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
       const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
       for (int i = tid; i < 2048; i += EV_T) hist[i] = 0;
       __syncthreads();
-      for (int i = tid; i < m; i += EV_T) {
-        const unsigned k = order_key(wt[i]);
-        if (pass == 0 || (k >> (sh + bits)) == (cut >> (sh + bits))) atomicAdd(&hist[(k >> sh) & (bins - 1)], 1);
+      for (int i = tid; i < m; i += EV_T * 4) {  // loads on their way together
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = wt[min(i + EV_T * e, m - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned k = order_key(y[e]);
+          if (i + EV_T * e < m && (pass == 0 || (k >> (sh + bits)) == (cut >> (sh + bits)))) atomicAdd(&hist[(k >> sh) & (bins - 1)], 1);
+        }
       }
       __syncthreads();
       int v[4], mine = 0, all;  // from the largest down: 4 bins a thread
 #pragma unroll
       for (int e = 0; e < 4; ++e) mine += v[e] = hist[2047 - 4 * tid - e];
-      int before = scan8(mine, red, all);
+      int before = scan8(mine, red[0], all);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (before < need && before + v[e] >= need) {
@@ -708,28 +718,47 @@ __global__ void __launch_bounds__(EV_T) cache4_evict_kernel(Evict4 p) {
     ties = need;
   }
   int done = 0, tied = 0;  // keys kept, keys equal to the cut so far
+  const u64 lower = (1ull << lane) - 1;
   for (int t0 = 0; t0 < n; t0 += EV_LIST) {
-    const int i0 = t0 + 8 * tid;
+    const int i0 = t0 + 512 * wv + lane;  // a wave's 8 times 64 keys
     unsigned k[8];
-    int equal = 0;
+    u64 equal[8], kept[8];
+    int ties_of = 0, kept_of = 0, cnt = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e] = i0 + 64 * e < m ? order_key(wt[i0 + 64 * e]) : 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      k[e] = i0 + e < m ? order_key(wt[i0 + e]) : 0;
-      equal += i0 + e < m && k[e] == cut;
+      equal[e] = __ballot(i0 + 64 * e < m && k[e] == cut);
+      ties_of += __popcll(equal[e]);
     }
-    int all, cnt, before = tied + scan8(equal, red, all);
-    tied += all;
-    unsigned kept = 0;
+    if (lane == 0) red[0][wv] = ties_of;
+    __syncthreads();
+    int before = tied;  // ties before the wave's
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      before += q < wv ? red[0][q] : 0;
+      tied += red[0][q];
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool tie = i0 + e < m && k[e] == cut;
-      if (i0 + e < n && (i0 + e >= m || k[e] > cut || (tie && before < ties))) kept |= 1u << e;
-      before += tie;
+      const int i = i0 + 64 * e;
+      kept[e] = __ballot(i < n && (i >= m || k[e] > cut || (k[e] == cut && before + __popcll(equal[e] & lower) < ties)));
+      before += __popcll(equal[e]);
+      kept_of += __popcll(kept[e]);
     }
-    int at = scan8(__popc(kept), red, cnt);
+    if (lane == 0) red[1][wv] = kept_of;
+    __syncthreads();
+    int at = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (kept >> e & 1) list[at++] = (unsigned short)(8 * tid + e);
+    for (int q = 0; q < 8; ++q) {
+      at += q < wv ? red[1][q] : 0;
+      cnt += red[1][q];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (kept[e] >> lane & 1) list[at + __popcll(kept[e] & lower)] = (unsigned short)(i0 - t0 + 64 * e);
+      at += __popcll(kept[e]);
+    }
     __syncthreads();
     const long src = from + t0, dst = to + done;
     auto codes = [&](int i, long row) {

@@ -2108,8 +2108,9 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     """Shorten sequences of more than ``above`` (None: ``keep``) keys to ``keep``: each KV head of each layer keeps the ``recent`` last keys and of
     the others those of largest accumulated ``weight`` (fp32 [layers,] slots, Hkv, max_seq; equal ones: the earlier; NaN least),
     in their order, with their weights. lens / slot int32 [B]; the kept rows go to the front of the same slot, or of slots ``to``
-    (then shorter sequences are copied too). What lies behind them is left as it was. Slots, and those of ``to``, are distinct.
-    c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: not lens itself)."""
+    (then shorter sequences are copied too). What lies behind them is left as it was. Slots are distinct, and those of ``to``, and
+    none of these is another row's slot. c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: no part
+    of lens)."""
     layered = c.k.dim() == 5
     dev, Hkv, D, slots, max_seq = _cache4(c, layered)
     B = lens.numel()
@@ -2119,7 +2120,7 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     _req(0 <= recent <= keep <= above, "0 <= recent <= keep <= above")
     if out is None:
         out = torch.empty_like(lens)
-    oa = _ints(out, B, dev, "out"); _req(oa != la or B == 0, "out: int32 [B] apart from lens")
+    oa = _ints(out, B, dev, "out"); _req(abs(oa - la) >= 4 * B, "out: int32 [B] apart from lens")
     _check(lib().da_cache4_evict(*map(_at, c), wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
                                  min(keep, max_seq), min(recent, max_seq), min(above, max_seq), _raw_stream()), "cache4_evict")
     return out

@@ -267,6 +267,15 @@ def test_what_is_refused(K):
     assert K.cache4_evict(c, w, i[:0], i[:0], 4, 2).numel() == 0
 
 
+def test_new_lengths_do_not_lie_over_the_old_ones(K):
+    c, w = K.new_cache4(2, 2, 64, 64, DEV), torch.zeros(2, 2, 64, device=DEV)
+    x, slot = torch.tensor([8, 9, 7], dtype=torch.int32, device=DEV), torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    for lens, out in ((x[:2], x[1:]), (x[1:], x[:2])):
+        with pytest.raises(ValueError, match="apart from lens"):
+            K.cache4_evict(c, w, lens, slot, 4, 2, out=out)
+    assert x.tolist() == [8, 9, 7]
+
+
 def test_evict_leaves_sequences_below_the_line(K):
     g = torch.Generator().manual_seed(4)
     c, cg = _filled(K, g, 3, 1, 300, 64)
