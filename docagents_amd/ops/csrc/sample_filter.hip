@@ -21,6 +21,7 @@
 #include "sample.h"
 
 constexpr int SF_GROUP = 64, SF_CHUNK = 512, SF_MAX_V = 1 << 18, SF_CAP = 2048, SF_BINS = 2048;
+constexpr unsigned SF_CROWD = 128;  // entries of a bin that are counted against one another
 constexpr int SF_MAX_GROUPS = SF_MAX_V / SF_GROUP;
 static_assert(SF_MAX_V / SF_CHUNK <= 1024 && SF_MAX_GROUPS <= 4096 && SF_CAP <= 2048, "the second launch's 1024 threads");
 typedef unsigned long long u64;
@@ -280,12 +281,12 @@ __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigne
   }
 }
 
-// The list in descending order; a key and its index are no other entry's
-__device__ __forceinline__ void sort_list(PickLds& S, unsigned count) {
-  const int tid = threadIdx.x;
+// The list's first `want` entries in descending order (what is behind them is not in order); a key and its index are no other entry's
+__device__ __forceinline__ void sort_list(PickLds& S, unsigned count, unsigned want) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   unsigned n2 = 64, p = 16;  // p threads an entry
   while (n2 < count) n2 *= 2, p /= 2;
-  if (n2 <= 512) {  // each entry's rank by counting the larger ones: n2^2 / 1024 comparisons a thread and no rounds
+  if (n2 <= 128) {  // each entry's rank by counting the larger ones
     const unsigned i = tid / p;
     const u64 mine = i < count ? S.list[i] : 0;
     unsigned rank = 0;
@@ -296,16 +297,70 @@ __device__ __forceinline__ void sort_list(PickLds& S, unsigned count) {
     __syncthreads();
     return;
   }
-  for (unsigned i = count + tid; i < n2; i += 1024) S.list[i] = 0;
-  for (unsigned size = 2; size <= n2; size *= 2)
-    for (unsigned step = size / 2; step > 0; step /= 2) {
-      __syncthreads();
-      for (unsigned i = tid; i < n2 / 2; i += 1024) {
-        const unsigned x = 2 * i - (i & (step - 1)), y = x + step;
-        const u64 q = S.list[x], r = S.list[y];
-        if ((q < r) == ((x & size) == 0)) { S.list[x] = r; S.list[y] = q; }
+  // into 2048 bins of equal width between the largest and the smallest value, then each bin's by counting
+  unsigned *const held = (unsigned*)S.C, *const start = held + SF_BINS;
+  u64 mine[2];
+  unsigned lo = ~0u, hi = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned i = tid + 1024 * e, key = i < count ? (unsigned)(S.list[i] >> 32) : 0;
+    mine[e] = i < count ? S.list[i] : 0;
+    hi = max(hi, key);
+    if (key > 0x007fffffu) lo = min(lo, key);  // (of -inf)
+    held[i] = 0;
+  }
+  lo = wave_min(lo);
+  hi = ~wave_min(~hi);
+  if (lane == 63) { S.redu[0][wv] = lo; S.redu[1][wv] = hi; }
+  if (tid == 0) S.found = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) { lo = min(lo, S.redu[0][i]); hi = max(hi, S.redu[1][i]); }
+  const float top = of_key(hi), range = lo < hi ? top - of_key(lo) : 0.f, scale = range > 0.f ? (SF_BINS - 1) / range : 0.f;
+  unsigned bin[2], slot[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float x = of_key((unsigned)(mine[e] >> 32));
+    bin[e] = (unsigned)fminf((x == top ? 0.f : top - x) * scale, (float)(SF_BINS - 1));
+    if (mine[e]) slot[e] = atomicAdd(&held[bin[e]], 1u);
+  }
+  __syncthreads();
+  const unsigned c0 = held[2 * tid], c1 = held[2 * tid + 1];
+  if (max(c0, c1) > SF_CROWD) S.found = 1;
+  const unsigned first = scan_before<unsigned>(c0 + c1, S.redu[2]);
+  start[2 * tid] = first;
+  start[2 * tid + 1] = first + c0;
+  __syncthreads();
+  if (S.found) {
+    for (unsigned i = count + tid; i < n2; i += 1024) S.list[i] = 0;
+    for (unsigned size = 2; size <= n2; size *= 2)
+      for (unsigned step = size / 2; step > 0; step /= 2) {
+        __syncthreads();
+        for (unsigned i = tid; i < n2 / 2; i += 1024) {
+          const unsigned x = 2 * i - (i & (step - 1)), y = x + step;
+          const u64 q = S.list[x], r = S.list[y];
+          if ((q < r) == ((x & size) == 0)) { S.list[x] = r; S.list[y] = q; }
+        }
       }
-    }
+    __syncthreads();
+    return;
+  }
+  unsigned at[2], n[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    at[e] = start[bin[e]];
+    n[e] = mine[e] && at[e] < want ? held[bin[e]] : 0;
+    if (n[e]) S.list[at[e] + slot[e]] = mine[e];
+  }
+  __syncthreads();
+  unsigned rank[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    for (unsigned j = 0; j < n[e]; ++j) rank[e] += S.list[at[e] + j] > mine[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (n[e]) S.list[at[e] + rank[e]] = mine[e];
   __syncthreads();
 }
 
@@ -421,7 +476,7 @@ __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S,
   collect(row, V, S, from, to, false);
   __syncthreads();
   const unsigned n = min(S.n_list, (unsigned)SF_CAP);
-  sort_list(S, n);
+  sort_list(S, n, n);
   double w[2], sum = 0;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -552,6 +607,38 @@ __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((addre
   }
 }
 
+// Rows of which more entries than the list holds pass the bound, but top-k keeps fewer: all that pass it into 2048 bins of equal width,
+// and those down to the k-th's bin into the list. Returns how many they are (or too many, as before)
+template <typename L>
+__device__ __attribute__((noinline)) unsigned collect_k(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, unsigned k,
+                                                        unsigned kappa, unsigned hi) {
+  const L* row = (const L*)global;
+  PickLds& S = *(PickLds*)lds;
+  const int tid = threadIdx.x;
+  const float top = of_key(hi), from = of_key(kappa), range = top - from, scale = (SF_BINS - 1) / range;
+  if (!(range > 0.f && range < INFINITY)) return SF_CAP + 1;
+  S.count[2 * tid] = S.count[2 * tid + 1] = 0;
+  __syncthreads();
+  each_entry(row, V, S, [&](float x, int) {
+    if (x >= from) atomicAdd(&S.count[(unsigned)fminf((top - x) * scale, (float)(SF_BINS - 1))], 1u);
+  });
+  __syncthreads();
+  const unsigned c0 = S.count[2 * tid], c1 = S.count[2 * tid + 1], before = scan_before<unsigned>(c0 + c1, S.redu[0]);
+  if (before < k && before + c0 + c1 >= k) {
+    const bool second = before + c0 < k;
+    S.bin = 2 * tid + second;
+    S.c_at = before + c0 + (second ? c1 : 0);
+  }
+  if (tid == 0) S.n_list = 0;
+  __syncthreads();
+  if (S.c_at > SF_CAP) return SF_CAP + 1;
+  // the bin's lower end, below what rounding could do
+  const float edge = (S.bin + 1) / scale, low = top - edge - 1e-6f * (fabsf(top) + edge);
+  collect(row, V, S, max(kappa, key_of(low)), hi, true);
+  __syncthreads();
+  return S.n_list;
+}
+
 // Up to 64 NW entries: NW waves (the others have ended), an entry a thread
 template <int NW>
 __device__ __forceinline__ u64 pick_few(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
@@ -596,7 +683,9 @@ __device__ __forceinline__ u64 pick_few(PickLds& S, unsigned count, const RowOpt
 
 __device__ __forceinline__ u64 pick_sorted(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
   const int tid = threadIdx.x;
-  sort_list(S, count);
+  const unsigned want = o.k ? min((unsigned)o.k, count) : count;
+  sort_list(S, count, want);
+  count = want;
   double w[2], sum = 0;
   unsigned over = 0;
 #pragma unroll
@@ -700,6 +789,8 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     z1 += S.redd[0][i];
     zt += S.redd[1][i];
   }
+  // entries 44 T below the top: 262144 of them hold 2e-14, a tenth of the rounding of a weight
+  kappa = max(kappa, key_of(fmaxf(top - (float)(44.0 * o.T), -INFINITY)));
   if (!(o.k && o.p < 1)) {  // (with both, the mass of the top k is needed)
     double least_w = o.m;
     if (o.p < 1) least_w = fmax(least_w, (1.0 - o.p) * zt / V);
@@ -724,7 +815,9 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   __syncthreads();
   collect(row, V, S, kappa, hi, true);  // (too many to sort: the counted way, whatever their number)
   __syncthreads();
-  const unsigned count = S.n_list;
+  unsigned count = S.n_list;
+  if (count > SF_CAP && o.k && o.k < SF_CAP)
+    count = collect_k((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, (unsigned)o.k, kappa, hi);
   u64 at;
   if (count <= 64) {
     if (tid >= 64) return;
@@ -735,8 +828,9 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   } else if (count <= SF_CAP) {
     at = pick_sorted(S, count, o, top, it, zt, u);
   } else {
-    // weights below a unit's half need no bins of their own: 32 T below the top
-    const float range = fminf(top - of_key(kappa), (float)(32.0 * o.T));
+    // weights below a unit's half do not count: 32 T below the top
+    kappa = max(kappa, key_of(fmaxf(top - (float)(32.0 * o.T), -INFINITY)));
+    const float range = top - of_key(kappa);
     at = pick_counted((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, range > 0.f ? (SF_BINS - 1) / range : 0.f, it, 0.0, kappa, hi, -1}, zt, u);
   }
   if (tid == 0) {
