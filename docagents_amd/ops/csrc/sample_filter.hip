@@ -215,38 +215,62 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   return t;
 }
 
-// The 4 neighbours of lane's in each of two groups of a wave's 8: x (NaN as -inf, NaN where there is none), the first ones' indices
+// A lane's 8 neighbours of a wave's 8 listed groups, as they are in memory: entries `at` .. at + 7 of the row, of which those from
+// `v` on are its own (a load that would pass the row's end begins 8 before it). Words, so that nothing waits for them here
 template <typename L>
-__device__ __forceinline__ void load_entries(const L* row, int V, const PickLds& S, int g0, float (&x)[8], int (&v)[2]) {
-  const int lane = threadIdx.x & 63, n = S.n_group;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int g = g0 + 4 * h + (lane >> 4);
-    v[h] = g < n ? S.group[g] * SF_GROUP + (lane & 15) * 4 : V;
-    if (v[h] + 4 <= V) {
-      L q[4];
-      __builtin_memcpy(q, row + v[h], sizeof(q));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * h + e] = __builtin_amdgcn_fmed3f(logit_f(q[e]), -INFINITY, INFINITY);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * h + e] = v[h] + e < V ? entry(logit_f(row[v[h] + e])) : __builtin_nanf("");
+struct Eight {
+  u32x4_t q[sizeof(L) / 2];
+  int at, v;
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(L) == 2) return __uint_as_float(e & 1 ? q[0][e >> 1] & 0xffff0000u : q[0][e >> 1] << 16);
+    else {
+      const unsigned u = q[e >> 2][e & 3];
+      return __uint_as_float(u);
     }
   }
+  __device__ __forceinline__ unsigned own8(int V) const {  // a bit each
+    return v < V ? (0xffu << (v - at)) & (0xffu >> max(at + 8 - V, 0)) : 0u;
+  }
+};
+template <typename L>
+__device__ __forceinline__ Eight<L> load_entries(const L* row, int V, const PickLds& S, int g0) {
+  const int lane = threadIdx.x & 63, g = g0 + (lane >> 3);
+  Eight<L> x;
+  x.v = g < S.n_group ? S.group[g] * SF_GROUP + (lane & 7) * 8 : V;
+  x.at = max(min(x.v, V - 8), 0);
+  if (V >= 8) {
+    __builtin_memcpy(x.q, row + x.at, sizeof(x.q));
+  } else {
+    L q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = row[min(e, V - 1)];
+    __builtin_memcpy(x.q, q, sizeof(x.q));
+  }
+  return x;
 }
 
-// f(x, index) for the entries of the listed groups (and x = NaN), by whole waves; in a loop where f is long: a launch fetches its
-// instructions anew
+// f(x, index) for the entries of the listed groups (and x = NaN beside them), by whole waves; in a loop where f is long: a
+// launch fetches its instructions anew
 template <typename L, typename F>
 __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S, F f) {
-  for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
+  const int n = S.n_group;
+  int g0 = (threadIdx.x >> 6) * 8;
+  Eight<L> next = load_entries(row, V, S, g0);
+  for (; g0 < n; g0 += 128) {
+    const Eight<L> now = next;
+    next = load_entries(row, V, S, g0 + 128);
     float x[8];
-    int v[2];
-    load_entries(row, V, S, g0, x, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
+    const unsigned own = now.own8(V);
+    if (own != 0xff) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = own >> e & 1 ? x[e] : __builtin_nanf("");
+    }
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      f(x[0], v[0] + e);
-      f(x[4], v[1] + e);
+      f(x[0], now.at + e);
+      f(x[4], now.at + 4 + e);
 #pragma unroll
       for (int i = 0; i < 3; ++i) { x[i] = x[i + 1]; x[4 + i] = x[5 + i]; }
     }
@@ -254,30 +278,45 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
 }
 
 // (key, ~index) of the listed groups' entries with lo <= key <= hi into the list (n_list of them; those past CAP are only counted,
-// and with `stop` no longer once they are)
+// and with `stop` no longer once they are). Few waves of 512 entries hold one in a narrow range: first the smallest distance from its
+// middle is looked at, of the entries as they are
 template <typename L>
 __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigned lo, unsigned hi, bool stop) {
-  const float from = of_key(lo), to = of_last(hi);
-  for (int g0 = (threadIdx.x >> 6) * 8, n = S.n_group; g0 < n; g0 += 128) {
+  const float from = of_key(lo), to = of_last(hi), mid = 0.5f * from + 0.5f * to;
+  const float half = 0.50001f * (to - from) + 1e-6f * fabsf(mid) + 1e-37f;
+  const bool any = !(half < INFINITY);
+  const int n = S.n_group;
+  int g0 = (threadIdx.x >> 6) * 8;
+  Eight<L> next = load_entries(row, V, S, g0);
+  for (; g0 < n; g0 += 128) {
     if (stop && *(volatile unsigned*)&S.n_list > SF_CAP) return;
-    float x[8];
-    int v[2];
-    load_entries(row, V, S, g0, x, v);
+    const Eight<L> now = next;
+    next = load_entries(row, V, S, g0 + 128);
+    float near = INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) near = fminf(near, fabsf(now[e] - mid));
+    if (!__ballot(any || near <= half)) continue;
     unsigned hits = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hits |= __builtin_amdgcn_fmed3f(x[e], from, to) == x[e] ? 1u << e : 0u;
+    for (int e = 0; e < 8; ++e) {
+      const float x = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
+      hits |= __builtin_amdgcn_fmed3f(x, from, to) == x ? 1u << e : 0u;
+    }
+    hits &= now.own8(V);
     if (!__ballot(hits)) continue;
     unsigned all = wave_scan((unsigned)__popc(hits)), at = all - __popc(hits);  // of the wave, before the lane's
     all = __builtin_amdgcn_readlane(all, 63);
     unsigned base = 0;
     if ((threadIdx.x & 63) == 0) base = atomicAdd(&S.n_list, all);
     at += __builtin_amdgcn_readfirstlane(base);
+#pragma unroll 1
+    for (; hits; hits &= hits - 1, ++at) {  // (a lane has one or none as a rule)
+      const int e = __builtin_ctz(hits);
+      float x = now[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (hits >> e & 1) {
-        if (at < SF_CAP) S.list[at] = ((u64)key_of(x[e]) << 32) | (unsigned)~(e < 4 ? v[0] + e : v[1] + e - 4);
-        ++at;
-      }
+      for (int i = 1; i < 8; ++i) x = e == i ? now[i] : x;
+      if (at < SF_CAP) S.list[at] = ((u64)key_of(entry(x)) << 32) | (unsigned)~(now.at + e);
+    }
   }
 }
 
