@@ -118,27 +118,35 @@ __device__ __forceinline__ float sum64(float v) {
   return sum_xhalf(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Groups and chunks begin at 16 bytes whatever the row does: group g is the entries 64 g - lead .. 64 g - lead + 63 that the row has
+template <typename L>
+__device__ __forceinline__ int lead_of(const L* row, int V) {
+  const int lead = (int)(((size_t)row & 15) / sizeof(L));
+  return V + lead <= SF_MAX_V ? lead : 0;
+}
+__host__ __device__ constexpr int groups_of(int V) { return (V + SF_GROUP - 1) / SF_GROUP; }
+__host__ __device__ constexpr int chunks_of(int V) { return (V + SF_CHUNK - 1) / SF_CHUNK; }
+constexpr int SF_LEAD = 7;  // at most
+
 // ------------------------------------------------------------------------------------------- first launch
 template <typename L>
 __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
   const int b = blockIdx.y, V = a.s.V, lane = threadIdx.x & 63, chunk = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int NC = (V + SF_CHUNK - 1) / SF_CHUNK, NG = (V + SF_GROUP - 1) / SF_GROUP, v0 = chunk * SF_CHUNK + lane * 8;
-  if (chunk >= NC) return;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
+  const int lead = lead_of(row, V), v0 = chunk * SF_CHUNK + lane * 8 - lead;
+  if (chunk >= chunks_of(V + lead)) return;
   float x[8];
-  if (v0 + 8 <= V && (((size_t)(row + v0)) & 15) == 0) {
-    if constexpr (sizeof(L) == 2) {
-      const u32x4_t u = *(const u32x4_t*)(row + v0);
+  if (v0 >= 0 && v0 + 8 <= V) {
+    u32x4_t u[sizeof(L) / 2];
+    __builtin_memcpy(u, row + v0, sizeof(u));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
-    } else {
-      const f32x4_t lo = *(const f32x4_t*)(row + v0), hi = *(const f32x4_t*)(row + v0 + 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e & 3] : hi[e & 3];
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (sizeof(L) == 2) x[e] = __uint_as_float(e & 1 ? u[0][e >> 1] & 0xffff0000u : u[0][e >> 1] << 16);
+      else x[e] = __uint_as_float((unsigned)u[e >> 2][e & 3]);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = v0 + e < V ? logit_f(row[v0 + e]) : -INFINITY;
+    for (int e = 0; e < 8; ++e) x[e] = (unsigned)(v0 + e) < (unsigned)V ? logit_f(row[v0 + e]) : -INFINITY;
   }
   float mx = -INFINITY;
 #pragma unroll
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     mx = fmaxf(mx, x[e]);
   }
   mx = max8(mx);  // a group is 8 lanes
-  if ((lane & 7) == 0 && v0 < V) a.gmax[(long)b * NG + v0 / SF_GROUP] = key_of(mx);
+  if ((lane & 7) == 0 && v0 < V) a.gmax[(long)b * groups_of(V + SF_LEAD) + chunk * 8 + (lane >> 3)] = key_of(mx);
   const float top = max_8_64(mx), use = top == -INFINITY ? 0.f : top;
   // 2^t with t rounded: 2^-24 |t| of a term, of the log-probability's sum that is
   float rest = 0.f;
@@ -168,7 +176,7 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     for (int e = 0; e < 8; ++e) zt += x[e] == -INFINITY ? 0.0 : weight(x[e], use, it);
     zt = wave_scan(zt);
   }
-  if (lane == 63) a.sums[(long)b * NC + chunk] = {zt, rest, top, n, 0};
+  if (lane == 63) a.sums[(long)b * chunks_of(V + SF_LEAD) + chunk] = {zt, rest, top, n, 0};
 }
 
 // ------------------------------------------------------------------------------------------- second launch
@@ -185,7 +193,8 @@ struct PickLds {
   unsigned redu[3][16];
   float topw[16];
   u64 redm[16];
-  unsigned kappa, n_group, n_list;
+  unsigned kappa, n_list;
+  int n_group, lead;
   unsigned bin, c_above, c_at, found, range[2];
   u64 m_above;
 };
@@ -215,12 +224,11 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   return t;
 }
 
-// A lane's 8 neighbours of a wave's 8 listed groups, as they are in memory: entries `at` .. at + 7 of the row, of which those from
-// `v` on are its own (a load that would pass the row's end begins 8 before it). Words, so that nothing waits for them here
+// A lane's 8 neighbours of a wave's 8 listed groups, as they are in memory, in words: nothing waits for them here
 template <typename L>
 struct Eight {
   u32x4_t q[sizeof(L) / 2];
-  int at, v;
+  int v;  // the first one's index
   __device__ __forceinline__ float operator[](int e) const {
     if constexpr (sizeof(L) == 2) return __uint_as_float(e & 1 ? q[0][e >> 1] & 0xffff0000u : q[0][e >> 1] << 16);
     else {
@@ -228,22 +236,21 @@ struct Eight {
       return __uint_as_float(u);
     }
   }
-  __device__ __forceinline__ unsigned own8(int V) const {  // a bit each
-    return v < V ? (0xffu << (v - at)) & (0xffu >> max(at + 8 - V, 0)) : 0u;
+  __device__ __forceinline__ unsigned there(int V) const {  // a bit each
+    return v < 0 ? 0xffu << -v & 0xffu >> max(v + 8 - V, 0) : 0xffu >> min(max(v + 8 - V, 0), 8);
   }
 };
 template <typename L>
 __device__ __forceinline__ Eight<L> load_entries(const L* row, int V, const PickLds& S, int g0) {
   const int lane = threadIdx.x & 63, g = g0 + (lane >> 3);
   Eight<L> x;
-  x.v = g < S.n_group ? S.group[g] * SF_GROUP + (lane & 7) * 8 : V;
-  x.at = max(min(x.v, V - 8), 0);
-  if (V >= 8) {
-    __builtin_memcpy(x.q, row + x.at, sizeof(x.q));
+  x.v = g < S.n_group ? S.group[g] * SF_GROUP + (lane & 7) * 8 - S.lead : V;
+  if (x.v >= 0 && x.v + 8 <= V) {
+    __builtin_memcpy(x.q, row + x.v, sizeof(x.q));
   } else {
     L q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = row[min(e, V - 1)];
+    for (int e = 0; e < 8; ++e) q[e] = (unsigned)(x.v + e) < (unsigned)V ? row[x.v + e] : (L)0;
     __builtin_memcpy(x.q, q, sizeof(x.q));
   }
   return x;
@@ -262,15 +269,15 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
-    const unsigned own = now.own8(V);
-    if (own != 0xff) {
+    const unsigned there = now.there(V);
+    if (there != 0xff) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = own >> e & 1 ? x[e] : __builtin_nanf("");
+      for (int e = 0; e < 8; ++e) x[e] = there >> e & 1 ? x[e] : __builtin_nanf("");
     }
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      f(x[0], now.at + e);
-      f(x[4], now.at + 4 + e);
+      f(x[0], now.v + e);
+      f(x[4], now.v + 4 + e);
 #pragma unroll
       for (int i = 0; i < 3; ++i) { x[i] = x[i + 1]; x[4 + i] = x[5 + i]; }
     }
@@ -302,7 +309,7 @@ __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigne
       const float x = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
       hits |= __builtin_amdgcn_fmed3f(x, from, to) == x ? 1u << e : 0u;
     }
-    hits &= now.own8(V);
+    hits &= now.there(V);
     if (!__ballot(hits)) continue;
     unsigned all = wave_scan((unsigned)__popc(hits)), at = all - __popc(hits);  // of the wave, before the lane's
     all = __builtin_amdgcn_readlane(all, 63);
@@ -315,7 +322,7 @@ __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigne
       float x = now[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) x = e == i ? now[i] : x;
-      if (at < SF_CAP) S.list[at] = ((u64)key_of(entry(x)) << 32) | (unsigned)~(now.at + e);
+      if (at < SF_CAP) S.list[at] = ((u64)key_of(entry(x)) << 32) | (unsigned)~(now.v + e);
     }
   }
 }
@@ -760,15 +767,16 @@ template <typename L>
 __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   __shared__ __attribute__((aligned(16))) PickLds S;
   const int b = blockIdx.x, V = a.s.V, tid = threadIdx.x, lane = tid & 63;
-  const int NG = (V + SF_GROUP - 1) / SF_GROUP, NC = (V + SF_CHUNK - 1) / SF_CHUNK;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
+  const int lead = lead_of(row, V), NG = groups_of(V + lead), NC = chunks_of(V + lead);
+  a.gmax += (long)b * groups_of(V + SF_LEAD);
   ChunkSum cs{0, 0.f, -INFINITY, 0, 0};
-  if (tid < NC) cs = a.sums[(long)b * NC + tid];
+  if (tid < NC) cs = a.sums[(long)b * chunks_of(V + SF_LEAD) + tid];
   unsigned gm[4];
   unsigned least = ~0u;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    gm[e] = tid + 1024 * e < NG ? a.gmax[(long)b * NG + tid + 1024 * e] : 0;
+    gm[e] = tid + 1024 * e < NG ? a.gmax[tid + 1024 * e] : 0;
     if (tid + 1024 * e < NG) least = min(least, gm[e]);
   }
   const RowOpts o = row_opts(a, b);
@@ -777,7 +785,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   if (a.u) u = a.u[b];
   else u = u01(a.s.seed, (a.s.ctr ? (unsigned)a.s.ctr[b] : a.s.step) * 131071u + (unsigned)b, 0u);
   u = fmin(fmax(u, 0.0), 1.0);
-  if (tid == 0) S.kappa = 0, S.n_group = 0, S.n_list = 0;
+  if (tid == 0) S.kappa = 0, S.n_group = 0, S.n_list = 0, S.lead = lead;
   S.count[tid] = 0;
   const float tops = max_8_64(max8(cs.m));
   least = wave_min(least);
@@ -847,7 +855,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     const u64 all = __ballot(hit);
     if (!all) continue;
     unsigned at = 0;
-    if (lane == 0) at = atomicAdd(&S.n_group, (unsigned)__popcll(all));
+    if (lane == 0) at = atomicAdd(&S.n_group, __popcll(all));
     at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
     if (hit) S.group[at] = (unsigned short)(tid + 1024 * e);
   }
@@ -880,8 +888,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
 }
 
 DA_EXPORT size_t da_sample_filtered_ws(int B, int V) {
-  const size_t NG = (V + SF_GROUP - 1) / SF_GROUP, NC = (V + SF_CHUNK - 1) / SF_CHUNK;
-  return B * (NC * sizeof(ChunkSum) + NG * 4);
+  return B * (chunks_of(V + SF_LEAD) * sizeof(ChunkSum) + groups_of(V + SF_LEAD) * (size_t)4);
 }
 
 DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int ld, double T, double p, double m, int k,
@@ -891,7 +898,7 @@ DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int 
                                  int eos3, void* stream) {
   if (V < 1 || V > SF_MAX_V || B > 65535 || (hist && (!pos || !start))) return (int)hipErrorInvalidValue;
   if (B == 0) return 0;
-  const int NC = (V + SF_CHUNK - 1) / SF_CHUNK;
+  const int NC = chunks_of(V + SF_LEAD);
   SampleArgs s{logits, V, ld, 0.f, seed, step, (const int*)ctr, (int*)out_tok, (float*)out_lp, (float*)conf, (int*)active,
                (int*)pos, (int*)lens, (int*)hist, (const int*)start, hist_ld, eos0, eos1, eos2, eos3};
   FilterArgs a{T, p, m, (const float*)Ts, (const float*)ps, (const float*)ms, k, (const int*)ks, (const float*)u,
