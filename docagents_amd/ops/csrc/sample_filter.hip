@@ -224,7 +224,8 @@ __device__ __forceinline__ unsigned block_sum_u(unsigned v, unsigned* red) {
   return t;
 }
 
-// A lane's 8 neighbours of a wave's 8 listed groups, as they are in memory, in words: nothing waits for them here
+// A lane's 8 neighbours of a wave's 8 listed groups, as they are in memory (NaN: the row has none there), in words: nothing waits
+// for them here
 template <typename L>
 struct Eight {
   u32x4_t q[sizeof(L) / 2];
@@ -250,7 +251,10 @@ __device__ __forceinline__ Eight<L> load_entries(const L* row, int V, const Pick
   } else {
     L q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = (unsigned)(x.v + e) < (unsigned)V ? row[x.v + e] : (L)0;
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (sizeof(L) == 2) q[e] = (unsigned)(x.v + e) < (unsigned)V ? row[x.v + e] : (L)0x7fff;
+      else q[e] = (unsigned)(x.v + e) < (unsigned)V ? row[x.v + e] : __builtin_nanf("");
+    }
     __builtin_memcpy(x.q, q, sizeof(x.q));
   }
   return x;
@@ -285,44 +289,38 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
 }
 
 // (key, ~index) of the listed groups' entries with lo <= key <= hi into the list (n_list of them; those past CAP are only counted,
-// and with `stop` no longer once they are). Few waves of 512 entries hold one in a narrow range: first the smallest distance from its
-// middle is looked at, of the entries as they are
+// and with `stop` no longer once they are). Bound by the vector ALU: three instructions an entry, the counts are scalar
 template <typename L>
 __device__ __forceinline__ void collect(const L* row, int V, PickLds& S, unsigned lo, unsigned hi, bool stop) {
-  const float from = of_key(lo), to = of_last(hi), mid = 0.5f * from + 0.5f * to;
-  const float half = 0.50001f * (to - from) + 1e-6f * fabsf(mid) + 1e-37f;
-  const bool any = !(half < INFINITY);
-  const int n = S.n_group;
+  const float from = of_key(lo), to = of_last(hi);
+  const int n = S.n_group, lane = threadIdx.x & 63;
   int g0 = (threadIdx.x >> 6) * 8;
   Eight<L> next = load_entries(row, V, S, g0);
   for (; g0 < n; g0 += 128) {
     if (stop && *(volatile unsigned*)&S.n_list > SF_CAP) return;
     const Eight<L> now = next;
     next = load_entries(row, V, S, g0 + 128);
-    float near = INFINITY;
+    u64 hits[8];
+    unsigned all = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) near = fminf(near, fabsf(now[e] - mid));
-    if (!__ballot(any || near <= half)) continue;
-    unsigned hits = 0;
+    for (int e = 0; e < 8; ++e) hits[e] = __ballot(__builtin_amdgcn_fmed3f(now[e], from, to) == now[e]);
+    if (from == -INFINITY) {  // and NaN
+      const unsigned there = now.there(V);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hits[e] |= __ballot(now[e] != now[e] && (there >> e & 1));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) all += __popcll(hits[e]);
+    if (!all) continue;
+    unsigned at = 0;
+    if (lane == 0) at = atomicAdd(&S.n_list, all);
+    at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
-      hits |= __builtin_amdgcn_fmed3f(x, from, to) == x ? 1u << e : 0u;
-    }
-    hits &= now.there(V);
-    if (!__ballot(hits)) continue;
-    unsigned all = wave_scan((unsigned)__popc(hits)), at = all - __popc(hits);  // of the wave, before the lane's
-    all = __builtin_amdgcn_readlane(all, 63);
-    unsigned base = 0;
-    if ((threadIdx.x & 63) == 0) base = atomicAdd(&S.n_list, all);
-    at += __builtin_amdgcn_readfirstlane(base);
-#pragma unroll 1
-    for (; hits; hits &= hits - 1, ++at) {  // (a lane has one or none as a rule)
-      const int e = __builtin_ctz(hits);
-      float x = now[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) x = e == i ? now[i] : x;
-      if (at < SF_CAP) S.list[at] = ((u64)key_of(entry(x)) << 32) | (unsigned)~(now.v + e);
+      if (!hits[e]) continue;
+      const unsigned mine = at + __builtin_amdgcn_mbcnt_hi((unsigned)(hits[e] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits[e], 0u));
+      if ((hits[e] >> lane & 1) && mine < SF_CAP) S.list[mine] = ((u64)key_of(entry(now[e])) << 32) | (unsigned)~(now.v + e);
+      at += __popcll(hits[e]);
     }
   }
 }
