@@ -10,18 +10,32 @@
 // changes them).
 //
 // Two launches. The first reads the row once, a wave to 512 entries: the largest entry of each 64 (group) and the sums of exp.
-// The second, a workgroup a row, never sorts the row: each filter bounds the kept entries from below before any of them is known,
+// The second, a workgroup a row, reads again only what can be kept. Each filter bounds the kept entries from below before any of them
+// is known,
 //   top-k  the k-th largest of the groups' largest entries (k groups have an entry as large)
 //   top-p  w >= (1 - p) C(V) / V: entries below it hold less than 1 - p of the mass together
 //   min-p  w >= min_p
-// and only groups whose largest entry passes the bound are read again. Up to CAP entries are sorted in LDS. More of them (flat
-// distributions) are counted into 2048 bins of equal width; a border (of top-k, top-p or u) falls into one bin, and that bin's
-// entries are sorted. If even those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
+//   all    w >= e^-44
+// and only groups whose largest entry passes the bound are read again. Up to CAP entries are sorted in LDS. Of more of them, where
+// top-k keeps fewer, those down to the bin of the k-th of 2048 bins of equal width are. More still (flat distributions) are counted
+// into such bins with their weights; a border (of top-k, top-p or u) falls into one bin, and that bin's entries are sorted. If even
+// those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
+//
+// Measured: one row of 32064 4.0 + 5.6 us, 32 of 128256 (bf16, 8 MB) 7.0 + 9.2, 128 of them in fp32 with settings of their own (66 MB) 17.5 +
+// 11.5 (the read at 3.8 TB/s, its start and end in it), latencies of launches and of some ten steps that wait for one another; 33
+// flat rows of 50257 5.6 + 60: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border (search, read, sort).
+// Several workgroups a row for that (25 -> 7) cost more in handing over; both launches as one (workgroups of 64 KB LDS, the row's last
+// one picks) 10.6 us for 9.4 of one row and 38 for 16 of 32.
 #include "common.h"
 #include "sample.h"
 
 constexpr int SF_GROUP = 64, SF_CHUNK = 512, SF_MAX_V = 1 << 18, SF_CAP = 2048, SF_BINS = 2048;
-constexpr unsigned SF_CROWD = 128;  // entries of a bin that are counted against one another
+// Waves that sort 64 entries each by counting, the others having ended; above them a workgroup sorts through bins. 32 rows, the whole
+// call in us: 65 entries 13.1 with one wave / 12.1 with two, 128 13.6 / 13.3, 192 14.7 / 14.5 / 14.7 with four, 256 14.4 / 15.8
+constexpr int SF_FEW = 2;
+// Entries of a bin that are counted against one another; in larger ones all are exchanged in pairs (2000 entries, each value 32 times
+// 22 us / 33, 100 times 25 / 33, 200 times 35 / 33)
+constexpr unsigned SF_CROWD = 128;
 constexpr int SF_MAX_GROUPS = SF_MAX_V / SF_GROUP;
 static_assert(SF_MAX_V / SF_CHUNK <= 1024 && SF_MAX_GROUPS <= 4096 && SF_CAP <= 2048, "the second launch's 1024 threads");
 typedef unsigned long long u64;
@@ -361,7 +375,7 @@ __device__ __forceinline__ void sort_list(PickLds& S, unsigned count, unsigned w
 #pragma unroll
   for (int i = 0; i < 16; ++i) { lo = min(lo, S.redu[0][i]); hi = max(hi, S.redu[1][i]); }
   const float top = of_key(hi), range = lo < hi ? top - of_key(lo) : 0.f, scale = range > 0.f ? (SF_BINS - 1) / range : 0.f;
-  unsigned bin[2], slot[2];
+  unsigned bin[2], slot[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const float x = of_key((unsigned)(mine[e] >> 32));
@@ -400,7 +414,10 @@ __device__ __forceinline__ void sort_list(PickLds& S, unsigned count, unsigned w
   unsigned rank[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < 2; ++e)
-    for (unsigned j = 0; j < n[e]; ++j) rank[e] += S.list[at[e] + j] > mine[e];
+    for (unsigned i = 0, j = slot[e]; i < n[e]; ++i) {  // from its own place on: the bins' starts may share a bank
+      rank[e] += S.list[at[e] + j] > mine[e];
+      j = j + 1 == n[e] ? 0 : j + 1;
+    }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < 2; ++e)
@@ -586,8 +603,8 @@ __device__ __forceinline__ Border equal_border(const L* row, int V, PickLds& S, 
 }
 
 // Rows of more entries than the list holds: the borders of top-k and of top-p, then u's. A function of its own, with the LDS as such:
-// inside the kernel its registers were the other rows' too (23 of them went to memory, 6.6 -> 8.3 us for one row of 32064), and
-// through generic pointers it took 95 us for 68 in 33 flat rows of 50257.
+// inside the kernel its registers were the other rows' too (23 of them went to memory, a row of 32064 took a quarter longer), and
+// through generic pointers it took 95 us for 68.
 typedef __attribute__((address_space(3))) PickLds* lds_pick_t;
 template <typename L>
 __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, RowOpts o,
@@ -867,9 +884,9 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   if (count <= 64) {
     if (tid >= 64) return;
     at = pick_few<1>(S, count, o, top, it, zt, u);
-  } else if (count <= 256) {
-    if (tid >= 256) return;
-    at = pick_few<4>(S, count, o, top, it, zt, u);
+  } else if (count <= 64 * SF_FEW) {
+    if (tid >= 64 * SF_FEW) return;
+    at = pick_few<SF_FEW>(S, count, o, top, it, zt, u);
   } else if (count <= SF_CAP) {
     at = pick_sorted(S, count, o, top, it, zt, u);
   } else {
