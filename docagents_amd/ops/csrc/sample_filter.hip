@@ -21,11 +21,11 @@
 // into such bins with their weights; a border (of top-k, top-p or u) falls into one bin, and that bin's entries are sorted. If even
 // those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
 //
-// Measured: one row of 32064 4.0 + 5.6 us, 32 of 128256 (bf16, 8 MB) 7.0 + 9.2, 128 of them in fp32 with settings of their own (66 MB) 17.5 +
-// 11.5 (the read at 3.8 TB/s, its start and end in it), latencies of launches and of some ten steps that wait for one another; 33
-// flat rows of 50257 5.6 + 60: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border (search, read, sort).
-// Several workgroups a row for that (25 -> 7) cost more in handing over; both launches as one (workgroups of 64 KB LDS, the row's last
-// one picks) 10.6 us for 9.4 of one row and 38 for 16 of 32.
+// Measured: one row of 32064 3.9 + 5.7 us, 32 of 128256 (bf16, 8 MB) 7.7 + 9.4, 128 of them in fp32 with settings of their own (66 MB)
+// 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait for one another;
+// 33 flat rows of 50257 6 + 61: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border (search, read,
+// sort). Several workgroups a row for that (25 -> 7) cost more in handing over; both launches as one (workgroups of 64 KB LDS, the
+// row's last one picks) 10.6 us for 9.4 of one row and 38 for 16 of 32.
 #include "common.h"
 #include "sample.h"
 
@@ -171,15 +171,16 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
   mx = max8(mx);  // a group is 8 lanes
   if ((lane & 7) == 0 && v0 < V) a.gmax[(long)b * groups_of(V + SF_LEAD) + chunk * 8 + (lane >> 3)] = key_of(mx);
   const float top = max_8_64(mx), use = top == -INFINITY ? 0.f : top;
-  // 2^t with t rounded: 2^-24 |t| of a term, of the log-probability's sum that is
+  // 2^t and what t's rounding left, or a term would be off by 2^-24 |t|
   float rest = 0.f;
   int n = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float q = __builtin_amdgcn_exp2f((x[e] - use) * 1.44269504f);
+    const float d = fmaxf(x[e] - use, -1e4f), t = d * 1.44269504f, q = __builtin_amdgcn_exp2f(t);
+    const float left = fmaf(d, 1.92596303e-8f, fmaf(d, 1.44269504f, -t));
     const u64 same = __ballot(x[e] == use);
     n += __popcll(same);
-    rest += x[e] == use ? 0.f : q;
+    rest += x[e] == use ? 0.f : fmaf(q, left * 0.693147181f, q);
   }
   rest = sum64(rest);
   const RowOpts o = row_opts(a, b);
@@ -815,7 +816,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   }
   double z1 = 0, zt = 0;
   if (cs.m != -INFINITY) {
-    z1 = ((double)cs.rest + cs.n) * (cs.m == top ? 1.f : __builtin_amdgcn_exp2f((cs.m - top) * 1.44269504f));
+    z1 = ((double)cs.rest + cs.n) * weight(cs.m, top, 1.0);
     if (o.p < 1 && o.k == 0) zt = cs.zt * weight(cs.m, top, it);
   }
   if (tid < 512) {
@@ -898,7 +899,8 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));
     const double d = x == top ? 0.0 : (double)x - (double)top;
-    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - (double)log1pf((float)(z1 - 1.0))));
+    const float log_z = log1pf((float)(z1 - 1.0));  // and a step of Newton's method
+    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - ((double)log_z + (z1 * exp_neg(-(double)log_z) - 1.0))));
   }
 }
 
