@@ -214,6 +214,9 @@ struct PickLds {
   u64 m_above;
 };
 
+// Bins a unit of logit, of a range of them (one of 0 or inf: one bin; finite, or the top's 0 would not be in the first bin)
+__device__ __forceinline__ float bins_over(float range) { return range > 0.f ? fminf((SF_BINS - 1) / range, 3e38f) : 0.f; }
+
 // The workgroup's sums over its threads, in order (16 waves): before the thread's own
 template <typename T>
 __device__ __forceinline__ T scan_before(T v, T* red) {
@@ -375,7 +378,7 @@ __device__ __forceinline__ void sort_list(PickLds& S, unsigned count, unsigned w
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i) { lo = min(lo, S.redu[0][i]); hi = max(hi, S.redu[1][i]); }
-  const float top = of_key(hi), range = lo < hi ? top - of_key(lo) : 0.f, scale = range > 0.f ? (SF_BINS - 1) / range : 0.f;
+  const float top = of_key(hi), range = lo < hi ? top - of_key(lo) : 0.f, scale = bins_over(range);
   unsigned bin[2], slot[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -677,7 +680,7 @@ __device__ __attribute__((noinline)) unsigned collect_k(const __attribute__((add
   const L* row = (const L*)global;
   PickLds& S = *(PickLds*)lds;
   const int tid = threadIdx.x;
-  const float top = of_key(hi), from = of_key(kappa), range = top - from, scale = (SF_BINS - 1) / range;
+  const float top = of_key(hi), from = of_key(kappa), range = top - from, scale = bins_over(range);
   if (!(range > 0.f && range < INFINITY)) return SF_CAP + 1;
   S.count[2 * tid] = S.count[2 * tid + 1] = 0;
   __syncthreads();
@@ -894,7 +897,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     // weights below a unit's half do not count: 32 T below the top
     kappa = max(kappa, key_of(fmaxf(top - (float)(32.0 * o.T), -INFINITY)));
     const float range = top - of_key(kappa);
-    at = pick_counted((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, range > 0.f ? (SF_BINS - 1) / range : 0.f, it, 0.0, kappa, hi, -1}, zt, u);
+    at = pick_counted((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, bins_over(range), it, 0.0, kappa, hi, -1}, zt, u);
   }
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));

@@ -1561,11 +1561,11 @@ def _row_option(v, B: int, dtype, dev: int, name: str):
 def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, top_p=1.0, min_p=0.0, u=None, out_tok=None,
                     out_lp=None, conf=None, active=None, ctr=None, pos=None, lens=None, hist=None, start=None, eos=()):
     """``sample`` from the entries that top-k, top-p and min-p leave (csrc/sample_filter.hip has the definition): logits [B, V]
-    (bf16 or fp32, rows of any stride, V up to 262144), one uniform number a row. u (fp32 [B], in [0, 1)): those numbers; None: drawn from (seed,
-    ctr or step, row), as ``sample``'s are. temperature, top_p, min_p: numbers, or fp32 [B] on the GPU; top_k: a number, or int32
-    [B]. temperature <= 0: greedy; top_k <= 0, top_p >= 1 and min_p <= 0 are off. Ties go to the lower index, NaN counts as -inf, and a
-    row of nothing else gives token 0 with log-probability -inf. Returns (tokens, logprobs): the untempered, unfiltered
-    distribution's. Bookkeeping as ``sample``'s."""
+    (bf16 or fp32, rows of any stride, V up to 262144), one uniform number a row. u (fp32 [B], in [0, 1)): those numbers; None:
+    drawn from (seed, ctr or step, row), as ``sample``'s are. temperature, top_p, min_p: numbers, or fp32 [B] on the GPU; top_k: a
+    number, or int32 [B]. temperature <= 0: greedy, inf: all finite entries alike; top_k <= 0, top_p >= 1 and min_p <= 0 are off.
+    Ties go to the lower index, NaN counts as -inf, and a row of nothing else gives token 0 with log-probability -inf. Returns
+    (tokens, logprobs): the untempered, unfiltered distribution's. Bookkeeping as ``sample``'s."""
     f32 = logits.dtype is torch.float32
     _req(logits.is_cuda and (f32 or logits.dtype is torch.bfloat16), "logits must be bf16 or fp32 on GPU")
     B, V = logits.shape

@@ -355,7 +355,7 @@ def sample_filtered(logits, temperature, seed=0, step=0, top_k=0, top_p=1.0, min
         d = torch.where(z == z[0], torch.zeros_like(z), z - z[0])  # (z may be inf)
         n = 1
         if T > 0:
-            w = torch.exp(d / T)
+            w = torch.where(d == -math.inf, 0.0, torch.exp(d / T))  # (whatever T, inf among it)
             C = w.cumsum(0)
             n = n_k = k if 0 < k < V else V
             if p < 1:

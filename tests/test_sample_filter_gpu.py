@@ -195,3 +195,63 @@ def test_drawn_as_often_as_its_probability(K):
     share = torch.zeros(V, dtype=torch.float64, device=DEV)
     share[top.indices] = torch.softmax(top.values.double() / 1.3, 0)
     assert ((torch.bincount(tok.long(), minlength=V) - share * B).abs() <= 1.01).all()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("copies", [1, 7, 127, 128, 129, 700])
+def test_lists_of_each_length(K, f32, copies):
+    """As many entries as each way to sort them takes, all different to all alike."""
+    g = torch.Generator().manual_seed(copies)
+    V, B = 4000, 3
+    x = (torch.randint(0, V // copies + 1, (B, V), generator=g).float() / 64 - 20)
+    x = x if f32 else x.bfloat16()
+    for k in (63, 64, 65, 127, 128, 129, 300, 1000, 2047, 2048, 2049, 3000):
+        _same(K, x, torch.rand(B, generator=g), temperature=7.0, top_k=k)
+        _same(K, x, torch.rand(B, generator=g), temperature=7.0, top_k=k, top_p=0.7, min_p=0.01)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("V", [2500, 30011, 131072])
+def test_top_k_of_many_candidates(K, f32, V):
+    """k near the number of groups and above it: the bound leaves more entries than the list holds."""
+    g = torch.Generator().manual_seed(V + 1)
+    B = 4
+    for sigma in (0.5, 4.0):
+        x = _logits(g, B, V, f32, sigma)
+        x[3] = x[3].round()  # thousands of equal ones
+        for k in (V // 70, V // 64 + 1, 1500, 2000, 2047, 2048):
+            _same(K, x, torch.rand(B, generator=g), temperature=0.9, top_k=k)
+            _same(K, x, torch.rand(B, generator=g), temperature=0.9, top_k=k, top_p=0.8)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T", [1e-38, 1e-4, 0.05, 1.0, 1e4, 1e30, math.inf])
+def test_any_temperature_and_value(K, f32, T):
+    """Weights of 1 and of 0 and everything beside them; infinite entries, NaN, the type's largest values."""
+    g = torch.Generator().manual_seed(11)
+    V = 5003
+    x = torch.randn(8, V, generator=g) * 3
+    x[1, torch.randperm(V, generator=g)[:1500]] = -math.inf
+    x[2, torch.randperm(V, generator=g)[:3000]] = math.nan
+    x[3, torch.randperm(V, generator=g)[:200]] = 3e38
+    x[4, torch.randperm(V, generator=g)[:200]] = -3e38
+    x[5, torch.randperm(V, generator=g)[:3]] = math.inf
+    x[6] = torch.where(torch.rand(V, generator=g) < 0.5, -0.0, 0.0)
+    x[7] *= 1e-38
+    x = x if f32 else x.bfloat16()
+    for opts in (dict(), dict(top_k=900), dict(top_k=3000), dict(top_p=0.6), dict(top_k=1200, top_p=0.9, min_p=0.5)):
+        _same(K, x, torch.rand(8, generator=g), temperature=T, **opts)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("V", [1, 3, 7, 8, 9, 57, 64, 120, 511, 2050])
+def test_short_rows_at_each_address(K, f32, V):
+    g = torch.Generator().manual_seed(V)
+    for lead in range(9):
+        for ld in (V + 8, V + 9):
+            whole = torch.full((3, ld), 99.0)
+            whole[:, lead:lead + V] = torch.randn(3, min(V, ld - lead), generator=g) * 2
+            whole = whole if f32 else whole.bfloat16()
+            on = whole.to(DEV)
+            for opts in (dict(top_p=0.9), dict(top_k=max(1, V // 2)), dict()):
+                _same(K, whole[:, lead:lead + V], torch.rand(3, generator=g), xg=on[:, lead:lead + V], temperature=0.8, **opts)
