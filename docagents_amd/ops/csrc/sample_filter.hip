@@ -9,7 +9,8 @@
 // (relative error 2e-13), sums in double or, where they are collected by atomics, in units of 2^-45 (whole numbers: no order
 // changes them).
 //
-// Two launches. The first reads the row once, a wave to 512 entries: the largest entry of each 64 (group) and the sums of exp.
+// Two launches, or one where a row has few workgroups. The first reads the row once, a wave to 512 entries: the largest entry of each
+// 64 (group) and the sums of exp.
 // The second, a workgroup a row, reads again only what can be kept. Each filter bounds the kept entries from below before any of them
 // is known,
 //   top-k  the k-th largest of the groups' largest entries (k groups have an entry as large)
@@ -21,15 +22,19 @@
 // into such bins with their weights; a border (of top-k, top-p or u) falls into one bin, and that bin's entries are sorted. If even
 // those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
 //
-// Measured: one row of 32064 3.9 + 5.7 us, 32 of 128256 (bf16, 8 MB) 7.7 + 9.4, 128 of them in fp32 with settings of their own (66 MB)
-// 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait for one another;
-// 33 flat rows of 50257 6 + 61: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border (search, read,
-// sort). Several workgroups a row for that (25 -> 7) cost more in handing over; both launches as one (workgroups of 64 KB LDS, the
-// row's last one picks) 10.6 us for 9.4 of one row and 38 for 16 of 32.
+// Measured: one row of 32064 10 us in one launch (3.9 + 5.7 in two), 32 of 128256 (bf16, 8 MB) 7.7 + 9.4, 128 of them in fp32 with settings
+// of their own (66 MB) 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait
+// for one another; 33 flat rows of 50257 6 + 61: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border
+// (search, read, sort). Several workgroups a row for that (25 -> 7) cost more in handing over.
 #include "common.h"
 #include "sample.h"
 
 constexpr int SF_GROUP = 64, SF_CHUNK = 512, SF_MAX_V = 1 << 18, SF_CAP = 2048, SF_BINS = 2048;
+// Both in one launch: rows that one workgroup takes (16 chunks), a CU each, and up to 64 workgroups of longer ones, whose last goes on
+// to the pick. us of calls one by one / in a graph, two launches and one: 1 - 256 rows of 8000 13.1 / 10.0 - 11.4 and 10.7 / 9.2 - 10.4 (320
+// 18.3 / 18.1, 18.7 / 18.7); one row of 32064 13.1 / 10.3 and 11.5 / 10.8, 16 of them 13.6 / 10.4 and 11.9 / 11.1 (64: 13.6 / 11.2, 12.0 /
+// 11.9), 4 of 128256 13.6 / 10.8 and 11.8 / 11.5 (32: 13.4 / 12.6, 21.5 / 20.7)
+constexpr int SF_WG = 16, SF_JOINED_ROWS = 256, SF_JOINED = 64;
 // Waves that sort 64 entries each by counting, the others having ended; above them a workgroup sorts through bins. 32 rows, the whole
 // call in us: 65 entries 13.1 with one wave / 12.1 with two, 128 13.6 / 13.3, 192 14.7 / 14.5 / 14.7 with four, 256 14.4 / 15.8
 constexpr int SF_FEW = 2;
@@ -51,6 +56,7 @@ struct FilterArgs {
   const float* u;
   unsigned* gmax;  // [B][groups]
   ChunkSum* sums;  // [B][chunks]
+  int* tickets;    // [B], 0 between launches: of rows of several workgroups in one launch
   SampleArgs s;
 };
 
@@ -142,10 +148,23 @@ __host__ __device__ constexpr int groups_of(int V) { return (V + SF_GROUP - 1) /
 __host__ __device__ constexpr int chunks_of(int V) { return (V + SF_CHUNK - 1) / SF_CHUNK; }
 constexpr int SF_LEAD = 7;  // at most
 
-// ------------------------------------------------------------------------------------------- first launch
-template <typename L>
-__global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
-  const int b = blockIdx.y, V = a.s.V, lane = threadIdx.x & 63, chunk = blockIdx.x * 4 + (threadIdx.x >> 6);
+// What is handed over within a launch passes the L2s of the XCDs (agent scope)
+template <bool JOINED, typename T>
+__device__ __forceinline__ void put(T* p, T v) {
+  if constexpr (JOINED) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else *p = v;
+}
+template <bool JOINED, typename T>
+__device__ __forceinline__ T get(const T* p) {
+  if constexpr (JOINED) return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else return *p;
+}
+
+// ------------------------------------------------------------------------------------------- statistics
+// A wave's 512 entries of row b
+template <typename L, bool JOINED>
+__device__ __forceinline__ void chunk_stats(const FilterArgs& a, int b, int chunk) {
+  const int V = a.s.V, lane = threadIdx.x & 63;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
   const int lead = lead_of(row, V), v0 = chunk * SF_CHUNK + lane * 8 - lead;
   if (chunk >= chunks_of(V + lead)) return;
@@ -169,7 +188,7 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     mx = fmaxf(mx, x[e]);
   }
   mx = max8(mx);  // a group is 8 lanes
-  if ((lane & 7) == 0 && v0 < V) a.gmax[(long)b * groups_of(V + SF_LEAD) + chunk * 8 + (lane >> 3)] = key_of(mx);
+  if ((lane & 7) == 0 && v0 < V) put<JOINED>(a.gmax + (long)b * groups_of(V + SF_LEAD) + chunk * 8 + (lane >> 3), key_of(mx));
   const float top = max_8_64(mx), use = top == -INFINITY ? 0.f : top;
   // 2^t and what t's rounding left, or a term would be off by 2^-24 |t|
   float rest = 0.f;
@@ -191,10 +210,20 @@ __global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
     for (int e = 0; e < 8; ++e) zt += x[e] == -INFINITY ? 0.0 : weight(x[e], use, it);
     zt = wave_scan(zt);
   }
-  if (lane == 63) a.sums[(long)b * chunks_of(V + SF_LEAD) + chunk] = {zt, rest, top, n, 0};
+  if (lane == 63) {
+    u64* to = (u64*)(a.sums + (long)b * chunks_of(V + SF_LEAD) + chunk);
+    put<JOINED>(to, __builtin_bit_cast(u64, zt));
+    put<JOINED>(to + 1, (u64)__float_as_uint(rest) | (u64)__float_as_uint(top) << 32);
+    put<JOINED>(to + 2, (u64)(unsigned)n);
+  }
 }
 
-// ------------------------------------------------------------------------------------------- second launch
+template <typename L>
+__global__ void __launch_bounds__(256) filter_stats_kernel(FilterArgs a) {
+  chunk_stats<L, false>(a, blockIdx.y, blockIdx.x * 4 + (threadIdx.x >> 6));
+}
+
+// ------------------------------------------------------------------------------------------- the pick
 struct PickLds {
   u64 list[SF_CAP];  // (key, ~index) of entries
   union {
@@ -608,9 +637,10 @@ __device__ __forceinline__ Border equal_border(const L* row, int V, PickLds& S, 
 
 // Rows of more entries than the list holds: the borders of top-k and of top-p, then u's. A function of its own, with the LDS as such:
 // inside the kernel its registers were the other rows' too (23 of them went to memory, a row of 32064 took a quarter longer), and
-// through generic pointers it took 95 us for 68.
+// through generic pointers it took 95 us for 68. One for
+// each kernel: it knows where the LDS is (66 us for 61).
 typedef __attribute__((address_space(3))) PickLds* lds_pick_t;
-template <typename L>
+template <typename L, bool JOINED>
 __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, RowOpts o,
                                                   Bins all, double zt, double u) {
   const L* row = (const L*)global;
@@ -674,7 +704,7 @@ __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((addre
 
 // Rows of which more entries than the list holds pass the bound, but top-k keeps fewer: all that pass it into 2048 bins of equal width,
 // and those down to the k-th's bin into the list. Returns how many they are (or too many, as before)
-template <typename L>
+template <typename L, bool JOINED>
 __device__ __attribute__((noinline)) unsigned collect_k(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, unsigned k,
                                                         unsigned kappa, unsigned hi) {
   const L* row = (const L*)global;
@@ -782,20 +812,39 @@ __device__ __forceinline__ u64 pick_sorted(PickLds& S, unsigned count, const Row
   return S.list[min(block_sum_u(c, S.redu[2]), n - 1)];
 }
 
-template <typename L>
+// JOINED: the statistics in the same launch, of which the last of a row's workgroups to have its own goes on
+template <typename L, bool JOINED>
 __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   __shared__ __attribute__((aligned(16))) PickLds S;
-  const int b = blockIdx.x, V = a.s.V, tid = threadIdx.x, lane = tid & 63;
+  const int b = JOINED ? blockIdx.y : blockIdx.x;
+  if constexpr (JOINED) {
+    chunk_stats<L, true>(a, b, blockIdx.x * SF_WG + (threadIdx.x >> 6));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (gridDim.x > 1) {
+      if (threadIdx.x == 0) {
+        S.found = __hip_atomic_fetch_add(a.tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        if (S.found) put<true>(a.tickets + b, 0);
+      }
+      __syncthreads();
+      if (!S.found) return;
+    }
+  }
+  const int V = a.s.V, tid = threadIdx.x, lane = tid & 63;
   const L* row = (const L*)a.s.logits + (long)b * a.s.ld;
   const int lead = lead_of(row, V), NG = groups_of(V + lead), NC = chunks_of(V + lead);
   a.gmax += (long)b * groups_of(V + SF_LEAD);
   ChunkSum cs{0, 0.f, -INFINITY, 0, 0};
-  if (tid < NC) cs = a.sums[(long)b * chunks_of(V + SF_LEAD) + tid];
+  if (tid < NC) {
+    const u64* p = (const u64*)(a.sums + (long)b * chunks_of(V + SF_LEAD) + tid);
+    const u64 q0 = get<JOINED>(p), q1 = get<JOINED>(p + 1), q2 = get<JOINED>(p + 2);
+    cs = {__builtin_bit_cast(double, q0), __uint_as_float((unsigned)q1), __uint_as_float((unsigned)(q1 >> 32)), (int)q2, 0};
+  }
   unsigned gm[4];
   unsigned least = ~0u;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    gm[e] = tid + 1024 * e < NG ? a.gmax[tid + 1024 * e] : 0;
+    gm[e] = tid + 1024 * e < NG ? get<JOINED>(a.gmax + tid + 1024 * e) : 0;
     if (tid + 1024 * e < NG) least = min(least, gm[e]);
   }
   const RowOpts o = row_opts(a, b);
@@ -883,7 +932,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   __syncthreads();
   unsigned count = S.n_list;
   if (count > SF_CAP && o.k && o.k < SF_CAP)
-    count = collect_k((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, (unsigned)o.k, kappa, hi);
+    count = collect_k<L, JOINED>((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, (unsigned)o.k, kappa, hi);
   u64 at;
   if (count <= 64) {
     if (tid >= 64) return;
@@ -897,7 +946,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     // weights below a unit's half do not count: 32 T below the top
     kappa = max(kappa, key_of(fmaxf(top - (float)(32.0 * o.T), -INFINITY)));
     const float range = top - of_key(kappa);
-    at = pick_counted((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, bins_over(range), it, 0.0, kappa, hi, -1}, zt, u);
+    at = pick_counted<L, JOINED>((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, bins_over(range), it, 0.0, kappa, hi, -1}, zt, u);
   }
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));
@@ -913,7 +962,7 @@ DA_EXPORT size_t da_sample_filtered_ws(int B, int V) {
 
 DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int ld, double T, double p, double m, int k,
                                  const void* Ts, const void* ps, const void* ms, const void* ks, const void* u, unsigned seed,
-                                 unsigned step, const void* ctr, void* ws, void* out_tok, void* out_lp, void* conf, void* active,
+                                 unsigned step, const void* ctr, void* ws, void* tickets, void* out_tok, void* out_lp, void* conf, void* active,
                                  void* pos, void* lens, void* hist, const void* start, int hist_ld, int eos0, int eos1, int eos2,
                                  int eos3, void* stream) {
   if (V < 1 || V > SF_MAX_V || B > 65535 || (hist && (!pos || !start))) return (int)hipErrorInvalidValue;
@@ -922,13 +971,19 @@ DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int 
   SampleArgs s{logits, V, ld, 0.f, seed, step, (const int*)ctr, (int*)out_tok, (float*)out_lp, (float*)conf, (int*)active,
                (int*)pos, (int*)lens, (int*)hist, (const int*)start, hist_ld, eos0, eos1, eos2, eos3};
   FilterArgs a{T, p, m, (const float*)Ts, (const float*)ps, (const float*)ms, k, (const int*)ks, (const float*)u,
-               (unsigned*)((char*)ws + (size_t)B * NC * sizeof(ChunkSum)), (ChunkSum*)ws, s};
+               (unsigned*)((char*)ws + (size_t)B * NC * sizeof(ChunkSum)), (ChunkSum*)ws, (int*)tickets, s};
   hipStream_t st = (hipStream_t)stream;
+  const int wgs = (NC + SF_WG - 1) / SF_WG;
+  if (wgs == 1 ? B <= SF_JOINED_ROWS : tickets && B * (long)wgs <= SF_JOINED) {
+    if (f32) filter_pick_kernel<float, true><<<dim3(wgs, B), 1024, 0, st>>>(a);
+    else filter_pick_kernel<bf16_t, true><<<dim3(wgs, B), 1024, 0, st>>>(a);
+    DA_LAUNCH_CHECK();
+  }
   if (f32) filter_stats_kernel<float><<<dim3((NC + 3) / 4, B), 256, 0, st>>>(a);
   else filter_stats_kernel<bf16_t><<<dim3((NC + 3) / 4, B), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if (f32) filter_pick_kernel<float><<<B, 1024, 0, st>>>(a);
-  else filter_pick_kernel<bf16_t><<<B, 1024, 0, st>>>(a);
+  if (f32) filter_pick_kernel<float, false><<<B, 1024, 0, st>>>(a);
+  else filter_pick_kernel<bf16_t, false><<<B, 1024, 0, st>>>(a);
   DA_LAUNCH_CHECK();
 }

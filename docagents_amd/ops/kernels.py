@@ -120,7 +120,7 @@ _SIGS = {
     "da_pool_l2norm_f16": [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "da_topk_dense_ws": [c_int] * 4,
     "da_topk_stream_ws": [c_int] * 4,
-    "da_sample_filtered": [c_void_p] + [c_int] * 4 + [ctypes.c_double] * 3 + [c_int] + [c_void_p] * 5 + [c_uint, c_uint] + [c_void_p] * 10
+    "da_sample_filtered": [c_void_p] + [c_int] * 4 + [ctypes.c_double] * 3 + [c_int] + [c_void_p] * 5 + [c_uint, c_uint] + [c_void_p] * 11
                           + [c_int] * 5 + [c_void_p],
     "da_sample_filtered_ws": [c_int] * 2,
     "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_int] * 6 + [c_void_p],
@@ -1549,6 +1549,7 @@ def sample(logits, temperature: float, seed: int, step: int = 0, out_tok=None, o
     return out_tok, out_lp
 
 
+FILTERED_WG = 8185  # entries of a row that one workgroup takes
 SAMPLE_FILTERED_MAX_V = 1 << 18  # entries of a row that sample_filtered takes (csrc/sample_filter.hip, SF_MAX_V)
 
 
@@ -1604,17 +1605,21 @@ def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, 
         hist_ld = hist.shape[1]
     e = (*eos[:4], -1, -1, -1, -1)
     L = lib()
-    ws = _call_scratch(_filtered_bytes(B, V), logits)
+    stream = _raw_stream()
+    nbytes, joined = _filtered_plan(B, V)
+    cnt = _counters(logits.device, stream).data_ptr() if joined else None
+    ws = _call_scratch(nbytes, logits)
     _check(L.da_sample_filtered(logits.data_ptr(), f32, B, V, ld, temperature, top_p, min_p, max(0, min(int(top_k), V)), Ts, ps, ms,
-                                ks, us, seed & 0xffffffff, step & 0xffffffff, _at(ctr), ws.data_ptr(), out_tok.data_ptr(),
+                                ks, us, seed & 0xffffffff, step & 0xffffffff, _at(ctr), ws.data_ptr(), cnt, out_tok.data_ptr(),
                                 out_lp.data_ptr(), _at(conf), _at(active), _at(pos), _at(lens), _at(hist), _at(start), hist_ld,
-                                e[0], e[1], e[2], e[3], _raw_stream()), "sample_filtered")
+                                e[0], e[1], e[2], e[3], stream), "sample_filtered")
     return out_tok, out_lp
 
 
 @_rule
-def _filtered_bytes(B: int, V: int) -> int:
-    return lib().da_sample_filtered_ws(B, V)
+def _filtered_plan(B: int, V: int):
+    """(bytes of scratch, whether a row's workgroups may share a launch that needs counters)."""
+    return lib().da_sample_filtered_ws(B, V), V > FILTERED_WG and B * -(-V // FILTERED_WG) <= 64
 
 
 def sample_partial(logits, temperature: float, seed: int, v0: int, step: int = 0, ctr=None, out=None):

@@ -255,3 +255,38 @@ def test_short_rows_at_each_address(K, f32, V):
             on = whole.to(DEV)
             for opts in (dict(top_p=0.9), dict(top_k=max(1, V // 2)), dict()):
                 _same(K, whole[:, lead:lead + V], torch.rand(3, generator=g), xg=on[:, lead:lead + V], temperature=0.8, **opts)
+
+
+@pytest.mark.parametrize("B,V", [(1, 8185), (256, 600), (257, 600), (9, 8186), (32, 9000), (33, 9000), (4, 128256), (5, 128256)])
+def test_one_launch_or_two(K, B, V):
+    """About the sizes where a row's workgroups begin to share a launch: one after the other, in graphs on one stream and on two."""
+    g = torch.Generator().manual_seed(B * V)
+    xs = [_logits(g, B, V, f32, 2.0) for f32 in (False, True)]
+    us = [torch.rand(B, generator=g) for _ in range(4)]
+    want = [[R.sample_filtered(x, 0.9, u=u, top_k=30, top_p=0.9)[0] for u in us[:2]] for x in xs]
+    xg, ug = [x.to(DEV) for x in xs], [u.to(DEV) for u in us]
+    call = lambda i, j: K.sample_filtered(xg[i], 0.9, u=ug[j], top_k=30, top_p=0.9)[0]  # noqa: E731
+    for i in range(2):
+        for j in range(2):
+            assert torch.equal(call(i, j).cpu(), want[i][j])
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            call(i, 0)
+            s.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                outs.append([call(i, j) for j in range(2)])
+            graphs.append(graph)
+    for _ in range(5):  # both on their way at once, and eager calls beside them
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = call(0, 1)
+        torch.cuda.synchronize()
+        assert torch.equal(eager.cpu(), want[0][1])
+        for i in range(2):
+            for j in range(2):
+                assert torch.equal(outs[i][j].cpu(), want[i][j])
+                outs[i][j].fill_(-7)
