@@ -1989,17 +1989,20 @@ def _same_device(*ts) -> int:
 
 
 def _cache4(c, layers: bool = False):
-    """(current device, KV heads, head dim, slots, max_seq) of a 4-bit cache (one layer's; ``layers``: with the layers in front)."""
+    """(current device, KV heads, head dim, slots, max_seq, addresses) of a 4-bit cache (one layer's; ``layers``: with the layers in front)."""
     k, ks, v, vs = c
     dev = _same_device(k, ks, v, vs)
-    shape, scales = k.shape, ks.shape
-    _req(len(shape) == 4 + layers and v.shape == shape and vs.shape == scales and scales[:-1] == shape[:-1] and scales[-1] == SCALE_BYTES,
-         "cache4: codes [slots, Hkv, max_seq, D / 2], scales [.., 4]")
-    for t in c:
-        _req(t.dtype is torch.uint8 and t.is_contiguous() and t.data_ptr() % 16 == 0, "cache4: contiguous uint8, 16-byte aligned")
-    Hkv, max_seq, D = shape[-3], shape[-2], 2 * shape[-1]
-    _req(D in (64, 96, 128) and max_seq < 1 << 31, "cache4: head dim 64, 96 or 128")
-    return dev, Hkv, D, shape[-4], max_seq
+    shape, scales, u8 = k.shape, ks.shape, torch.uint8
+    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
+    if not (len(shape) == 4 + layers and v.shape == shape and vs.shape == scales and scales[:-1] == shape[:-1] and scales[-1] == SCALE_BYTES):
+        raise ValueError("cache4: codes [slots, Hkv, max_seq, D / 2], scales [.., 4]")
+    if not (k.dtype is u8 and ks.dtype is u8 and v.dtype is u8 and vs.dtype is u8 and k.is_contiguous() and ks.is_contiguous()
+            and v.is_contiguous() and vs.is_contiguous() and (at[0] | at[1] | at[2] | at[3]) % 16 == 0):
+        raise ValueError("cache4: contiguous uint8, 16-byte aligned")
+    *_, slots, Hkv, max_seq, D = shape
+    if D not in (32, 48, 64) or max_seq >= 1 << 31:
+        raise ValueError("cache4: head dim 64, 96 or 128")
+    return dev, Hkv, 2 * D, slots, max_seq, at
 
 
 def _weight4(weight, c, dev: int):
@@ -2025,11 +2028,11 @@ def cache4_write(k, v, c: Cache4, slot, at, weight=None) -> None:
     """Keys and values k, v [T, Hkv * D] (bf16, rows of any stride) of T tokens into places ``at`` of slots ``slot`` (int32 [T])
     of a 4-bit cache, rounded to the nearest code (ties to even). One token a place; a token whose place lies outside the cache
     is not written. weight (fp32 [slots, Hkv, max_seq]): a written key's accumulated weight begins at 0."""
-    dev, Hkv, D, slots, max_seq = _cache4(c)
+    dev, Hkv, D, slots, max_seq, cache = _cache4(c)
     (ka, kl), (va, vl) = _rows16(k, Hkv * D, dev, "k"), _rows16(v, Hkv * D, dev, "v")
     T = k.shape[0]
     _req(v.shape[0] == T and k.shape[1] == v.shape[1] == Hkv * D, "k and v: the same tokens, [T, Hkv * D]")
-    _check(lib().da_cache4_write(None, ka, va, kl, vl, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"), None, None, 0, *map(_at, c),
+    _check(lib().da_cache4_write(None, ka, va, kl, vl, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"), None, None, 0, *cache,
                                  None if weight is None else _weight4(weight, c, dev), T, 0, Hkv, D, slots, max_seq, _raw_stream()),
            "cache4_write")
 
@@ -2038,7 +2041,7 @@ def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4
     """``rope_cache`` with a 4-bit cache: q and k heads of qkv [T, (H + 2 Hkv) * D] rotated in place (by position ``pos``), k
     and v written as ``cache4_write`` writes them, to places ``at`` (which are not the positions once keys have been evicted).
     A token whose position lies outside the table is left as it is, and not written."""
-    dev, Hc, Dc, slots, max_seq = _cache4(c)
+    dev, Hc, Dc, slots, max_seq, cache = _cache4(c)
     q, ld = _rows16(qkv, (H + 2 * Hkv) * D, dev, "qkv")
     T = qkv.shape[0]
     _req(Hc == Hkv and Dc == D and qkv.is_contiguous() and qkv.shape[1] == (H + 2 * Hkv) * D, "qkv shape")
@@ -2046,7 +2049,7 @@ def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4
          and cos_sin.shape[1] == D // 2, "cos_sin must be fp32 [max_pos, D/2, 2]")
     ld = qkv.shape[1]
     _check(lib().da_cache4_write(q, q + 2 * H * D, q + 2 * (H + Hkv) * D, ld, ld, _ints(slot, T, dev, "slot"), _ints(at, T, dev, "at"),
-                                 _ints(pos, T, dev, "pos"), cos_sin.data_ptr(), cos_sin.shape[0], *map(_at, c),
+                                 _ints(pos, T, dev, "pos"), cos_sin.data_ptr(), cos_sin.shape[0], *cache,
                                  None if weight is None else _weight4(weight, c, dev), T, H, Hkv, D, slots, max_seq, _raw_stream()),
            "rope_cache4")
     return qkv
@@ -2054,11 +2057,11 @@ def rope_cache4(qkv, pos, cos_sin, H: int, Hkv: int, D: int, slot, at, c: Cache4
 
 def cache4_read(c: Cache4, slot: int, n: int):
     """The first n keys and values of a slot as bf16 [Hkv, n, D] (exact: what the codes stand for)."""
-    dev, Hkv, D, slots, max_seq = _cache4(c)
+    dev, Hkv, D, slots, max_seq, cache = _cache4(c)
     _req(0 <= slot < slots and 0 <= n <= max_seq, "cache4_read: outside the cache")
     k = c.k.new_empty((Hkv, n, D), dtype=torch.bfloat16)
     v = torch.empty_like(k)
-    _check(lib().da_cache4_read(*map(_at, c), Hkv, D, slots, max_seq, slot, n, k.data_ptr(), v.data_ptr(), _raw_stream()), "cache4_read")
+    _check(lib().da_cache4_read(*cache, Hkv, D, slots, max_seq, slot, n, k.data_ptr(), v.data_ptr(), _raw_stream()), "cache4_read")
     return k, v
 
 
@@ -2082,7 +2085,7 @@ def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: in
     pre (int32 [B, 2]: P, slot; P % 64 == 0): the keys [0, P) of a row are those of another slot.
     weight (fp32 [slots, Hkv, max_seq]; not with pre): each key's probability, summed over the query heads of its KV head, is
     added to it (what ``cache4_evict`` goes by). Rows then have slots of their own."""
-    dev, Hc, Dc, slots, max_seq = _cache4(c)
+    dev, Hc, Dc, slots, max_seq, cache = _cache4(c)
     _req(Hc == Hkv and Dc == D and H % Hkv == 0 and H // Hkv <= 16, "decode_attn4: head dim, KV heads, query heads")
     qa, ldq = _rows16(q, H * D, dev, "q")
     B = q.shape[0]
@@ -2103,7 +2106,7 @@ def decode_attn4(q, c: Cache4, lens, slot, H: int, Hkv: int, D: int, max_len: in
     stream = _raw_stream()
     cnt = _counters(q.device, stream).data_ptr() if joined else None
     ws = _call_scratch(nbytes, q)
-    _check(lib().da_decode_attn4(qa, ldq, *map(_at, c), la, sa, pa, B, H, Hkv, D, slots, max_seq, max_len, nsplit, keys,
+    _check(lib().da_decode_attn4(qa, ldq, *cache, la, sa, pa, B, H, Hkv, D, slots, max_seq, max_len, nsplit, keys,
                                  D ** -0.5 if scale is None else scale, ws.data_ptr(), wa, out.data_ptr(), out.stride(0), cnt, stream),
            "decode_attn4")
     return out
@@ -2117,7 +2120,7 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     none of these is another row's slot. c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: no part
     of lens)."""
     layered = c.k.dim() == 5
-    dev, Hkv, D, slots, max_seq = _cache4(c, layered)
+    dev, Hkv, D, slots, max_seq, cache = _cache4(c, layered)
     B = lens.numel()
     wa, la, sa = _weight4(weight, c, dev), _ints(lens, B, dev, "lens"), _ints(slot, B, dev, "slot")
     ta = sa if to is None else _ints(to, B, dev, "to")
@@ -2126,6 +2129,6 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     if out is None:
         out = torch.empty_like(lens)
     oa = _ints(out, B, dev, "out"); _req(abs(oa - la) >= 4 * B, "out: int32 [B] apart from lens")
-    _check(lib().da_cache4_evict(*map(_at, c), wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
+    _check(lib().da_cache4_evict(*cache, wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
                                  min(keep, max_seq), min(recent, max_seq), min(above, max_seq), _raw_stream()), "cache4_evict")
     return out
