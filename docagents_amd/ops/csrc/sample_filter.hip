@@ -243,6 +243,18 @@ struct PickLds {
   u64 m_above;
 };
 
+// A value that all lanes hold, in scalar registers: what a function is given is in vector ones, and a branch on it is taken both ways
+template <typename T>
+__device__ __forceinline__ T uniform(T v) {
+  constexpr int N = sizeof(T) / 4;
+  unsigned q[N];
+  __builtin_memcpy(q, &v, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = __builtin_amdgcn_readfirstlane(q[i]);
+  __builtin_memcpy(&v, q, sizeof(T));
+  return v;
+}
+
 // Bins a unit of logit, of a range of them (one of 0 or inf: one bin; finite, or the top's 0 would not be in the first bin)
 __device__ __forceinline__ float bins_over(float range) { return range > 0.f ? fminf((SF_BINS - 1) / range, 3e38f) : 0.f; }
 
@@ -472,15 +484,15 @@ struct Goal {
 // 2^shift keys from hi
 struct Bins {
   float top, scale;
-  double it, least;  // weights below `least` do not count
-  unsigned lo, hi;   // nor do other keys
+  double it;
+  unsigned lo, hi;  // other keys do not count
   int shift;
 
-  __device__ unsigned of(float x) const {
-    if (shift >= 0) return (hi - key_of(x)) >> shift;
+  __device__ unsigned of_width(float x) const {  // of equal width
     const float d = x == top ? 0.f : top - x;
     return (unsigned)fminf(d * scale, (float)(SF_BINS - 1));
   }
+  __device__ unsigned of(float x) const { return shift >= 0 ? (hi - key_of(x)) >> shift : of_width(x); }
   __device__ double weight_of(float x) const { return weight(x, top, it); }
   __device__ double weight_of(unsigned key) const { return weight_of(of_key(key)); }
   __device__ static u64 units(double w) {  // rint(w 2^45): the low bits of the sum with 2^52
@@ -492,20 +504,41 @@ struct Bins {
   }
 };
 
+// A weight is e^(-its bin's middle) e^r, |r| <= 1 / 120 in narrow bins: those of e^r are summed (to r^5 / 120: 5e-16 left), a third of
+// the whole exponential's instructions (33 flat rows of 50257: 61 -> SF us), and the bins' factors applied behind it
 template <typename L>
 __device__ __forceinline__ void fill_bins(const L* row, int V, PickLds& S, const Bins& r) {
   __syncthreads();
   for (int i = threadIdx.x; i < SF_BINS; i += 1024) { S.mass[i] = 0; S.count[i] = 0; }
   __syncthreads();
   const float from = of_key(r.lo), to = of_last(r.hi);
-  each_entry(row, V, S, [&](float x, int) {
-    if (__builtin_amdgcn_fmed3f(x, from, to) != x) return;
-    const double w = r.weight_of(x);
-    if (w < r.least) return;
-    const unsigned at = r.of(x);
-    atomicAdd(&S.count[at], 1u);
-    atomicAdd(&S.mass[at], Bins::units(w));
-  });
+  const double step = r.it / r.scale;  // of the exponent, a bin
+  if (r.shift < 0 && step <= 1.0 / 60) {
+    const double top = r.top, half = 0.5 * step;
+    each_entry(row, V, S, [&](float x, int) {
+      if (__builtin_amdgcn_fmed3f(x, from, to) != x) return;
+      const unsigned at = r.of_width(x);
+      const double e = fma(fmin((double)x - top, 0.0), r.it, fma((double)at, step, half));  // (0 of infinite ones)
+      double q = 1.0 / 120;
+      q = fma(q, e, 1.0 / 24);
+      q = fma(q, e, 1.0 / 6);
+      q = fma(q, e, 0.5);
+      q = fma(q, e, 1.0);
+      q = fma(q, e, 1.0);
+      atomicAdd(&S.count[at], 1u);
+      atomicAdd(&S.mass[at], Bins::units(q));
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < SF_BINS; i += 1024)
+      if (S.mass[i]) S.mass[i] = (u64)rint((double)S.mass[i] * exp_neg(-fma((double)i, step, half)));
+  } else {
+    each_entry(row, V, S, [&](float x, int) {
+      if (__builtin_amdgcn_fmed3f(x, from, to) != x) return;
+      const unsigned at = r.of(x);
+      atomicAdd(&S.count[at], 1u);
+      atomicAdd(&S.mass[at], Bins::units(r.weight_of(x)));
+    });
+  }
   __syncthreads();
 }
 
@@ -541,6 +574,24 @@ __device__ __forceinline__ void find_bin(PickLds& S, const Goal& goal, unsigned 
   __syncthreads();
 }
 
+// The smallest key of lo .. hi for which f holds, as it does for the larger ones (and for hi); whole waves: 64 keys of a range at a time
+template <typename F>
+__device__ __forceinline__ unsigned first_key(unsigned lo, unsigned hi, F f) {
+  const unsigned lane = threadIdx.x & 63;
+  while (lo < hi) {
+    const unsigned step = (hi - lo) / 64 + 1, k = lo + lane * step;
+    const u64 in = __ballot(k >= lo && k < hi && f(k));
+    if (!in) {  // behind the last key tried
+      lo += (hi - 1 - lo) / step * step + 1;
+      continue;
+    }
+    const unsigned i = __builtin_ctzll(in);
+    hi = lo + i * step;
+    lo = i ? hi - step + 1 : lo;
+  }
+  return lo;
+}
+
 // The border in the bin that was found (of equal width, up to CAP entries): its entries sorted
 template <typename L>
 __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S, const Bins& r, const Goal& goal) {
@@ -548,25 +599,14 @@ __device__ __forceinline__ Border sorted_border(const L* row, int V, PickLds& S,
   const unsigned bin = S.bin, above = S.c_above;
   const double m_above = (double)S.m_above;
   if (tid == 0) S.n_list = 0;
-  // the bin's keys, from the first of it to before the first of the bin above: 64 keys of a range at a time
+  // the bin's keys, from the first of it to before the first of the bin above
   if (tid < 128) {
-    const unsigned upto = tid < 64 ? bin : bin - 1;
-    unsigned a = r.lo, b = r.hi;  // the smallest key of bin <= upto, of weight >= least (hi is one, in bin 0)
-    while (a < b && upto < SF_BINS) {
-      const unsigned step = (b - a) / 64 + 1, k = a + (tid & 63) * step;
-      const u64 in = __ballot(k >= a && k < b && r.of(of_key(k)) <= upto && (r.least <= 0 || r.weight_of(k) >= r.least));
-      if (!in) {  // behind the last key tried
-        a += (b - 1 - a) / step * step + 1;
-        continue;
-      }
-      const unsigned i = __builtin_ctzll(in);
-      b = a + i * step;
-      a = i ? b - step + 1 : a;
-    }
-    if ((tid & 63) == 0) S.range[tid >> 6] = tid < 64 ? a : upto < SF_BINS ? a - 1 : r.hi;
+    const unsigned upto = tid < 64 ? bin : bin - 1;  // (hi is in bin 0)
+    const unsigned a = upto < SF_BINS ? first_key(r.lo, r.hi, [&](unsigned k) { return r.of_width(of_key(k)) <= upto; }) : r.hi + 1;
+    if ((tid & 63) == 0) S.range[tid >> 6] = tid < 64 ? a : a - 1;
   }
   __syncthreads();
-  const unsigned from = S.range[0], to = S.range[1];
+  const unsigned from = uniform(S.range[0]), to = uniform(S.range[1]);
   collect(row, V, S, from, to, false);
   __syncthreads();
   const unsigned n = min(S.n_list, (unsigned)SF_CAP);
@@ -643,20 +683,33 @@ typedef __attribute__((address_space(3))) PickLds* lds_pick_t;
 template <typename L, bool JOINED>
 __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, RowOpts o,
                                                   Bins all, double zt, double u) {
-  const L* row = (const L*)global;
+  const L* row = (const L*)uniform(global);
   PickLds& S = *(PickLds*)lds;
   const int tid = threadIdx.x;
+  V = uniform(V);
+  o = {uniform(o.T), uniform(o.p), uniform(o.m), uniform(o.k)};
+  all = {uniform(all.top), uniform(all.scale), uniform(all.it), uniform(all.lo), uniform(all.hi), -1};
+  zt = uniform(zt);
+  u = uniform(u);
   Border end{0, 0};  // of what is kept (last 0: all that counts)
   const bool mass_of_k = o.k && o.p < 1;  // the mass of the top k counts, whatever min-p leaves of them
+  auto from_min_p = [&] {  // the keys of too small a weight for it
+    if (tid < 64) S.range[0] = first_key(all.lo, all.hi, [&](unsigned k) { return all.weight_of(k) >= o.m; });
+    __syncthreads();
+    all.lo = uniform(S.range[0]);
+    __syncthreads();
+  };
+  if (o.m > 0 && !mass_of_k) from_min_p();
   Bins r = all;
-  r.least = mass_of_k ? 0.0 : o.m;
-  bool filled = false;
+  bool filled = false, cut = !mass_of_k;
   int border = o.k ? 0 : o.p < 1 ? 1 : 2;
   unsigned above = 0;
   u64 m_above = 0;
   for (;;) {
-    if (border == 2 && r.shift < 0 && mass_of_k && o.m > r.least && r.weight_of((unsigned)(end.last >> 32)) < o.m) {
-      r.least = o.m;
+    if (border == 2 && r.shift < 0 && o.m > 0 && !cut && r.weight_of((unsigned)(end.last >> 32)) < o.m) {
+      cut = true;
+      from_min_p();
+      r.lo = all.lo;
       filled = false;
       end.last = 0;
     }
@@ -673,14 +726,14 @@ __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((addre
                                     : Goal{OVER_MASS, 0, u * end.mass};
     find_bin(S, goal, above, m_above);
     Border b;
-    if (r.shift < 0 && S.c_at <= SF_CAP) {
+    if (r.shift < 0 && uniform(S.c_at) <= SF_CAP) {
       b = sorted_border(row, V, S, r, goal);
     } else {
       // too many in one bin: all the keys into bins of keys, and again the bin that is found, until it is one key
       if (r.shift >= 0) {
-        above = S.c_above;
-        m_above = S.m_above;
-        r.hi -= S.bin << r.shift;
+        above = uniform(S.c_above);
+        m_above = uniform(S.m_above);
+        r.hi -= uniform(S.bin) << r.shift;
         const unsigned low = r.hi - ((1u << r.shift) - 1);
         if (low > r.lo && low <= r.hi) r.lo = low;
       }
@@ -707,9 +760,13 @@ __device__ __attribute__((noinline)) u64 pick_counted(const __attribute__((addre
 template <typename L, bool JOINED>
 __device__ __attribute__((noinline)) unsigned collect_k(const __attribute__((address_space(1))) L* global, int V, lds_pick_t lds, unsigned k,
                                                         unsigned kappa, unsigned hi) {
-  const L* row = (const L*)global;
+  const L* row = (const L*)uniform(global);
   PickLds& S = *(PickLds*)lds;
   const int tid = threadIdx.x;
+  V = uniform(V);
+  k = uniform(k);
+  kappa = uniform(kappa);
+  hi = uniform(hi);
   const float top = of_key(hi), from = of_key(kappa), range = top - from, scale = bins_over(range);
   if (!(range > 0.f && range < INFINITY)) return SF_CAP + 1;
   S.count[2 * tid] = S.count[2 * tid + 1] = 0;
@@ -946,7 +1003,7 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     // weights below a unit's half do not count: 32 T below the top
     kappa = max(kappa, key_of(fmaxf(top - (float)(32.0 * o.T), -INFINITY)));
     const float range = top - of_key(kappa);
-    at = pick_counted<L, JOINED>((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, bins_over(range), it, 0.0, kappa, hi, -1}, zt, u);
+    at = pick_counted<L, JOINED>((const __attribute__((address_space(1))) L*)row, V, (lds_pick_t)&S, o, Bins{top, bins_over(range), it, kappa, hi, -1}, zt, u);
   }
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));
