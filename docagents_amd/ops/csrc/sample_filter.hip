@@ -24,8 +24,8 @@
 //
 // Measured: one row of 32064 10 us in one launch (3.9 + 5.7 in two), 32 of 128256 (bf16, 8 MB) 7.7 + 9.4, 128 of them in fp32 with settings
 // of their own (66 MB) 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait
-// for one another; 33 flat rows of 50257 6 + 61: 25 us weigh 40000 entries or so on one CU (75 vector instructions each), 10 a border
-// (search, read, sort). Several workgroups a row for that (25 -> 7) cost more in handing over.
+// for one another; 33 flat rows of 50257 6 + 50: 16 us weigh 40000 entries or so on one CU (vector instructions), 10 a border (search,
+// read, sort). Several workgroups a row for that took a quarter of its time and twice as much again for handing over.
 #include "common.h"
 #include "sample.h"
 
@@ -504,8 +504,8 @@ struct Bins {
   }
 };
 
-// A weight is e^(-its bin's middle) e^r, |r| <= 1 / 120 in narrow bins: those of e^r are summed (to r^5 / 120: 5e-16 left), a third of
-// the whole exponential's instructions (33 flat rows of 50257: 61 -> SF us), and the bins' factors applied behind it
+// A weight is e^(-its bin's middle) e^r, |r| <= 1 / 120 in narrow bins: those of e^r are summed (to r^5 / 120: 5e-16 left), half of
+// the whole exponential's instructions (25 -> 16 us of 33 flat rows of 50257), and the bins' factors applied behind it
 template <typename L>
 __device__ __forceinline__ void fill_bins(const L* row, int V, PickLds& S, const Bins& r) {
   __syncthreads();
