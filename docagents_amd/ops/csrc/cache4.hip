@@ -231,10 +231,10 @@ __device__ __forceinline__ void read_k4(unsigned at, unsigned at_s, unsigned (&k
   if constexpr (D == 128) {
     u32x4_t x[4];
     asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\t"
-                 "ds_read_b128 %3, %8 offset:3072\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
+                 "ds_read_b128 %3, %8 offset:%10\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:64\n\t"
                  "ds_read_b32 %6, %9 offset:128\n\tds_read_b32 %7, %9 offset:192\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-                 : "v"(at), "v"(at_s) : "memory");
+                 : "v"(at), "v"(at_s), "n"(3 * 1024) : "memory");
 #pragma unroll
     for (int e = 0; e < 16; ++e) k[e >> 2][e & 3] = x[e >> 2][e & 3];
   } else if constexpr (D == 64) {
