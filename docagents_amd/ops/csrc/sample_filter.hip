@@ -235,6 +235,7 @@ struct PickLds {
   unsigned short group[SF_MAX_GROUPS];  // the groups that pass the bound
   double redd[2][16];
   unsigned redu[3][16];
+  int redt[8];
   float topw[16];
   u64 redm[16];
   unsigned kappa, n_list;
@@ -331,7 +332,7 @@ __device__ __forceinline__ void each_entry(const L* row, int V, const PickLds& S
     next = load_entries(row, V, S, g0 + 128);
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(now[e], -INFINITY, INFINITY);
+    for (int e = 0; e < 8; ++e) x[e] = entry(now[e]);  // (a median of -inf and inf would be folded to a minimum, and NaN be inf)
     const unsigned there = now.there(V);
     if (there != 0xff) {
 #pragma unroll
@@ -923,15 +924,18 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
     if (tid == 0) sample_bookkeep(a.s, b, 0, -INFINITY);
     return;
   }
-  double z1 = 0, zt = 0;
+  double z1 = 0, zt = 0;  // of exp(x - top) without the entries of `top`, and how many these are
+  int tops_n = 0;
   if (cs.m != -INFINITY) {
-    z1 = ((double)cs.rest + cs.n) * weight(cs.m, top, 1.0);
+    z1 = ((double)cs.rest + (cs.m == top ? 0 : cs.n)) * weight(cs.m, top, 1.0);
+    tops_n = cs.m == top ? cs.n : 0;
     if (o.p < 1 && o.k == 0) zt = cs.zt * weight(cs.m, top, it);
   }
   if (tid < 512) {
     z1 = wave_scan(z1);
     zt = wave_scan(zt);
-    if (lane == 63) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; }
+    tops_n = wave_scan(tops_n);
+    if (lane == 63) { S.redd[0][tid >> 6] = z1; S.redd[1][tid >> 6] = zt; S.redt[tid >> 6] = tops_n; }
   }
   const unsigned hi = key_of(top);
   // ---- the bound ----
@@ -956,9 +960,11 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   }
   __syncthreads();
   z1 = zt = 0;
+  tops_n = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     z1 += S.redd[0][i];
+    tops_n += S.redt[i];
     zt += S.redd[1][i];
   }
   // entries 44 T below the top: 262144 of them hold 2e-14, a tenth of the rounding of a weight
@@ -1008,8 +1014,13 @@ __global__ void __launch_bounds__(1024) filter_pick_kernel(FilterArgs a) {
   if (tid == 0) {
     const float x = of_key((unsigned)(at >> 32));
     const double d = x == top ? 0.0 : (double)x - (double)top;
-    const float log_z = log1pf((float)(z1 - 1.0));  // and a step of Newton's method
-    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - ((double)log_z + (z1 * exp_neg(-(double)log_z) - 1.0))));
+    const double y = z1 + (tops_n - 1);  // what the others are beside the first: log(1 + y) to y's own precision
+    double log_z = y * (1.0 - y * (0.5 - y * (1.0 / 3)));
+    if (y > 1e-4) {  // (and a step of Newton's method)
+      log_z = log1pf((float)y);
+      log_z += (1.0 + y) * exp_neg(-log_z) - 1.0;
+    }
+    sample_bookkeep(a.s, b, (int)~(unsigned)at, (float)(d - log_z));
   }
 }
 

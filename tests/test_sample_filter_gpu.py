@@ -290,3 +290,19 @@ def test_one_launch_or_two(K, B, V):
             for j in range(2):
                 assert torch.equal(outs[i][j].cpu(), want[i][j])
                 outs[i][j].fill_(-7)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("top", [None, math.inf])
+def test_not_numbers_among_more_entries_than_the_list_holds(K, f32, top):
+    """NaN is -inf where top-k's bin is looked for, where weights are counted, and beside infinite entries."""
+    g = torch.Generator().manual_seed(21)
+    B, V = 5, 9000
+    x = torch.randn(B, V, generator=g) * 2
+    x[torch.rand(B, V, generator=g) < 0.4] = math.nan
+    if top is not None:
+        x[torch.rand(B, V, generator=g) < 0.3] = top  # thousands
+    x = x if f32 else x.bfloat16()
+    for opts in (dict(top_k=250), dict(top_k=700, top_p=0.6), dict(top_k=2000), dict(top_p=0.9), dict()):
+        for T in (0.8, 5.0):
+            _same(K, x, torch.rand(B, generator=g), temperature=T, **opts)
