@@ -22,9 +22,9 @@
 // into such bins with their weights; a border (of top-k, top-p or u) falls into one bin, and that bin's entries are sorted. If even
 // those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
 //
-// Measured: one row of 32064 10 us in one launch (3.9 + 5.7 in two), 32 of 128256 (bf16, 8 MB) 7.7 + 9.4, 128 of them in fp32 with settings
+// Measured: one row of 32064 11 us in one launch (3.9 + 5.7 in two), 32 of 128256 (bf16, 8 MB) 8.0 + 9.9, 128 of them in fp32 with settings
 // of their own (66 MB) 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait
-// for one another; 33 flat rows of 50257 6 + 50: 16 us weigh 40000 entries or so on one CU (vector instructions), 10 a border (search,
+// for one another; 33 flat rows of 50257 6 + 52: 16 us weigh 40000 entries or so on one CU (vector instructions), 10 a border (search,
 // read, sort). Several workgroups a row for that took a quarter of its time and twice as much again for handing over.
 #include "common.h"
 #include "sample.h"
