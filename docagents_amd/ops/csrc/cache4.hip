@@ -163,6 +163,10 @@ DA_EXPORT int da_cache4_read(void* ck, void* cks, void* cv, void* cvs, int Hkv, 
 //                           8 keys, as bytes of two elements, and row c of tile i is element (D / 16) c + i
 // The order in which a product takes its elements and keys is that of the bytes in memory: nothing is transposed, and the
 // keys' order spreads a wave's reads of V over all LDS banks.
+// The weights P keep 24 bits: a head has three columns of them where there are places (G <= 5), 8 bits each, or two (G <= 8); each
+// column's lane has the same scores and cuts its own piece off them, and the pieces' outputs and sums are added in fp32. More heads (two
+// products a tile, the second with what the first left) and two columns: 16 bits. Rounded to 8 bits they were off by up to 2^-8 of
+// sum p |v|, as much as the output's own rounding.
 // A wave walks 64 keys at a time, copied by LDS-DMA (1 KiB an instruction, rows past the end are zeros) into two places of its
 // own: a place is filled again as soon as its codes are in registers, with counted waits and no barrier.
 struct Attn4 {
@@ -280,7 +284,13 @@ __device__ __forceinline__ void read_v4(unsigned at, unsigned at_s, unsigned (&v
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int D, bool W>
+// Columns of a head's weights; 1: two products
+__host__ __device__ constexpr int columns4(int G) { return G <= 5 ? 3 : G <= 8 ? 2 : 1; }
+
+__device__ __forceinline__ unsigned upper(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+__device__ __forceinline__ float less_upper(float x, unsigned mask) { return x - __uint_as_float(__float_as_uint(x) & mask); }
+
+template <int D, bool W, int NC>  // NC: columns4
 __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   constexpr int CH = D / 32, VB = D / 32, NT = D / 16, RB = D / 2, KT = 64;
   constexpr int ST = 1, ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4, STAGE = 2 * HALF;  // DMA instructions, bytes of K or V
@@ -305,10 +315,12 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   }
   char* mine = ring + w * ST * STAGE;
 
+  const int piece = NC > 1 ? (c >= G) + (NC > 2 && c >= 2 * G) : 0, cg = c - piece * G;  // the column's piece of its head's weights
+  const unsigned cut0 = piece > 0 ? 0xffff0000u : 0u, cut1 = piece > 1 ? 0xffff0000u : 0u;
   bf16x8_t qf[CH];
 #pragma unroll
   for (int t = 0; t < CH; ++t)
-    qf[t] = c < G && a.scale_log2e != 0.f ? *(const bf16x8_t*)(a.q + (long)b * a.ldq + (hk * G + c) * D + (f * CH + t) * 8) : bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    qf[t] = cg < G && a.scale_log2e != 0.f ? *(const bf16x8_t*)(a.q + (long)b * a.ldq + (hk * G + cg) * D + (f * CH + t) * 8) : bf16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
   // the scale is applied behind the largest score's choice: a positive one (q takes the sign, and the 0)
   const float scale = a.scale_log2e != 0.f ? fabsf(a.scale_log2e) : 1.f;
   const short flip = a.scale_log2e < 0.f ? (short)0x8000 : (short)0;
@@ -396,16 +408,21 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
     const float use = m == -INFINITY ? 0.f : m * scale;
-    unsigned pw[8];
+    unsigned pw[8], rest[NC == 1 ? 8 : 1];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[tt][i] = __builtin_amdgcn_exp2f(fmaf(s[tt][i], scale, -use));
         if constexpr (W) l += s[tt][i];
+        if constexpr (NC > 1) s[tt][i] = less_upper(s[tt][i], cut0);
+        if constexpr (NC > 2) s[tt][i] = less_upper(s[tt][i], cut1);
       }
-      pw[2 * tt] = pack_bf2(s[tt][0], s[tt][1]);
-      pw[2 * tt + 1] = pack_bf2(s[tt][2], s[tt][3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pw[2 * tt + h] = upper(__float_as_uint(s[tt][2 * h]), __float_as_uint(s[tt][2 * h + 1]));
+        if constexpr (NC == 1) rest[2 * tt + h] = pack_bf2(less_upper(s[tt][2 * h], 0xffff0000u), less_upper(s[tt][2 * h + 1], 0xffff0000u));
+      }
     }
     landed();
     const unsigned vt_at = (unsigned)(size_t)(lds_t)vt;
@@ -428,8 +445,14 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         if constexpr (VB > 3) vv[j][3] = bf2_of4<3>(word[j], scale_of(vs[j], (c * NT + 6) >> 5));
       }
       const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{pw[4 * hf], pw[4 * hf + 1], pw[4 * hf + 2], pw[4 * hf + 3]});
-      // the weights' sum as a product with ones, of the weights as they are rounded for V (the accumulated ones are divided by their own)
-      ol = mfma16(bf16x8_t{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80}, pb, ol);
+      // the weights' sum as a product with ones: of the pieces that V meets (the accumulated weights are divided by their own)
+      constexpr bf16x8_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
+      ol = mfma16(ones, pb, ol);
+      bf16x8_t pr;
+      if constexpr (NC == 1) {
+        pr = __builtin_bit_cast(bf16x8_t, u32x4_t{rest[4 * hf], rest[4 * hf + 1], rest[4 * hf + 2], rest[4 * hf + 3]});
+        ol = mfma16(ones, pr, ol);
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         u32x4_t va;
@@ -437,6 +460,7 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         for (int e = 0; e < 4; ++e)
           va[e] = __builtin_amdgcn_perm(vv[2 * e + 1][i >> 1], vv[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
         o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pb, o[i]);
+        if constexpr (NC == 1) o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pr, o[i]);
       }
     }
     stage = stage + 1 == ST ? 0 : stage + 1;
@@ -465,8 +489,14 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
 #pragma unroll
     for (int ww = 0; ww < 4; ++ww) {
       const float e = exp2f(sm[ww][g] - use);
-      acc += so[(ww * 16 + g) * (D + 1) + d] * e;
-      sum += sl[ww][g] * e;
+      float x = 0.f, y = 0.f;
+#pragma unroll
+      for (int j = NC - 1; j >= 0; --j) {
+        x += so[(ww * 16 + g + j * G) * (D + 1) + d];
+        y += sl[ww][g + j * G];
+      }
+      acc += x * e;
+      sum += y * e;
       if constexpr (W) sumw += slw[ww][g] * e;
     }
     const long at = ((long)b * a.H + hk * G + g) * a.nsplit + split;
@@ -571,8 +601,16 @@ DA_EXPORT size_t da_decode_attn4_ws(int B, int H, int D, int max_len, int nsplit
 template <int D>
 static int attn4(Attn4& a, hipStream_t st) {
   const dim3 grid(a.c.Hkv, a.B, a.nsplit);
-  if (a.weight) decode_attn4_kernel<D, true><<<grid, 256, 0, st>>>(a);
-  else decode_attn4_kernel<D, false><<<grid, 256, 0, st>>>(a);
+  const int nc = columns4(a.H / a.c.Hkv);
+  if (a.weight) {
+    if (nc == 3) decode_attn4_kernel<D, true, 3><<<grid, 256, 0, st>>>(a);
+    else if (nc == 2) decode_attn4_kernel<D, true, 2><<<grid, 256, 0, st>>>(a);
+    else decode_attn4_kernel<D, true, 1><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (nc == 3) decode_attn4_kernel<D, false, 3><<<grid, 256, 0, st>>>(a);
+    else if (nc == 2) decode_attn4_kernel<D, false, 2><<<grid, 256, 0, st>>>(a);
+    else decode_attn4_kernel<D, false, 1><<<grid, 256, 0, st>>>(a);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (a.weight || (a.nsplit > 1 && !a.cnt))
