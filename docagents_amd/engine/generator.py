@@ -36,6 +36,10 @@ class GenResult:
         self.tokens, self.mean_prob, self.n_tokens = tokens, mean_prob, n_tokens
 
 
+EVICT_AFTER = 16  # places of a slot that a prompt leaves to the steps, where sequences are shortened
+NOWHERE = -1 << 40  # the place of a row without a sequence: no step gets it to a slot's end
+
+
 class Generator:
     def __init__(self, model, max_batch: int = 64, max_seq: int = 4096, temperature: float = 0.2,
                  seed: int = 0, eos=(), use_graphs: bool = True, max_prefill_tokens: int = 65536,
@@ -61,9 +65,9 @@ class Generator:
             # one extra slot: the dummy slot for padded rows of a bucket
             model.alloc_cache(max_batch + 1, max_seq)
         self.cache = model.cache
-        # a model that shortens its sequences does so between steps, at most check_every of them apart: those that by then
-        # could be out of places
-        self.evict_above = self.cache.max_seq - check_every if model.kv_keep else 0
+        # a model that shortens its sequences does so before a step whose key has no place (``make_room``); a prompt leaves
+        # EVICT_AFTER places, so that as many steps have weighed its keys before any goes
+        self.evict_above = self.cache.max_seq - EVICT_AFTER if model.kv_keep else 0
         if model.kv_keep and not model.kv_keep < self.evict_above:
             raise ValueError(f"kv_keep={model.kv_keep}: slots of {self.cache.max_seq} places leave room for fewer "
                              f"than {max(0, self.evict_above)}")
@@ -124,10 +128,17 @@ class Generator:
         if n + max_new > most:
             raise ValueError(f"prompt of {n} tokens + {max_new} new exceeds the context ({most})")
 
-    def evict(self, st: DecodeState):
-        """Between steps, at most check_every of them apart: shorten the sequences that need it (models with kv_keep)."""
-        if self.evict_above:
-            self.model.evict(st, self.evict_above)
+    def make_room(self, st: DecodeState, at: np.ndarray):
+        """Before each decode step: the model shortens the sequences whose slot is full and that go on (models with kv_keep).
+        ``at`` is the host's count of where each row's next key goes, moved on here: what happens to a sequence depends on its
+        own steps only, not on how they are grouped. A row that has stopped on the device is behind its count and stays as it is."""
+        if not self.evict_above:
+            return
+        full = at == self.cache.max_seq
+        if full.any():
+            self.model.evict(st, self.cache.max_seq - 1)
+            at[full] = self.model.kv_keep
+        at += 1
 
     def _capture(self, st: DecodeState):
         # warm up on a side stream (allocator + lazy init), then capture one step
@@ -308,7 +319,7 @@ class Generator:
         except BaseException:
             self.cache.release(slots)
             raise
-        return _Wave(st, n, B, slots, max_new - 1)
+        return _Wave(st, n, B, slots, max_new - 1, plen)
 
     def _wave_decode(self, w: "_Wave"):
         """The wave's decode steps on the current stream (graph replays; the host checks every
@@ -323,6 +334,7 @@ class Generator:
             while done < steps:
                 k = min(self.check_every, steps - done)
                 for _ in range(k):
+                    self.make_room(st, w.at)
                     if st.graph is not None:
                         st.graph.replay()
                     else:
@@ -330,8 +342,6 @@ class Generator:
                     # padded rows never advance past the dummy slot's capacity
                 done += k
                 self.stats["decode_steps"] += k
-                if done < steps:
-                    self.evict(st)
                 if done < steps and int(st.active[:n].sum().item()) == 0:
                     break
                 if B > n:
@@ -456,11 +466,12 @@ class Generator:
 
 
 class _Wave:
-    __slots__ = ("st", "n", "B", "slots", "steps", "t0")
+    __slots__ = ("st", "n", "B", "slots", "steps", "t0", "at")
 
-    def __init__(self, st, n, B, slots, steps):
+    def __init__(self, st, n, B, slots, steps, plen):
         self.st, self.n, self.B, self.slots, self.steps = st, n, B, slots, steps
         self.t0 = None
+        self.at = plen.copy()  # Generator.make_room's count
 
 
 class ContinuousScheduler:
@@ -514,6 +525,7 @@ class ContinuousScheduler:
         self.buckets: dict[int, DecodeState] = {self.B: self.st}
         self.rows: list = [None] * self.B        # row -> (tag, slot, budget)
         self.left: list = [None] * self.B        # row -> decode steps it may still need (budget - 1 - steps run)
+        self.at = np.full(self.B, NOWHERE, dtype=np.int64)  # row -> Generator.make_room's count
         self.pending: collections.deque = collections.deque()
         self._reset_rows(list(range(self.B)))
         self.stats = {"admitted": 0, "finished": 0, "ticks": 0, "steps": 0, "head_hits": 0, "heads_built": 0}
@@ -561,8 +573,7 @@ class ContinuousScheduler:
             ahead: collections.deque = collections.deque()
             track = stop is not None and k > 1 and st.graph is not None
             while ran < k:
-                if ran % self.gen.check_every == 0:
-                    self.gen.evict(st)
+                self.gen.make_room(st, self.at)
                 if st.graph is not None:
                     st.graph.replay()
                 else:
@@ -737,6 +748,7 @@ class ContinuousScheduler:
         for r, (p, b, tag), sl, h in zip(rows, take, slots, hs):
             self.rows[r] = (tag, sl, int(b), h)
             self.left[r] = int(b) - 1  # the first token came from the prefill
+            self.at[r] = len(p)
         self.stats["admitted"] += n
         # a budget of one token (or an immediate EOS) finishes at prefill
         return self._reap(rows)
@@ -834,6 +846,7 @@ class ContinuousScheduler:
             self.gen.stats["decode_tokens"] += int(cnt)
             self.rows[r] = None
             self.left[r] = None
+            self.at[r] = NOWHERE
             slots.append(sl)
         self._reset_rows(fin)
         st.hist.index_fill_(0, idx, -1)

@@ -332,7 +332,8 @@ class LlamaDecoder:
 
     def evict(self, st: "DecodeState", above: int) -> None:
         """Shorten the rows of a decode state whose sequences have more than ``above`` keys to ``kv_keep`` (all layers; the
-        lengths follow, the positions go on). A row's length counts the token that the next step will write."""
+        lengths follow, the positions go on). A row's length counts the token that the next step will write. Keys go by the
+        attention of decode steps alone: a prompt's own attention collects no weights."""
         c = self.cache
         torch.sub(st.lens, 1, out=st.at)
         n = self.ops.cache4_evict(c.all, c.weight, st.at, st.slot, self.kv_keep, self.kv_recent, above=above)

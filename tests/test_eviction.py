@@ -1,0 +1,93 @@
+"""When sequences are shortened (a 4-bit cache with kv_keep), on the CPU: as soon as a slot is full and the sequence goes on, never
+before, whatever else runs beside it."""
+import pytest
+
+from docagents_amd.engine.generator import ContinuousScheduler, Generator
+from docagents_amd.models import make_decoder
+from docagents_amd.models.configs import DecoderConfig
+
+TINY = DecoderConfig("tiny-4", vocab=512, hidden=128, layers=2, heads=2, kv_heads=1, ffn=128, max_pos=512, rope_theta=1e4)
+KEEP = dict(kv_bits=4, kv_keep=20, kv_recent=8)
+SLOT = 64
+
+
+def _decoder(counts=None, **kw):
+    m = make_decoder(TINY, "cpu", seed=3, **kw)
+    inner = m.evict
+
+    def evict(st, above):
+        before = st.lens.clone()
+        inner(st, above)
+        counts.extend(int(n) - 1 for n in before[st.lens != before])
+    if counts is not None:
+        m.evict = evict
+    return m
+
+
+def _scheduler(cut, **kw):
+    m = _decoder(cut, **kw)
+    m.alloc_cache(6, SLOT)
+    return ContinuousScheduler(Generator(m, max_batch=2, max_seq=SLOT, temperature=0.0), B=2, max_new_cap=200)
+
+
+def _drain(s, steps, later=()):
+    """Tokens of each tag; ``later``: (tick, prompt, max_new, tag) that arrive while others run."""
+    out, tick = {}, 0
+    while s.busy() or any(t > tick for t, *_ in later):
+        for t, prompt, n, tag in later:
+            if t == tick:
+                s.submit(prompt, n, tag)
+        out.update({tag: r.tokens for tag, r in s.tick(steps)})
+        tick += 1
+    return out
+
+
+@pytest.mark.parametrize("steps", [1, 3, 5, 8, 16])
+@pytest.mark.parametrize("prompt", [[4] * 48, [5, 9, 2, 77, 31]])
+def test_what_fits_its_slot_is_not_shortened(steps, prompt):
+    """Prompt and answer together fill the slot to its last place."""
+    new = SLOT - len(prompt)
+    want = Generator(_decoder(kv_bits=4), max_batch=1, max_seq=SLOT, temperature=0.0).generate([prompt], new)[0]
+    cut = []
+    s = _scheduler(cut, **KEEP)
+    s.submit(prompt, new, 0)
+    assert _drain(s, steps)[0] == want.tokens and want.n_tokens == new and cut == []
+    assert Generator(_decoder(cut, **KEEP), max_batch=1, max_seq=SLOT, temperature=0.0).generate([prompt], new)[0].tokens == want.tokens
+    assert cut == []
+
+
+def test_shortened_as_its_own_steps_have_it():
+    """The same tokens whatever the ticks are, and with other requests that come and go beside it; each cut is of a full slot."""
+    prompt, new = [5, 9, 2, 77, 31], 150
+    cut = []
+    want = Generator(_decoder(cut, **KEEP), max_batch=1, max_seq=SLOT, temperature=0.0).generate([prompt], new)[0].tokens
+    assert len(want) == new and cut == [SLOT] * 3  # 5 + 149 keys: 64, then 44 more each time
+    for steps in (1, 3, 8, 16):
+        cut = []
+        s = _scheduler(cut, **KEEP)
+        s.submit(prompt, new, "a")
+        got = _drain(s, steps, [(2, [4] * 30, 11, "b"), (9, [8] * 48, 40, "c")])
+        assert got["a"] == want and len(got["b"]) == 11 and len(got["c"]) == 40
+        assert set(cut) == {SLOT}
+
+
+def test_one_token_more_than_the_slot_holds():
+    cut = []
+    m = _decoder(cut, **KEEP)
+    gen = Generator(m, max_batch=2, max_seq=SLOT, temperature=0.0)
+    # the last token's key is not written: SLOT + 1 tokens of prompt and answer fit
+    assert gen.generate([[4] * 40], SLOT + 1 - 40)[0].n_tokens == SLOT + 1 - 40 and cut == []
+    assert gen.generate([[4] * 40], SLOT + 2 - 40)[0].n_tokens == SLOT + 2 - 40 and cut == [SLOT]
+    assert all(int(st.lens.max()) <= SLOT + 1 for st in gen.states.values())
+
+
+def test_a_prompt_leaves_places_for_steps():
+    """16 decode steps have weighed a prompt's keys before any of them goes."""
+    cut = []
+    gen = Generator(_decoder(cut, **KEEP), max_batch=1, max_seq=SLOT, temperature=0.0, check_every=4)
+    with pytest.raises(ValueError, match="48 places"):
+        gen.generate([[4] * 49], 40)
+    gen.generate([[4] * 48], 17)
+    assert cut == []
+    gen.generate([[4] * 48], 18)
+    assert cut == [SLOT]
