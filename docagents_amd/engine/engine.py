@@ -201,8 +201,11 @@ class Engine:
         return v
 
     def context_budget(self, max_new: int) -> int:
-        most = self.gen.cache.max_seq - max_new - 8
-        return min(most, self.gen.evict_above) if self.gen.evict_above else most
+        """Tokens that a prompt may have beside ``max_new`` generated ones: both share a slot; where sequences are shortened the
+        prompt has a slot, less the places it leaves, and both share the model's positions."""
+        if self.gen.evict_above:
+            return min(self.gen.evict_above, self.dec_cfg.max_pos - max_new - 8)
+        return self.gen.cache.max_seq - max_new - 8
 
     def _answer_tail(self, question: str) -> str:
         return f"\nQuestion: {question}<|end|>\n<|assistant|>\n"

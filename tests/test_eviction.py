@@ -91,3 +91,39 @@ def test_a_prompt_leaves_places_for_steps():
     assert cut == []
     gen.generate([[4] * 48], 18)
     assert cut == [SLOT]
+
+
+# ------------------------------------------------------------------------------------------- through the engine
+def _engine(**kw):
+    from docagents_amd.engine.engine import Engine
+    return Engine("tiny-enc", "tiny-dec", "cpu", max_batch=2, max_new_tokens=6, summary_max_new=6, use_graphs=False, temperature=0.0, **kw)
+
+
+def test_an_engine_answers_past_its_slots():
+    """Slots of 512 places: 600 tokens of an answer behind a prompt that fills its slot up to the places it leaves. Without kv_keep
+    the same answer leaves no room for context."""
+    chunks = [[100 + i] * 40 for i in range(20)]
+    e = _engine(max_seq=512, **{**KEEP, "kv_keep": 128, "kv_recent": 32})
+    long, short = e.answer_prompt_ids("what?", chunks, 600), e.answer_prompt_ids("what?", chunks, 20)
+    assert long == short and 512 - 16 - 41 <= len(long) <= 512 - 16
+    cut, inner = [], e.decoder.evict
+
+    def evict(st, above):
+        cut.append(int(st.lens.max()) - 1)
+        inner(st, above)
+    e.decoder.evict = evict
+    assert len(e.answer_many([("what?", chunks, 0.5)], 600)) == 1
+    r = e.gen.generate([long], 600)[0]
+    # 600 tokens, or the model's end of answer before: cut as often as the slot was full
+    steps, n = r.n_tokens - 1, 0
+    at = len(long)
+    while at + steps > 512:
+        steps -= 512 - at
+        at, n = 128, n + 1
+    assert n >= 1 and cut == [512] * (2 * n)
+    # the positions bound both together
+    assert e.context_budget(4000) == 4096 - 4000 - 8
+    with pytest.raises(ValueError, match="context"):
+        e.gen.generate([long], 4096)
+    plain = _engine(max_seq=512, kv_bits=4)
+    assert plain.context_budget(600) < 0 and plain.context_budget(20) == 512 - 20 - 8
