@@ -39,7 +39,7 @@ _ENGINES = {}
 
 def local_engine(cfg: Config):
     """One in-process Engine per config (LLM_PROVIDER=local)."""
-    key = (cfg.embed_arch, cfg.llm_arch, cfg.llm_dtype, cfg.top_k, cfg.top_p, cfg.min_p, cfg.kv_bits, cfg.kv_keep, cfg.kv_recent)
+    key = (cfg.embed_arch, cfg.llm_arch, cfg.llm_dtype, cfg.top_k, cfg.top_p, cfg.min_p, cfg.kv_bits, cfg.kv_keep, cfg.kv_recent, cfg.max_seq)
     if key not in _ENGINES:
         import torch
         from .engine.engine import Engine
@@ -51,7 +51,7 @@ def local_engine(cfg: Config):
                                enc_dtype="fp8" if cfg.dtype == "fp8" else "bf16",
                                llm_dtype=cfg.llm_dtype, top_k=cfg.top_k, top_p=cfg.top_p, min_p=cfg.min_p,
                                kv_bits=cfg.kv_bits, kv_keep=cfg.kv_keep, kv_recent=cfg.kv_recent,
-                               max_seq=4096 if dev == "cuda" else 1024)
+                               max_seq=cfg.slot_keys(dev))
     return _ENGINES[key]
 
 

@@ -75,8 +75,11 @@ class Config:
     # 128 rows 40.6 q/s vs 64 rows 38.3 (profiles/r6/stack)
     max_batch: int = field(default=0, metadata={"env": "ENGINE_MAX_BATCH"})
     kv_cache_gb: float = field(default=0.0, metadata={"env": "KV_CACHE_GB"})  # 0 -> auto
+    # keys of a sequence that the decoder's cache holds; 0 = 4096 on a GPU, 1024 on a CPU (the model's positions at most)
+    max_seq: int = field(default=0, metadata={"env": "ENGINE_MAX_SEQ"})
     # keys and values of a Llama / Phi-3 decoder's cache: 16 (bf16) or 4 bits; with 4, KV_KEEP > 0 shortens a sequence that has
-    # filled its slot to that many keys a KV head (the KV_RECENT last ones and those attended to most)
+    # filled its slot (ENGINE_MAX_SEQ, then less than the model's positions) to that many keys a KV head: the KV_RECENT last ones
+    # and those that decode steps attended to most
     kv_bits: int = field(default=16, metadata={"env": "KV_BITS"})
     kv_keep: int = field(default=0, metadata={"env": "KV_KEEP"})
     kv_recent: int = field(default=0, metadata={"env": "KV_RECENT"})
@@ -151,6 +154,10 @@ class Config:
     ENGINE_DTYPES = ("bf16", "fp16", "fp8")
     LLM_DTYPES = ("bf16", "fp32")
 
+    def slot_keys(self, device_type: str) -> int:
+        """``Engine(max_seq=)`` of this configuration."""
+        return self.max_seq or (4096 if device_type == "cuda" else 1024)
+
     def validate_engine(self) -> "Config":
         """Startup check of the engine keys whose wrong value would otherwise silently run a
         different configuration (the engine process calls it before touching the GPU)."""
@@ -162,6 +169,8 @@ class Config:
             raise ValueError(f"KV_BITS={self.kv_bits} is not supported (4 | 16)")
         if self.kv_keep and (self.kv_bits != 4 or not 0 <= self.kv_recent <= self.kv_keep):
             raise ValueError(f"KV_KEEP={self.kv_keep}, KV_RECENT={self.kv_recent} need KV_BITS=4 and 0 <= KV_RECENT <= KV_KEEP")
+        if self.max_seq < 0:
+            raise ValueError(f"ENGINE_MAX_SEQ={self.max_seq}: want 0 (the default) or more")
         if self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1:
             raise ValueError(f"LLM_TOP_K={self.top_k}, LLM_TOP_P={self.top_p}, LLM_MIN_P={self.min_p}: want k >= 0, 0 < p <= 1, 0 <= min_p <= 1")
         if self.index_kind not in ("flat", "ivfflat"):

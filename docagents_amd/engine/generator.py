@@ -68,6 +68,9 @@ class Generator:
         # a model that shortens its sequences does so before a step whose key has no place (``make_room``); a prompt leaves
         # EVICT_AFTER places, so that as many steps have weighed its keys before any goes
         self.evict_above = self.cache.max_seq - EVICT_AFTER if model.kv_keep else 0
+        if model.kv_keep and self.cache.max_seq >= model.cfg.max_pos:
+            raise ValueError(f"kv_keep={model.kv_keep}: slots of {self.cache.max_seq} places hold all {model.cfg.max_pos} positions of "
+                             f"{model.cfg.name}, no sequence outgrows them (smaller ones: max_seq, ENGINE_MAX_SEQ)")
         if model.kv_keep and not model.kv_keep < self.evict_above:
             raise ValueError(f"kv_keep={model.kv_keep}: slots of {self.cache.max_seq} places leave room for fewer "
                              f"than {max(0, self.evict_above)}")

@@ -107,7 +107,7 @@ def main(argv=None) -> int:
                  kv_cache_gb=cfg.kv_cache_gb,
                  temperature=cfg.temperature, max_new_tokens=cfg.max_new_tokens,
                  summary_max_new=cfg.summary_max_new_tokens, index_kind=cfg.index_kind, ivf_lists=cfg.ivf_lists,
-                 ivf_probes=cfg.ivf_probes, max_seq=4096 if dev.type == "cuda" else 1024,
+                 ivf_probes=cfg.ivf_probes, max_seq=cfg.slot_keys(dev.type),
                  enc_dtype=cfg.dtype, llm_dtype=cfg.llm_dtype, top_k=cfg.top_k, top_p=cfg.top_p, min_p=cfg.min_p,
                  kv_bits=cfg.kv_bits, kv_keep=cfg.kv_keep, kv_recent=cfg.kv_recent)
     if cfg.engine_admit_tokens > 0:

@@ -127,3 +127,26 @@ def test_an_engine_answers_past_its_slots():
         e.gen.generate([long], 4096)
     plain = _engine(max_seq=512, kv_bits=4)
     assert plain.context_budget(600) < 0 and plain.context_budget(20) == 512 - 20 - 8
+
+
+def test_slots_that_hold_every_position_are_refused():
+    """No sequence outgrows them: the weights would be collected for nothing."""
+    for slot in (TINY.max_pos, 10 * TINY.max_pos):
+        with pytest.raises(ValueError, match="512 positions"):
+            Generator(_decoder(**KEEP), max_batch=1, max_seq=slot)
+    Generator(_decoder(**KEEP), max_batch=1, max_seq=TINY.max_pos - 1)
+    Generator(_decoder(kv_bits=4), max_batch=1, max_seq=TINY.max_pos)
+
+
+def test_slots_of_the_configuration(monkeypatch):
+    from docagents_amd import app
+    from docagents_amd.config import Config, load
+    assert Config().slot_keys("cuda") == 4096 and Config().slot_keys("cpu") == 1024
+    cfg = load({"ENGINE_MAX_SEQ": "256", "KV_BITS": "4", "KV_KEEP": "64", "KV_RECENT": "16", "EMBED_ARCH": "tiny-enc", "LLM_ARCH": "tiny-dec"})
+    assert cfg.validate_engine().slot_keys("cuda") == 256
+    with pytest.raises(ValueError, match="ENGINE_MAX_SEQ"):
+        Config().replace(max_seq=-1).validate_engine()
+    monkeypatch.setattr(app, "_ENGINES", {})
+    e = app.local_engine(cfg)
+    assert e.gen.cache.max_seq == 256 and e.gen.evict_above == 240
+    assert app.local_engine(cfg) is e and app.local_engine(cfg.replace(max_seq=300)) is not e
