@@ -167,7 +167,7 @@ class Config:
             raise ValueError(f"LLM_DTYPE={self.llm_dtype!r} is not supported (choose one of {', '.join(self.LLM_DTYPES)})")
         if self.kv_bits not in (4, 16):
             raise ValueError(f"KV_BITS={self.kv_bits} is not supported (4 | 16)")
-        if self.kv_keep and (self.kv_bits != 4 or not 0 <= self.kv_recent <= self.kv_keep):
+        if (self.kv_keep and self.kv_bits != 4) or not 0 <= self.kv_recent <= self.kv_keep:
             raise ValueError(f"KV_KEEP={self.kv_keep}, KV_RECENT={self.kv_recent} need KV_BITS=4 and 0 <= KV_RECENT <= KV_KEEP")
         if self.max_seq < 0:
             raise ValueError(f"ENGINE_MAX_SEQ={self.max_seq}: want 0 (the default) or more")

@@ -10,8 +10,8 @@ def make_decoder(cfg, device="cuda", seed: int = 0, tp=None, weights: dict | Non
         raise ValueError(f"{cfg.name}: dtype {dtype!r} is not supported ({', '.join(decoder_dtypes(cfg))})")
     if isinstance(cfg, HybridConfig):
         from .hybrid import HybridDecoder
-        if kv_bits != 16 or kv_keep:
-            raise ValueError(f"{cfg.name}: its caches are in the activations' type (kv_bits=16, kv_keep=0)")
+        if kv_bits != 16 or kv_keep or kv_recent:
+            raise ValueError(f"{cfg.name}: its caches are in the activations' type (kv_bits=16, kv_keep=0, kv_recent=0)")
         return HybridDecoder(cfg, device, seed=seed, tp=tp, weights=weights, dtype=dtype)
     from .llama import LlamaDecoder
     return LlamaDecoder(cfg, device, seed=seed, tp=tp, weights=weights, kv_bits=kv_bits, kv_keep=kv_keep, kv_recent=kv_recent)

@@ -278,12 +278,12 @@ class LlamaDecoder:
                  weights: dict | None = None, kv_bits: int = 16, kv_keep: int = 0, kv_recent: int = 0):
         """kv_bits: of the cache's keys and values (16: bf16; 4: ``ops.cache4``). kv_keep (4 bits only; 0: off): a sequence
         that fills its slot is shortened to that many keys a KV head, the ``kv_recent`` last ones and of the others those that
-        were attended to most, and goes on to the model's last position (``evict``)."""
+        decode steps attended to most, and goes on to the model's last position (``evict``)."""
         if kv_bits not in (4, 16):
             raise ValueError(f"kv_bits={kv_bits}: 4 or 16")
         if kv_bits == 4 and cfg.head_dim not in (64, 96, 128):
             raise ValueError(f"{cfg.name}: a 4-bit cache holds heads of 64, 96 or 128, not {cfg.head_dim}")
-        if kv_keep and (kv_bits != 4 or not 0 <= kv_recent <= kv_keep):
+        if (kv_keep and kv_bits != 4) or not 0 <= kv_recent <= kv_keep:
             raise ValueError(f"kv_keep={kv_keep}, kv_recent={kv_recent}: a 4-bit cache, 0 <= kv_recent <= kv_keep")
         self.kv_bits, self.kv_keep, self.kv_recent = kv_bits, kv_keep, kv_recent
         if kv_keep:  # a head's keys are not another sequence's to drop, and a step adds to the keys' weights

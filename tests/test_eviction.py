@@ -150,3 +150,16 @@ def test_slots_of_the_configuration(monkeypatch):
     e = app.local_engine(cfg)
     assert e.gen.cache.max_seq == 256 and e.gen.evict_above == 240
     assert app.local_engine(cfg) is e and app.local_engine(cfg.replace(max_seq=300)) is not e
+
+
+def test_recent_keys_without_a_number_to_keep_are_refused():
+    """They would be ignored."""
+    from docagents_amd.config import Config
+    from docagents_amd.models.configs import decoder_config
+    for kw in (dict(kv_recent=8), dict(kv_bits=4, kv_recent=8), dict(kv_bits=4, kv_recent=-1), dict(kv_bits=4, kv_keep=-4, kv_recent=-8)):
+        with pytest.raises(ValueError, match="KV_RECENT"):
+            Config().replace(**kw).validate_engine()
+        with pytest.raises(ValueError, match="kv_recent"):
+            make_decoder(TINY, "cpu", **kw)
+    with pytest.raises(ValueError, match="kv_recent"):
+        make_decoder(decoder_config("tiny-binupel"), "cpu", kv_recent=8)
