@@ -796,7 +796,16 @@ __device__ __attribute__((noinline)) unsigned collect_k(const __attribute__((add
 template <int NW>
 __device__ __forceinline__ u64 pick_few(PickLds& S, unsigned count, const RowOpts& o, float top, double it, double zt, double u) {
   const unsigned tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  auto sync = [] { if constexpr (NW > 1) __syncthreads(); };
+  // (a lone wave's lanes run together and its LDS accesses are in order: only the compiler has to keep them so)
+  auto sync = [] {
+    if constexpr (NW > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
   auto votes = [&](bool v, unsigned* red) {  // threads of the NW waves for which v
     const unsigned n = __popcll(__ballot(v));
     if constexpr (NW == 1) return n;
