@@ -1037,6 +1037,15 @@ DA_EXPORT size_t da_sample_filtered_ws(int B, int V) {
   return B * (chunks_of(V + SF_LEAD) * sizeof(ChunkSum) + groups_of(V + SF_LEAD) * (size_t)4);
 }
 
+static int workgroups_of(int V) { return (chunks_of(V + SF_LEAD) + SF_WG - 1) / SF_WG; }  // of a row, in one launch
+
+// Whether B rows go in one launch, and how many tickets (ints, 0) that takes: none where a workgroup has a whole row
+static bool one_launch(int B, int V) {
+  const int wgs = workgroups_of(V);
+  return wgs == 1 ? B <= SF_JOINED_ROWS : B * (long)wgs <= SF_JOINED;
+}
+DA_EXPORT int da_sample_filtered_tickets(int B, int V) { return workgroups_of(V) > 1 && one_launch(B, V) ? B : 0; }
+
 DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int ld, double T, double p, double m, int k,
                                  const void* Ts, const void* ps, const void* ms, const void* ks, const void* u, unsigned seed,
                                  unsigned step, const void* ctr, void* ws, void* tickets, void* out_tok, void* out_lp, void* conf, void* active,
@@ -1050,8 +1059,9 @@ DA_EXPORT int da_sample_filtered(const void* logits, int f32, int B, int V, int 
   FilterArgs a{T, p, m, (const float*)Ts, (const float*)ps, (const float*)ms, k, (const int*)ks, (const float*)u,
                (unsigned*)((char*)ws + (size_t)B * NC * sizeof(ChunkSum)), (ChunkSum*)ws, (int*)tickets, s};
   hipStream_t st = (hipStream_t)stream;
-  const int wgs = (NC + SF_WG - 1) / SF_WG;
-  if (wgs == 1 ? B <= SF_JOINED_ROWS : tickets && B * (long)wgs <= SF_JOINED) {
+  const int wgs = workgroups_of(V);
+  if (one_launch(B, V)) {
+    if (wgs > 1 && !tickets) return (int)hipErrorInvalidValue;
     if (f32) filter_pick_kernel<float, true><<<dim3(wgs, B), 1024, 0, st>>>(a);
     else filter_pick_kernel<bf16_t, true><<<dim3(wgs, B), 1024, 0, st>>>(a);
     DA_LAUNCH_CHECK();

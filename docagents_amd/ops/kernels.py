@@ -123,6 +123,7 @@ _SIGS = {
     "da_sample_filtered": [c_void_p] + [c_int] * 4 + [ctypes.c_double] * 3 + [c_int] + [c_void_p] * 5 + [c_uint, c_uint] + [c_void_p] * 11
                           + [c_int] * 5 + [c_void_p],
     "da_sample_filtered_ws": [c_int] * 2,
+    "da_sample_filtered_tickets": [c_int] * 2,
     "da_cache4_write": [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 4 + [c_int] + [c_void_p] * 5 + [c_int] * 6 + [c_void_p],
     "da_cache4_read": [c_void_p] * 4 + [c_int] * 6 + [c_void_p] * 3,
     "da_cache4_evict": [c_void_p] * 9 + [c_int] * 9 + [c_void_p],
@@ -134,7 +135,7 @@ _PART_OF = {n: "token" for n in (
     "da_quant_fp8_rows", "da_rmsnorm", "da_swiglu_interleaved", "da_layernorm", "da_layernorm_q", "da_layernorm_f16",
     "da_bert_embed_ln", "da_bert_embed_ln_q", "da_bert_embed_ln_f16", "da_embed", "da_pool_l2norm", "da_pool_l2norm_f16",
     "da_rope_cache", "da_sample", "da_sample_partial", "da_sample_chunked", "da_sample_finalize",
-    "da_sample_filtered", "da_sample_filtered_ws")}
+    "da_sample_filtered", "da_sample_filtered_ws", "da_sample_filtered_tickets")}
 _PART_OF |= {n: "cache4" for n in _SIGS if n.startswith(("da_cache4", "da_decode_attn4"))}
 
 
@@ -1549,7 +1550,6 @@ def sample(logits, temperature: float, seed: int, step: int = 0, out_tok=None, o
     return out_tok, out_lp
 
 
-FILTERED_WG = 8185  # entries of a row that one workgroup takes
 SAMPLE_FILTERED_MAX_V = 1 << 18  # entries of a row that sample_filtered takes (csrc/sample_filter.hip, SF_MAX_V)
 
 
@@ -1606,8 +1606,8 @@ def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, 
     e = (*eos[:4], -1, -1, -1, -1)
     L = lib()
     stream = _raw_stream()
-    nbytes, joined = _filtered_plan(B, V)
-    cnt = _counters(logits.device, stream).data_ptr() if joined else None
+    nbytes, tickets = _filtered_plan(B, V)
+    cnt = _counters(logits.device, stream).data_ptr() if tickets else None
     ws = _call_scratch(nbytes, logits)
     _check(L.da_sample_filtered(logits.data_ptr(), f32, B, V, ld, temperature, top_p, min_p, max(0, min(int(top_k), V)), Ts, ps, ms,
                                 ks, us, seed & 0xffffffff, step & 0xffffffff, _at(ctr), ws.data_ptr(), cnt, out_tok.data_ptr(),
@@ -1618,8 +1618,8 @@ def sample_filtered(logits, temperature, seed: int = 0, step: int = 0, top_k=0, 
 
 @_rule
 def _filtered_plan(B: int, V: int):
-    """(bytes of scratch, whether a row's workgroups may share a launch that needs counters)."""
-    return lib().da_sample_filtered_ws(B, V), V > FILTERED_WG and B * -(-V // FILTERED_WG) <= 64
+    """(bytes of scratch, counters of a launch that the workgroups of a row share: 0 for another)."""
+    return lib().da_sample_filtered_ws(B, V), lib().da_sample_filtered_tickets(B, V)
 
 
 def sample_partial(logits, temperature: float, seed: int, v0: int, step: int = 0, ctr=None, out=None):
