@@ -168,7 +168,7 @@ DA_EXPORT int da_cache4_read(void* ck, void* cks, void* cv, void* cvs, int Hkv, 
 // products a tile, the second with what the first left) and two columns: 16 bits. Rounded to 8 bits they were off by up to 2^-8 of
 // sum p |v|, as much as the output's own rounding.
 // A wave walks 64 keys at a time, copied by LDS-DMA (1 KiB an instruction, rows past the end are zeros) into two places of its
-// own: a place is filled again as soon as its codes are in registers, with counted waits and no barrier.
+// own, K's and V's: a place is filled again as soon as its codes are in registers, with counted waits and no barrier.
 struct Attn4 {
   const bf16_t* q;
   int ldq;
@@ -293,9 +293,9 @@ __device__ __forceinline__ float less_upper(float x, unsigned mask) { return x -
 template <int D, bool W, int NC>  // NC: columns4
 __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   constexpr int CH = D / 32, VB = D / 32, NT = D / 16, RB = D / 2, KT = 64;
-  constexpr int ST = 1, ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4, STAGE = 2 * HALF;  // DMA instructions, bytes of K or V
+  constexpr int ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4;  // DMA instructions, bytes of K or V
   typedef __attribute__((address_space(3))) void* lds_t;
-  constexpr int SO = 4 * 16 * (D + 1) * 4, RING = 4 * ST * STAGE;
+  constexpr int SO = 4 * 16 * (D + 1) * 4, RING = 4 * 2 * HALF;
   __shared__ __attribute__((aligned(16))) char ring[(SO > RING ? SO : RING) + 16];
   __shared__ float sm[4][16], sl[4][16], slw[W ? 4 : 1][16];
   __shared__ int last;
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     if ((unsigned)s < (unsigned)a.c.slots) head = row_of(a.c, s, hk, 0);
     else P = 0;
   }
-  char* mine = ring + w * ST * STAGE;
+  char *const kt = ring + w * 2 * HALF, *const vt = kt + HALF;
 
   const int piece = NC > 1 ? (c >= G) + (NC > 2 && c >= 2 * G) : 0, cg = c - piece * G;  // the column's piece of its head's weights
   const unsigned cut0 = piece > 0 ? 0xffff0000u : 0u, cut1 = piece > 1 ? 0xffff0000u : 0u;
@@ -342,8 +342,10 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(dst + i * 1024), 16, swizzled ? ko[i & 3] : (i * 64 + lane) * 16, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(dst + KT * RB), 4, lane * 4, 0, 0, 2);
   };
-  auto landed = [&]() __attribute__((always_inline)) {  // the oldest K or V; the three issued after it may be on their way
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * ST - 1) * PH) : "memory");
+  // the older of K and V; the other one's copies may be on their way. What else is (scores that are stored) makes it wait for more:
+  // never for less
+  auto landed = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PH) : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
   f32x4_t o[NT];
@@ -353,25 +355,19 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   float m = -INFINITY, l = 0.f;  // m of the scores before their scale
   const int kr = 4 * (c & 3) + (c >> 2);  // the lane's key of 16
 
-#pragma unroll
-  for (int i = 0; i < ST; ++i) {
-    issue(a.c.k, a.c.ks, true, kstart + (w + 4 * i) * KT, mine + i * STAGE);
-    issue(a.c.v, a.c.vs, false, kstart + (w + 4 * i) * KT, mine + i * STAGE + HALF);
-  }
+  issue(a.c.k, a.c.ks, true, kstart + w * KT, kt);
+  issue(a.c.v, a.c.vs, false, kstart + w * KT, vt);
 #pragma unroll
   for (int t = 0; t < CH; ++t) {
     qf[t] ^= bf16x8_t{flip, flip, flip, flip, flip, flip, flip, flip};
     asm volatile("" : "+v"(qf[t]));
   }
-  int stage = 0;
   for (int t0 = kstart + w * KT; t0 < kend; t0 += 4 * KT) {
-    char* kt = mine + stage * STAGE;
-    char* vt = kt + HALF;
     landed();
     unsigned kw[4][CH], ks[4];
     const unsigned kt_at = (unsigned)(size_t)(lds_t)kt;
     read_k4<D>(kt_at + kr * RB + (D == 128 ? ((f ^ (c & 3)) << 4) : f * CH * 4), kt_at + KT * RB + kr * 4, kw, ks);
-    issue(a.c.k, a.c.ks, true, t0 + 4 * ST * KT, kt);
+    issue(a.c.k, a.c.ks, true, t0 + 4 * KT, kt);
     f32x4_t s[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
@@ -432,7 +428,7 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
       const unsigned v_at = vt_at + f * RB + c * VB, s_at = vt_at + KT * RB + f * 4;
       if (hf) {
         read_v4<D, 1>(v_at, s_at, word, vs);
-        issue(a.c.v, a.c.vs, false, t0 + 4 * ST * KT, vt);
+        issue(a.c.v, a.c.vs, false, t0 + 4 * KT, vt);
       } else {
         read_v4<D, 0>(v_at, s_at, word, vs);
       }
@@ -463,7 +459,6 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         if constexpr (NC == 1) o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pr, o[i]);
       }
     }
-    stage = stage + 1 == ST ? 0 : stage + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (pieces past the end write zeros)
   if constexpr (W) {
