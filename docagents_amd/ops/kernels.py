@@ -2118,7 +2118,7 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     in their order, with their weights. lens / slot int32 [B]; the kept rows go to the front of the same slot, or of slots ``to``
     (then shorter sequences are copied too). What lies behind them is left as it was. Slots are distinct, and those of ``to``, and
     none of these is another row's slot. c and weight may have the layers in front. Returns the new lengths, int32 [B] (``out``: no part
-    of lens)."""
+    of lens, slot or to)."""
     layered = c.k.dim() == 5
     dev, Hkv, D, slots, max_seq, cache = _cache4(c, layered)
     B = lens.numel()
@@ -2128,7 +2128,8 @@ def cache4_evict(c: Cache4, weight, lens, slot, keep: int, recent: int, to=None,
     _req(0 <= recent <= keep <= above, "0 <= recent <= keep <= above")
     if out is None:
         out = torch.empty_like(lens)
-    oa = _ints(out, B, dev, "out"); _req(abs(oa - la) >= 4 * B, "out: int32 [B] apart from lens")
+    oa = _ints(out, B, dev, "out")
+    _req(min(abs(oa - la), abs(oa - sa), abs(oa - ta)) >= 4 * B, "out: int32 [B] apart from lens, slot and to")
     _check(lib().da_cache4_evict(*cache, wa, la, sa, ta, oa, c.k.shape[0] if layered else 1, B, Hkv, D, slots, max_seq,
                                  min(keep, max_seq), min(recent, max_seq), min(above, max_seq), _raw_stream()), "cache4_evict")
     return out
