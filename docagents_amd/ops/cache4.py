@@ -12,7 +12,7 @@ MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 class Cache4(NamedTuple):
     """Keys and values in 4 bits: codes uint8 [..., slots, Hkv, max_seq, D / 2] (element 2 j of a row in the low half of byte j;
     a code is a sign and one of ``MAGNITUDES``), scales uint8 [..., slots, Hkv, max_seq, 4], one for 32 elements along the head:
-    2^(byte - 127), 255 for a block that holds an inf or a NaN. A leading dimension is the layer (``layer`` takes one)."""
+    2^(byte - 127), 255 for a block that holds an inf or a NaN (elements from 1.75 2^127 on read as inf). A leading dimension is the layer (``layer`` takes one)."""
     k: torch.Tensor
     k_scale: torch.Tensor
     v: torch.Tensor

@@ -7,7 +7,8 @@
 // bf16, one conversion instruction makes two of them, and both products run on bf16 MFMA. Rows are whole and in order, so that
 // a token is written, read and moved by itself. 136 bytes a key and KV head of 128 for 512 in bf16.
 // Scale of a block with largest magnitude a = m 2^e (1 <= m < 2): 2^(e - 2) for m < 1.75 and 2^(e - 1) above it (6 stands for
-// up to 7 then): root mean square error 11.2 % of normal values, 11.5 % if the step is at m = 2 or 1.5.
+// up to 7 then): root mean square error 11.2 % of normal values, 11.5 % if the step is at m = 2 or 1.5. The smallest scale is 2^-126
+// (codes of it may be subnormal); an element of 1.75 2^127 or more is 2^128, which reads as inf.
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf2_t;

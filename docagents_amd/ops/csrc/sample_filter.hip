@@ -22,8 +22,12 @@
 // into such bins with their weights; a border (of top-k, top-p or u) falls into one bin, and that bin's entries are sorted. If even
 // those are too many (thousands of equal logits), the ordered 32-bit key is split by 11 bits a time.
 //
-// Measured: one row of 32064 11 us in one launch (3.9 + 5.7 in two), 32 of 128256 (bf16, 8 MB) 8.0 + 9.9, 128 of them in fp32 with settings
-// of their own (66 MB) 18.5 + 12 (the read at 3.6 TB/s, its start and end in it), latencies of launches and of some ten steps that wait
+// What the sums are off by, in weights of the largest entry: sorted rows V e^-44 (2e-14 at 2^18 entries) and the roundings of their
+// sums; counted ones V (2^-46 + e^-32), 7e-9 at 2^18 entries and 1e-9 at 50257: each weight is rounded to a unit, and entries 32 T below
+// the top are left out. A token is the definition's unless it lies that near to a border.
+//
+// Measured: one row of 32064 11 us in one launch (3.9 + 5.7 in two), 64 of 128256 (bf16, 16 MB) 8.0 + 9.9 (the read at 2.0 TB/s, its
+// start and end in it), 128 of them in fp32 with settings of their own (66 MB) 18.5 + 12 (3.6 TB/s), latencies of launches and of some ten steps that wait
 // for one another; 33 flat rows of 50257 6 + 52: 16 us weigh 40000 entries or so on one CU (vector instructions), 10 a border (search,
 // read, sort). Several workgroups a row for that took a quarter of its time and twice as much again for handing over.
 #include "common.h"
@@ -81,7 +85,7 @@ __device__ __forceinline__ float of_key(unsigned k);
 __device__ __forceinline__ float of_last(unsigned k) { return of_key(k - (k == 0x7fffffffu)); }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// e^a for a <= 0: 2^n by the exponent, e^r (|r| <= ln 2 / 2) by its series
+// e^a for a <= 0: a = n ln 2 + r with ln 2 in two parts (Cody and Waite's reduction), 2^n by the exponent, e^r (|r| <= ln 2 / 2) by its series
 __device__ __forceinline__ double exp_neg(double a) {
   const double n = rint(a * 1.4426950408889634);
   const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.69314718036912382, a));
