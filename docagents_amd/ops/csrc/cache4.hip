@@ -164,10 +164,10 @@ DA_EXPORT int da_cache4_read(void* ck, void* cks, void* cv, void* cvs, int Hkv, 
 //                           8 keys, as bytes of two elements, and row c of tile i is element (D / 16) c + i
 // The order in which a product takes its elements and keys is that of the bytes in memory: nothing is transposed, and the
 // keys' order spreads a wave's reads of V over all LDS banks.
-// The weights P keep 24 bits: a head has three columns of them where there are places (G <= 5), 8 bits each, or two (G <= 8); each
-// column's lane has the same scores and cuts its own piece off them, and the pieces' outputs and sums are added in fp32. More heads (two
-// products a tile, the second with what the first left) and two columns: 16 bits. Rounded to 8 bits they were off by up to 2^-8 of
-// sum p |v|, as much as the output's own rounding.
+// The weights P keep 16 bits, in two pieces of 8: where there are places (G <= 8) a head has two columns, whose lanes have the same
+// scores and take a piece each; with more heads the second piece has a product of its own. Pieces' outputs and sums are added in fp32.
+// In 8 bits weights were off by up to 2^-8 of sum p |v|, as much as the output's own rounding; a third column leaves nothing, at one
+// percent of the time more (64 x 8192 keys: 80.1 us in 8 bits, 81.8 in 16, 82.6 in 24).
 // A wave walks 64 keys at a time, copied by LDS-DMA (1 KiB an instruction, rows past the end are zeros) into two places of its
 // own, K's and V's: a place is filled again as soon as its codes are in registers, with counted waits and no barrier.
 struct Attn4 {
@@ -178,7 +178,6 @@ struct Attn4 {
   int B, H, max_len, nsplit, keys, ldo;
   float scale_log2e;
   float *po, *pm, *pl;  // of the splits
-  float* plw;           // their sums of unrounded weights, or null
   float* sc;            // scores [B, H, ld_sc] (log2; 16 keys as 4 f + i for 4 i + f), or null
   int ld_sc;
   float* weight;
@@ -285,20 +284,17 @@ __device__ __forceinline__ void read_v4(unsigned at, unsigned at_s, unsigned (&v
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Columns of a head's weights; 1: two products
-__host__ __device__ constexpr int columns4(int G) { return G <= 5 ? 3 : G <= 8 ? 2 : 1; }
+// The upper halves of two words: floats cut off to bf16
+__device__ __forceinline__ unsigned upper(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 
-__device__ __forceinline__ unsigned upper(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
-__device__ __forceinline__ float less_upper(float x, unsigned mask) { return x - __uint_as_float(__float_as_uint(x) & mask); }
-
-template <int D, bool W, int NC>  // NC: columns4
+template <int D, bool W, bool TWO>  // TWO: two columns a head
 __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   constexpr int CH = D / 32, VB = D / 32, NT = D / 16, RB = D / 2, KT = 64;
   constexpr int ND = KT * RB / 1024, PH = ND + 1, HALF = KT * RB + KT * 4;  // DMA instructions, bytes of K or V
   typedef __attribute__((address_space(3))) void* lds_t;
   constexpr int SO = 4 * 16 * (D + 1) * 4, RING = 4 * 2 * HALF;
   __shared__ __attribute__((aligned(16))) char ring[(SO > RING ? SO : RING) + 16];
-  __shared__ float sm[4][16], sl[4][16], slw[W ? 4 : 1][16];
+  __shared__ float sm[4][16], sl[4][16];
   __shared__ int last;
   const int hk = blockIdx.x, b = blockIdx.y, split = blockIdx.z, G = a.H / a.c.Hkv;
   const int L = len4(a, b), act = splits4(a, L);
@@ -316,8 +312,9 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   }
   char *const kt = ring + w * 2 * HALF, *const vt = kt + HALF;
 
-  const int piece = NC > 1 ? (c >= G) + (NC > 2 && c >= 2 * G) : 0, cg = c - piece * G;  // the column's piece of its head's weights
-  const unsigned cut0 = piece > 0 ? 0xffff0000u : 0u, cut1 = piece > 1 ? 0xffff0000u : 0u;
+  const bool second = TWO && c >= G;  // the column's piece of its head's weights
+  const int cg = second ? c - G : c;
+  const unsigned cut = second || !TWO ? 0xffff0000u : 0u;
   bf16x8_t qf[CH];
 #pragma unroll
   for (int t = 0; t < CH; ++t)
@@ -353,7 +350,7 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   f32x4_t ol = {0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // m of the scores before their scale
+  float m = -INFINITY;  // of the scores before their scale
   const int kr = 4 * (c & 3) + (c >> 2);  // the lane's key of 16
 
   issue(a.c.k, a.c.ks, true, kstart + w * KT, kt);
@@ -399,26 +396,22 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     if (__ballot(mx > m)) {  // (a new maximum is rare after the first tiles)
       const float mn = fmaxf(m, mx), alpha = exp2f((m - (mn == -INFINITY ? 0.f : mn)) * scale);
       m = mn;
-      if constexpr (W) l *= alpha;
       ol *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
     const float use = m == -INFINITY ? 0.f : m * scale;
-    unsigned pw[8], rest[NC == 1 ? 8 : 1];
+    unsigned pw[8], rest[TWO ? 1 : 8];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[tt][i] = __builtin_amdgcn_exp2f(fmaf(s[tt][i], scale, -use));
-        if constexpr (W) l += s[tt][i];
-        if constexpr (NC > 1) s[tt][i] = less_upper(s[tt][i], cut0);
-        if constexpr (NC > 2) s[tt][i] = less_upper(s[tt][i], cut1);
-      }
+      for (int i = 0; i < 4; ++i) s[tt][i] = __builtin_amdgcn_exp2f(fmaf(s[tt][i], scale, -use));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        pw[2 * tt + h] = upper(__float_as_uint(s[tt][2 * h]), __float_as_uint(s[tt][2 * h + 1]));
-        if constexpr (NC == 1) rest[2 * tt + h] = pack_bf2(less_upper(s[tt][2 * h], 0xffff0000u), less_upper(s[tt][2 * h + 1], 0xffff0000u));
+        const unsigned first = upper(s[tt][2 * h], s[tt][2 * h + 1]);
+        const float r0 = s[tt][2 * h] - __uint_as_float((first << 16) & cut), r1 = s[tt][2 * h + 1] - __uint_as_float(first & cut);
+        pw[2 * tt + h] = TWO ? upper(r0, r1) : first;
+        if constexpr (!TWO) rest[2 * tt + h] = upper(r0, r1);
       }
     }
     landed();
@@ -442,11 +435,11 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         if constexpr (VB > 3) vv[j][3] = bf2_of4<3>(word[j], scale_of(vs[j], (c * NT + 6) >> 5));
       }
       const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{pw[4 * hf], pw[4 * hf + 1], pw[4 * hf + 2], pw[4 * hf + 3]});
-      // the weights' sum as a product with ones: of the pieces that V meets (the accumulated weights are divided by their own)
+      // the weights' sum as a product with ones: of the pieces that V meets
       constexpr bf16x8_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
       ol = mfma16(ones, pb, ol);
       bf16x8_t pr;
-      if constexpr (NC == 1) {
+      if constexpr (!TWO) {
         pr = __builtin_bit_cast(bf16x8_t, u32x4_t{rest[4 * hf], rest[4 * hf + 1], rest[4 * hf + 2], rest[4 * hf + 3]});
         ol = mfma16(ones, pr, ol);
       }
@@ -457,19 +450,14 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
         for (int e = 0; e < 4; ++e)
           va[e] = __builtin_amdgcn_perm(vv[2 * e + 1][i >> 1], vv[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
         o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pb, o[i]);
-        if constexpr (NC == 1) o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pr, o[i]);
+        if constexpr (!TWO) o[i] = mfma16(__builtin_bit_cast(bf16x8_t, va), pr, o[i]);
       }
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (pieces past the end write zeros)
-  if constexpr (W) {
-    l += __shfl_xor(l, 16, 64);
-    l = sum_xhalf(l);
-  }
   if (f == 0) {
     sm[w][c] = m * scale;
     sl[w][c] = ol[0];
-    if constexpr (W) slw[w][c] = l;
   }
   __syncthreads();  // every wave is done with its places
   float* so = (float*)ring;  // [4][16][D + 1]
@@ -481,19 +469,18 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
   for (int i = tid; i < G * D; i += 256) {
     const int g = i / D, d = i - g * D;
     const float M = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g])), use = M == -INFINITY ? 0.f : M;
-    float acc = 0.f, sum = 0.f, sumw = 0.f;
+    float acc = 0.f, sum = 0.f;
 #pragma unroll
     for (int ww = 0; ww < 4; ++ww) {
       const float e = exp2f(sm[ww][g] - use);
       float x = 0.f, y = 0.f;
 #pragma unroll
-      for (int j = NC - 1; j >= 0; --j) {
+      for (int j = TWO; j >= 0; --j) {
         x += so[(ww * 16 + g + j * G) * (D + 1) + d];
         y += sl[ww][g + j * G];
       }
       acc += x * e;
       sum += y * e;
-      if constexpr (W) sumw += slw[ww][g] * e;
     }
     const long at = ((long)b * a.H + hk * G + g) * a.nsplit + split;
     if (act == 1) a.out[(long)b * a.ldo + (hk * G + g) * D + d] = f2bf(L ? acc / sum : 0.f);
@@ -501,7 +488,6 @@ __global__ void __launch_bounds__(256, 4) decode_attn4_kernel(Attn4 a) {
     if (d == 0) {
       put4(a.pm + at, M);
       put4(a.pl + at, sum);
-      if constexpr (W) a.plw[at] = sumw;
     }
   }
   if (act == 1 || !a.cnt) return;
@@ -560,7 +546,7 @@ __global__ void __launch_bounds__(256) decode_attn4_join_kernel(Attn4 a) {
   for (int g = tid >> 4; g < G; g += 16) {  // 16 lanes a head
     float M = -INFINITY, sum = 0.f;
     for (int x = tid & 15; x < act; x += 16) {
-      const float m = a.pm[first + (long)g * a.nsplit + x], l = a.plw[first + (long)g * a.nsplit + x], mx = fmaxf(M, m);
+      const float m = a.pm[first + (long)g * a.nsplit + x], l = a.pl[first + (long)g * a.nsplit + x], mx = fmaxf(M, m);
       sum = sum * exp2f(M - mx) + l * exp2f(m - mx);
       M = mx;
     }
@@ -591,21 +577,19 @@ __global__ void __launch_bounds__(256) decode_attn4_join_kernel(Attn4 a) {
 }
 
 DA_EXPORT size_t da_decode_attn4_ws(int B, int H, int D, int max_len, int nsplit, int weight) {
-  return 4 * ((size_t)B * H * ((nsplit * (D + 3) + 3) / 4 * 4) + (weight ? (size_t)B * H * ((max_len + 63) / 64 * 64) : 0));
+  return 4 * ((size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4) + (weight ? (size_t)B * H * ((max_len + 63) / 64 * 64) : 0));
 }
 
 template <int D>
 static int attn4(Attn4& a, hipStream_t st) {
   const dim3 grid(a.c.Hkv, a.B, a.nsplit);
-  const int nc = columns4(a.H / a.c.Hkv);
+  const bool two = a.H / a.c.Hkv <= 8;
   if (a.weight) {
-    if (nc == 3) decode_attn4_kernel<D, true, 3><<<grid, 256, 0, st>>>(a);
-    else if (nc == 2) decode_attn4_kernel<D, true, 2><<<grid, 256, 0, st>>>(a);
-    else decode_attn4_kernel<D, true, 1><<<grid, 256, 0, st>>>(a);
+    if (two) decode_attn4_kernel<D, true, true><<<grid, 256, 0, st>>>(a);
+    else decode_attn4_kernel<D, true, false><<<grid, 256, 0, st>>>(a);
   } else {
-    if (nc == 3) decode_attn4_kernel<D, false, 3><<<grid, 256, 0, st>>>(a);
-    else if (nc == 2) decode_attn4_kernel<D, false, 2><<<grid, 256, 0, st>>>(a);
-    else decode_attn4_kernel<D, false, 1><<<grid, 256, 0, st>>>(a);
+    if (two) decode_attn4_kernel<D, false, true><<<grid, 256, 0, st>>>(a);
+    else decode_attn4_kernel<D, false, false><<<grid, 256, 0, st>>>(a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
@@ -620,10 +604,10 @@ DA_EXPORT int da_decode_attn4(const void* q, int ldq, void* ck, void* cks, void*
                               int keys, float scale, void* ws, void* weight, void* out, int ldo, void* counters, void* stream) {
   if (Hkv < 1 || H % Hkv || H / Hkv > 16 || max_len < 1 || max_len > max_seq || nsplit < 1 || nsplit > 65535 || keys < 1 || B > 65535) return (int)hipErrorInvalidValue;
   if (B == 0) return 0;
-  const size_t n = (size_t)B * H * nsplit, all = (size_t)B * H * ((nsplit * (D + 3) + 3) / 4 * 4);
+  const size_t n = (size_t)B * H * nsplit, all = (size_t)B * H * ((nsplit * (D + 2) + 3) / 4 * 4);
   Attn4 a{(const bf16_t*)q, ldq, {(uint8_t*)ck, (uint8_t*)cks, (uint8_t*)cv, (uint8_t*)cvs, slots, Hkv, max_seq},
           (const int*)lens, (const int*)slot, (const int*)pre, B, H, max_len, nsplit, keys, ldo, scale * 1.44269504f,
-          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), (float*)ws + n * (D + 2), weight ? (float*)ws + all : nullptr,
+          (float*)ws, (float*)ws + n * D, (float*)ws + n * (D + 1), weight ? (float*)ws + all : nullptr,
           (max_len + 63) / 64 * 64, (float*)weight, (bf16_t*)out, weight ? nullptr : (int*)counters};
   hipStream_t st = (hipStream_t)stream;
   return D == 64 ? attn4<64>(a, st) : D == 96 ? attn4<96>(a, st) : D == 128 ? attn4<128>(a, st) : (int)hipErrorInvalidValue;

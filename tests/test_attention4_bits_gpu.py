@@ -1,8 +1,8 @@
 """The bits that attention over the 4-bit cache keeps of its weights (csrc/cache4.hip), against the oracle in 64 bits.
 
 Tolerance. Keys, values and queries are exact in bf16. A weight is 2^x of a score summed in fp32: with |score| <= 64 its relative
-error is 64 * 2^-22 at most, 2e-5 with the exponential's own. It meets the values in pieces of 8 bits: three of them leave nothing,
-two 2^-16 of it (cut off) or 2^-17 (rounded). Sums in fp32 over the products of a wave, some dozen of them, and their join: 64 *
+error is 64 * 2^-22 at most, 2e-5 with the exponential's own. It meets the values in two pieces of 8 bits, cut off: 2^-16 of it
+is left. Sums in fp32 over the products of a wave, some dozen of them, and their join: 64 *
 2^-24 = 4e-6. So what is rounded to the output is within t = 2 (2e-5 + 2^-16 + 4e-6) sum p |v| < 1e-4 sum p |v| of exact (the sum of the
 weights has the same errors), and the output between the roundings of exact - t and of exact + t. Weights of 8 bits are off by up to
 39e-4 sum p |v|."""
